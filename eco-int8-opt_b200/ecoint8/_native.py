@@ -7,6 +7,7 @@ CPU path: a CPU tensor, a missing library or a non-sm_100 device raises
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import pathlib
 import threading
@@ -64,6 +65,29 @@ class Fp32Hyper(ctypes.Structure):
                 ("weight_decay", c_d), ("grad_clip", c_d), ("bc1", c_d), ("bc2", c_d), ("seed", c_u64)]
 
 
+class Logits(ctypes.Structure):
+    """``eco_logits_t``."""
+
+    _fields_ = [("x", c_p), ("type", c_i32), ("pad_", c_i32), ("n0", c_i64), ("n1", c_i64), ("s0", c_i64),
+                ("s1", c_i64), ("cols", c_i64), ("mul", c_d)]
+
+
+class Grad(ctypes.Structure):
+    """``eco_grad_t``."""
+
+    _fields_ = [("g", c_p), ("s0", c_i64), ("s1", c_i64)]
+
+
+class SavedI8(ctypes.Structure):
+    """``eco_saved_i8_t``."""
+
+    _fields_ = [("q", c_p), ("scale", c_p), ("ld_q", c_i64), ("ld_scale", c_i64)]
+
+
+F32, BF16, F16, I8 = 0, 1, 2, 3
+TYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16, torch.int8: I8}
+_LP, _GP, _SP = ctypes.POINTER(Logits), ctypes.POINTER(Grad), ctypes.POINTER(SavedI8)
+
 # name -> (restype, argtypes); one line per entry point of the header
 _SIGS = {
     "eco_abi_version": (c_i32, []),
@@ -109,6 +133,20 @@ _SIGS = {
     "eco_quantize_dynamic_f32": (c_i32, [c_p, c_i64, c_i64, c_i64, c_p, c_p, c_i64, c_p, c_p]),
     "eco_fp32_eco_step": (c_i32, [ctypes.POINTER(Fp32Layer), c_i32, ctypes.POINTER(Fp32Hyper), c_p, c_i64, c_p]),
     "eco_fp32_eco_scratch_len": (c_i64, [ctypes.POINTER(Fp32Layer), c_i32]),
+    "eco_token_logp": (c_i32, [_LP, c_p, c_p, c_p, c_i64, c_p, c_p, c_p, c_p, c_p]),
+    "eco_token_grad": (c_i32, [_LP, c_p, c_p, c_p, c_p, c_d, _GP, c_p]),
+    "eco_policy_grad": (c_i32, [_LP, c_p, c_p, c_p, c_p, c_p, c_d, c_d, c_d, c_d, c_d, c_p, c_p, c_p, _GP, c_p]),
+    "eco_policy_tokens": (c_i32, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_p, c_p, c_d, c_d, c_d, c_d, c_p, c_p, c_p]),
+    "eco_preference_pairs": (c_i32, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_p, c_i64, c_i64, c_i32, c_d, c_d, c_i32,
+                                     c_d, c_p, c_p, c_p, c_p, c_p, c_p]),
+    "eco_ckpt_pack": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, _SP, c_p]),
+    "eco_ckpt_restore": (c_i32, [_SP, c_i32, c_i64, c_i64, c_p, c_i64, c_p]),
+    "eco_gated_act": (c_i32, [c_p, c_i64, c_p, c_i64, c_i32, c_i32, c_i64, c_i64, c_p, c_i64, _SP, _SP, c_p]),
+    "eco_gated_act_bwd": (c_i32, [c_p, c_i64, c_i32, c_i32, c_i64, c_i64, _SP, _SP, c_p, c_i64, c_p, c_i64, c_p]),
+    "eco_rms_norm": (c_i32, [c_p, c_i64, c_i32, c_i64, c_i64, c_p, c_i32, c_d, c_p, c_i64, _SP, c_p, c_p]),
+    "eco_rms_norm_bwd_scratch": (c_i64, [c_i64, c_i64]),
+    "eco_rms_norm_bwd": (c_i32, [c_p, c_i64, c_i32, c_i64, c_i64, c_p, c_i32, _SP, c_p, c_p, c_i64, c_p, c_p, c_i64,
+                                 c_p]),
 }
 
 _lib = None
@@ -181,6 +219,16 @@ def stream() -> int:
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device(dev: torch.device):
+    """A context in which ``dev`` is the current device (nothing to do when it is already)."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return _SAME_DEVICE
+    return torch.cuda.device(dev)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

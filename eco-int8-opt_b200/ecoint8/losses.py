@@ -1,0 +1,380 @@
+"""Post-training objectives on a model's logits, with their gradients.
+
+The reference's one objective is cross entropy (``ecoint8.quant.cross_entropy_grad_i8``
+here); these stand beside it, and need the log-probability of one given token per row:
+
+* ``token_logprobs``: the log-probabilities (what old and reference policies are asked for);
+* ``policy_loss``: clipped policy loss with a KL term against a reference;
+* ``preference_loss``: a loss over pairs of log ratios (preferred against rejected sequences).
+
+Each loss has two forms.  ``*_loss_grad`` returns the loss and the gradient with respect to
+the logits in one call, as ``cross_entropy_grad_i8`` does: for loops that feed a gradient to
+``backward_i8`` themselves (int8 logits with their scale ``s_out``; the gradient is fp32,
+with respect to the dequantized logits, for ``quantize_tensor_dynamic``) and for CUDA-graph
+capture.  ``*_loss`` is differentiable: its backward reads the logits again and computes the
+probabilities anew, so nothing of the logits' size is kept.
+
+Logits are ``[rows, vocab]`` or ``[batch, length, vocab]``, fp32, bf16, fp16 or int8, with any
+row strides (``logits[:, :-1]`` is read in place) as long as the vocabulary is contiguous.
+Rows with a false ``mask`` or a token outside ``[0, vocab)`` (such as -100) do not count: their
+logits are not read and may hold anything, and their gradient is zero.  Sums over rows are
+taken in fp64 and in a fixed order: the same call gives the same bits.  A row of infinities or
+NaN that counts makes its results NaN.  The gradient of ``logits[b, t]`` starts at the same
+address modulo 16 bytes as that row, so gradients may come with padded strides.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import NamedTuple
+
+import torch
+
+from . import _native as nat
+
+_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+
+
+class PolicyLoss(NamedTuple):
+    """``loss``, ``kl`` (mean of the KL term) and ``clip_fraction``: 0-dim fp32 on the device;
+    ``grad``: the logits' gradient (None from ``policy_loss``); ``logp``: fp32 per token, 0
+    where a row does not count."""
+
+    loss: torch.Tensor
+    grad: torch.Tensor | None
+    logp: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+class PreferenceLoss(NamedTuple):
+    """``loss``: 0-dim fp32; ``grad``: the logits' gradient (None from ``preference_loss``);
+    ``log_ratio`` fp32 ``[2 pairs]``: each sequence's sum (or mean) of ``logp - ref_logp``;
+    ``margin`` fp32 ``[pairs]``: ``beta`` times the preferred less the rejected one's."""
+
+    loss: torch.Tensor
+    grad: torch.Tensor | None
+    log_ratio: torch.Tensor
+    margin: torch.Tensor
+
+
+def _spec(x, mul):
+    n0, n1, s0, s1 = (1, x.shape[0], 0, x.stride(0)) if x.dim() == 2 else (*x.shape[:2], x.stride(0), x.stride(1))
+    return nat.Logits(x.data_ptr(), nat.TYPES[x.dtype], 0, n0, n1, s0, s1, x.shape[-1], mul)
+
+
+class _Rows:
+    """Logits as the kernels take them, with their tokens and mask."""
+
+    __slots__ = ("x", "spec", "lead", "rows", "tokens", "mask", "gain", "dev")
+
+    def __init__(self, logits, tokens, mask, temperature, s_out):
+        self.dev = nat.require_cuda(logits, tokens, mask)
+        if logits.dtype not in nat.TYPES or logits.dim() not in (2, 3):
+            raise AssertionError("logits must be fp32, bf16, fp16 or int8, [rows, vocab] or [batch, length, vocab]")
+        self.lead = lead = logits.shape[:-1]
+        if tokens.dtype != torch.int64 or tokens.shape != lead:
+            raise AssertionError(f"tokens must be int64 {list(lead)}, one per row of logits")
+        if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != lead):
+            raise AssertionError(f"mask must be bool {list(lead)}")
+        if logits.shape[-1] == 0:
+            raise AssertionError("an empty vocabulary")
+        temperature = float(temperature)
+        if not (temperature > 0.0 and math.isfinite(temperature)):
+            raise ValueError("temperature must be positive")
+        i8 = logits.dtype == torch.int8
+        if i8 != (s_out is not None):
+            raise ValueError("int8 logits need their scale s_out, and only they have one")
+        scale = float(s_out) if i8 else 1.0
+        if not (scale > 0.0 and math.isfinite(scale)):
+            raise ValueError("s_out must be positive")
+        x = logits if logits.stride(-1) == 1 or logits.shape[-1] == 1 else logits.contiguous()
+        self.x = x
+        self.gain = 1.0 / temperature
+        self.rows = tokens.numel()
+        self.spec = _spec(x, scale / temperature)
+        self.tokens = tokens.contiguous()
+        self.mask = None if mask is None else mask.contiguous()
+
+    def per_row(self, t, name):
+        """A per-token fp32 tensor in the rows' order (broadcast to the tokens' shape)."""
+        if t is None:
+            return None
+        nat.require_cuda(self.x, t)
+        if t.dtype != torch.float32:
+            raise AssertionError(f"{name} must be fp32")
+        if t.shape != self.lead:
+            try:
+                t = t.expand(self.lead)
+            except RuntimeError:
+                raise AssertionError(f"{name} must broadcast to {list(self.lead)}") from None
+        return t.contiguous()
+
+    def new_grad(self):
+        """``(tensor, eco_grad_t)``: rows that start like the logits' rows modulo 16 bytes."""
+        x, cols = self.x, self.x.shape[-1]
+        n0, n1 = self.spec.n0, self.spec.n1
+        if x.dtype == torch.int8:
+            dtype, per, want0, want1, skew = torch.float32, 4, 0, 0, 0
+        else:
+            dtype, per = x.dtype, 16 // x.element_size()
+            want0, want1, skew = self.spec.s0, self.spec.s1, x.data_ptr() % 16 // x.element_size()
+        s1 = cols + (want1 - cols) % per
+        s0 = n1 * s1 + (want0 - n1 * s1) % per if n0 > 1 else n1 * s1
+        if skew == 0 and s1 == cols and s0 == n1 * s1:
+            g = torch.empty(x.shape, dtype=dtype, device=x.device)
+        else:
+            shape, strides = ((n1, cols), (s1, 1)) if x.dim() == 2 else ((n0, n1, cols), (s0, s1, 1))
+            g = torch.empty(skew + n0 * s0, dtype=dtype, device=x.device).as_strided(shape, strides, skew)
+        return g, nat.Grad(g.data_ptr(), s0, s1)
+
+    def token_logp(self, logp=None, lp64=None, stats=None, coef=None, cu=None):
+        nat.call("eco_token_logp", ctypes.byref(self.spec), self.tokens.data_ptr(), nat.ptr(self.mask), nat.ptr(cu),
+                 0 if cu is None else cu.numel() - 1, nat.ptr(logp), nat.ptr(lp64), nat.ptr(stats), nat.ptr(coef),
+                 nat.stream())
+
+    def token_grad(self, stats, coef, scale=None):
+        with nat.on_device(self.dev):
+            g, spec = self.new_grad()
+            nat.call("eco_token_grad", ctypes.byref(self.spec), self.tokens.data_ptr(), stats.data_ptr(),
+                     coef.data_ptr(), nat.ptr(scale), self.gain, ctypes.byref(spec), nat.stream())
+        return g
+
+    def new(self, *shape, dtype=torch.float32):
+        return torch.empty(shape, dtype=dtype, device=self.dev)
+
+
+def _keep_rows(ctx, rows, stats, coef=None):
+    # The logits and tokens go through autograd's saved tensors (checked for changes in place,
+    # and open to hooks that move or pack them); the row statistics and coefficients are the
+    # kernels' own and stay as they are.
+    ctx.save_for_backward(rows.x, rows.tokens)
+    ctx.own = (rows.gain, rows.spec.mul, stats, coef)
+
+
+def _saved_rows(ctx):
+    """``(rows, stats, coef)``: the forward's rows over the tensors that autograd hands back."""
+    x, tokens = ctx.saved_tensors
+    gain, mul, stats, coef = ctx.own
+    rows = _Rows.__new__(_Rows)
+    rows.x = x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+    rows.tokens, rows.mask, rows.gain, rows.dev = tokens.contiguous(), None, gain, x.device
+    rows.lead, rows.rows = tokens.shape, tokens.numel()
+    rows.spec = _spec(rows.x, mul)
+    return rows, stats, coef
+
+
+# ------------------------------------------------------------------ log-probabilities
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, temperature, s_out):
+        rows = _Rows(logits, tokens, mask, temperature, s_out)
+        with nat.on_device(rows.dev):
+            logp = rows.new(*rows.lead)
+            stats = rows.new(rows.rows, 2) if ctx.needs_input_grad[0] else None
+            rows.token_logp(logp=logp, stats=stats)
+        if stats is not None:
+            _keep_rows(ctx, rows, stats)
+        return logp
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogp):
+        rows, stats, _ = _saved_rows(ctx)
+        return rows.token_grad(stats, dlogp.contiguous()), None, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, mask: torch.Tensor | None = None,
+                   temperature: float = 1.0, s_out: float | None = None) -> torch.Tensor:
+    """``log softmax(logits / temperature)`` at ``tokens``: fp32, the tokens' shape, 0 where a
+    row does not count.  Differentiable with respect to floating logits."""
+    return _TokenLogprobs.apply(logits, tokens, mask, temperature, s_out)
+
+
+# ------------------------------------------------------------------ policy loss
+
+
+def _policy_args(rows, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, denom):
+    old = rows.per_row(old_logp, "old_logp")
+    adv = rows.per_row(advantages, "advantages")
+    ref = rows.per_row(ref_logp, "ref_logp")
+    clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
+    if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
+        raise ValueError("clip_low must lie in [0, 1] and clip_high must not be negative")
+    if not math.isfinite(kl_coef):
+        raise ValueError("kl_coef must be finite")
+    if kl_coef != 0.0 and ref is None:
+        raise ValueError("a KL term needs ref_logp")
+    denom = 0.0 if denom is None else float(denom)
+    if denom < 0.0 or not math.isfinite(denom):
+        raise ValueError("denom must be positive")
+    keep = (old, adv, ref)
+    return keep, (old.data_ptr(), adv.data_ptr(), nat.ptr(ref), 1.0 - clip_low, 1.0 + clip_high, kl_coef, denom)
+
+
+def policy_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, *,
+                     ref_logp: torch.Tensor | None = None, mask: torch.Tensor | None = None, clip_low: float = 0.2,
+                     clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0,
+                     s_out: float | None = None, denom: float | None = None) -> PolicyLoss:
+    """Clipped policy loss with a KL term, and its gradient with respect to the logits.
+
+    Over the rows that count, with ``lp = token_logprobs(...)`` and ``r = exp(lp - old_logp)``::
+
+        loss = sum(max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high)) + kl_coef k) / denom
+        k    = exp(ref_logp - lp) - (ref_logp - lp) - 1
+
+    ``advantages`` (A), ``old_logp`` and ``ref_logp`` are fp32 and broadcast to the tokens' shape.
+    ``denom``: default the number of rows that count (at least 1); a caller that splits a batch
+    over steps or ranks gives the whole batch's.  No row that counts: loss and gradient 0.  One
+    read of the logits and one write of the gradient; no host synchronisation."""
+    rows = _Rows(logits, tokens, mask, temperature, s_out)
+    keep, args = _policy_args(rows, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, denom)
+    with nat.on_device(rows.dev):
+        g, spec = rows.new_grad()
+        logp, terms, out = rows.new(*rows.lead), rows.new(3, rows.rows), rows.new(3)
+        nat.call("eco_policy_grad", ctypes.byref(rows.spec), rows.tokens.data_ptr(), nat.ptr(rows.mask), *args,
+                 rows.gain, logp.data_ptr(), terms.data_ptr(), out.data_ptr(), ctypes.byref(spec), nat.stream())
+    loss, kl, clipped = out.unbind()
+    return PolicyLoss(loss, g, logp, kl, clipped)
+
+
+class _PolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, temperature, s_out, old_logp, advantages, ref_logp, *how):
+        rows = _Rows(logits, tokens, mask, temperature, s_out)
+        keep, args = _policy_args(rows, old_logp, advantages, ref_logp, *how)
+        with nat.on_device(rows.dev):
+            logp, out, coef = rows.new(*rows.lead), rows.new(3), rows.new(rows.rows)
+            lp64, stats = rows.new(rows.rows, dtype=torch.float64), rows.new(rows.rows, 2)
+            rows.token_logp(logp=logp, lp64=lp64, stats=stats)
+            nat.call("eco_policy_tokens", lp64.data_ptr(), rows.tokens.data_ptr(), nat.ptr(rows.mask), rows.rows,
+                     rows.x.shape[-1], *args, coef.data_ptr(), out.data_ptr(), nat.stream())
+        _keep_rows(ctx, rows, stats, coef)
+        loss, kl, clipped = out.unbind()
+        ctx.mark_non_differentiable(logp, kl, clipped)
+        ctx.set_materialize_grads(False)
+        return loss, logp, kl, clipped
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, *_):
+        if dloss is None:
+            return (None,) * 12
+        rows, stats, coef = _saved_rows(ctx)
+        return (rows.token_grad(stats, coef, dloss),) + (None,) * 11
+
+
+def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tensor, advantages: torch.Tensor, *,
+                ref_logp: torch.Tensor | None = None, mask: torch.Tensor | None = None, clip_low: float = 0.2,
+                clip_high: float = 0.2, kl_coef: float = 0.0, temperature: float = 1.0, s_out: float | None = None,
+                denom: float | None = None) -> PolicyLoss:
+    """``policy_loss_grad`` as a differentiable loss (``.grad`` is None; call ``.loss.backward()``).
+    Gradients flow to the logits alone."""
+    loss, logp, kl, clipped = _PolicyLoss.apply(logits, tokens, mask, temperature, s_out, old_logp, advantages,
+                                                ref_logp, clip_low, clip_high, kl_coef, denom)
+    return PolicyLoss(loss, None, logp, kl, clipped)
+
+
+# ------------------------------------------------------------------ preference loss
+
+
+def _preference_forward(rows, ref_logp, beta, kind, label_smoothing, average, cu_seqlens, denom):
+    ref = rows.per_row(ref_logp, "ref_logp")
+    if ref is None:
+        raise AssertionError("ref_logp must be given")
+    if kind not in _KINDS:
+        raise ValueError(f"kind must be one of {sorted(_KINDS)}")
+    beta, label_smoothing = float(beta), float(label_smoothing)
+    if not (beta > 0.0 and math.isfinite(beta)) or not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("beta must be positive and label_smoothing lie in [0, 1]")
+    if cu_seqlens is None:
+        if len(rows.lead) != 2 or rows.lead[0] % 2 or rows.lead[0] == 0:
+            raise AssertionError("logits must be [2 pairs, length, vocab], or packed rows with cu_seqlens")
+        pairs, seq_len = rows.lead[0] // 2, rows.lead[1]
+    else:
+        nat.require_cuda(rows.x, cu_seqlens)
+        if len(rows.lead) != 1:
+            raise AssertionError("with cu_seqlens, logits must be packed: [rows, vocab]")
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 3 or \
+                cu_seqlens.numel() % 2 == 0:
+            raise AssertionError("cu_seqlens must be int32 [2 pairs + 1]")
+        cu_seqlens = cu_seqlens.contiguous()
+        pairs, seq_len = cu_seqlens.numel() // 2, 0
+    denom = float(pairs) if denom is None else float(denom)
+    if not (denom > 0.0 and math.isfinite(denom)):
+        raise ValueError("denom must be positive")
+    n = rows.rows
+    wide = rows.new(n + pairs, dtype=torch.float64)  # log-probabilities, then each pair's loss
+    lp64, pair_loss = wide[:n], wide[n:]
+    stats, coef, out = rows.new(n, 2), rows.new(n), rows.new(3 * pairs + 1)
+    log_ratio, margin, loss = out[:2 * pairs], out[2 * pairs:3 * pairs], out[3 * pairs]
+    rows.token_logp(lp64=lp64, stats=stats, coef=coef, cu=cu_seqlens)
+    nat.call("eco_preference_pairs", lp64.data_ptr(), rows.tokens.data_ptr(), nat.ptr(rows.mask), n,
+             rows.x.shape[-1], ref.data_ptr(), nat.ptr(cu_seqlens), seq_len, pairs, _KINDS[kind], beta,
+             label_smoothing, int(bool(average)), denom, coef.data_ptr(), log_ratio.data_ptr(), margin.data_ptr(),
+             pair_loss.data_ptr(), loss.data_ptr(), nat.stream())
+    return stats, coef, loss, log_ratio, margin
+
+
+def preference_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: torch.Tensor, *, beta: float = 0.1,
+                         kind: str = "sigmoid", label_smoothing: float = 0.0, average: bool = False,
+                         mask: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None,
+                         temperature: float = 1.0, s_out: float | None = None,
+                         denom: float | None = None) -> PreferenceLoss:
+    """Loss over pairs of sequences, and its gradient with respect to the logits.
+
+    ``logits`` ``[2 pairs, length, vocab]``: the preferred sequences, then the rejected ones in
+    the same order; or packed ``[rows, vocab]`` with ``cu_seqlens`` int32 ``[2 pairs + 1]`` on the
+    device (rows outside ``[cu_seqlens[0], cu_seqlens[-1])`` do not count; offsets beyond the rows
+    are cut there).  ``ref_logp``: the reference's log-probability of each token
+    (``token_logprobs``).  With ``D`` a sequence's sum over its counting rows of ``logp - ref_logp``
+    (``average``: over their number; 0 for a sequence without any) and ``h = beta (D_preferred -
+    D_rejected)``::
+
+        sigmoid: -(1 - e) log sigmoid(h) - e log sigmoid(-h)     e = label_smoothing
+        hinge:   max(0, 1 - h)
+        ipo:     (h / beta - 1 / (2 beta))^2
+
+    (``label_smoothing`` belongs to ``sigmoid``; the others ignore it.)  ``loss``: the sum over the
+    pairs by ``denom``, by default their number.  A sequence's gradient needs all its rows, so
+    the logits are read twice."""
+    rows = _Rows(logits, tokens, mask, temperature, s_out)
+    with nat.on_device(rows.dev):
+        stats, coef, loss, log_ratio, margin = _preference_forward(rows, ref_logp, beta, kind, label_smoothing,
+                                                                   average, cu_seqlens, denom)
+        return PreferenceLoss(loss, rows.token_grad(stats, coef), log_ratio, margin)
+
+
+class _PreferenceLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, mask, temperature, s_out, *how):
+        rows = _Rows(logits, tokens, mask, temperature, s_out)
+        with nat.on_device(rows.dev):
+            stats, coef, loss, log_ratio, margin = _preference_forward(rows, *how)
+        _keep_rows(ctx, rows, stats, coef)
+        ctx.mark_non_differentiable(log_ratio, margin)
+        ctx.set_materialize_grads(False)
+        return loss, log_ratio, margin
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, *_):
+        if dloss is None:
+            return (None,) * 12
+        rows, stats, coef = _saved_rows(ctx)
+        return (rows.token_grad(stats, coef, dloss),) + (None,) * 11
+
+
+def preference_loss(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: torch.Tensor, *, beta: float = 0.1,
+                    kind: str = "sigmoid", label_smoothing: float = 0.0, average: bool = False,
+                    mask: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None,
+                    temperature: float = 1.0, s_out: float | None = None,
+                    denom: float | None = None) -> PreferenceLoss:
+    """``preference_loss_grad`` as a differentiable loss (``.grad`` is None; call
+    ``.loss.backward()``).  Gradients flow to the logits alone."""
+    loss, log_ratio, margin = _PreferenceLoss.apply(logits, tokens, mask, temperature, s_out, ref_logp, beta, kind,
+                                                    label_smoothing, average, cu_seqlens, denom)
+    return PreferenceLoss(loss, None, log_ratio, margin)

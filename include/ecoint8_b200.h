@@ -439,6 +439,119 @@ ECO_API int eco_fp32_eco_step(const eco_fp32_layer_t* layers, int n_layers, cons
 /* The scratch length (doubles) eco_fp32_eco_step needs for these layers (<= 0 on bad input). */
 ECO_API int64_t eco_fp32_eco_scratch_len(const eco_fp32_layer_t* layers, int n_layers);
 
+/* ------------------------------------------- objectives on token log-probabilities --
+ * No counterpart in the reference, whose one objective is cross entropy (above).  Logits
+ * [n0, n1, cols] with row strides s0, s1 (elements) and unit column stride; their rows are
+ * numbered n1 * i0 + i1, and tokens, mask and every per-row array have n0 * n1 values in
+ * that order.  x = raw * mul (1 / temperature; int8 logits: also their scale).  A row counts
+ * when its mask byte is nonzero (mask nullable) and its token lies in [0, cols); other rows
+ * are not read, have log-probability 0 and zeros as gradient.  Fewer than 2^31 rows, at most
+ * 2^28 columns. */
+enum { ECO_F32 = 0, ECO_BF16 = 1, ECO_F16 = 2, ECO_I8 = 3 };
+enum { ECO_PREFERENCE_SIGMOID = 0, ECO_PREFERENCE_HINGE = 1, ECO_PREFERENCE_IPO = 2 };
+
+typedef struct {
+  const void* x;
+  int32_t type; /* ECO_F32 .. ECO_I8 */
+  int32_t pad_;
+  int64_t n0, n1, s0, s1, cols;
+  double mul;
+} eco_logits_t;
+
+/* The gradient's rows: the logits' type (fp32 for int8 logits), row strides in elements.
+ * Every row has to start where the logits' row starts modulo 16 bytes (on 16 bytes for int8
+ * logits). */
+typedef struct {
+  void* g;
+  int64_t s0, s1;
+} eco_grad_t;
+
+/* lp = x_token - log sum exp x, for each row: fp32 and / or fp64 (either nullable).
+ * row_stats (nullable): float [rows, 2] for eco_token_grad.  coef_zero (nullable): float
+ * [rows], set to zeros.  cu_seqlens (nullable): int32 [num_seqs + 1]; rows outside
+ * [cu_seqlens[0], cu_seqlens[num_seqs]) do not count. */
+ECO_API int eco_token_logp(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
+                           const int32_t* cu_seqlens, int64_t num_seqs, float* logp, double* logp64,
+                           float* row_stats, float* coef_zero, eco_stream_t stream);
+
+/* g_j = c ([j = token] - softmax(x)_j), c = coef[row] * gain * *scale (scale nullable). */
+ECO_API int eco_token_grad(const eco_logits_t* logits, const int64_t* tokens, const float* row_stats,
+                           const float* coef, const float* scale, double gain, const eco_grad_t* grad,
+                           eco_stream_t stream);
+
+/* Clipped policy loss with a KL term, over the rows that count (n of them; denom > 0
+ * replaces max(n, 1)):
+ *   r = exp(lp - old);  l = max(-A r, -A clip(r, low, high)) + kl_coef k
+ *   k = exp(ref - lp) - (ref - lp) - 1  (0 without ref_logp)
+ * out[0..2] = sum l / denom, sum k / denom, share of rows whose clipped term is the larger.
+ * eco_policy_grad does all of it from the logits in two launches: logp [rows], terms float
+ * [3, rows] (workspace), the gradient times gain.  eco_policy_tokens starts from fp64
+ * log-probabilities and leaves each row's d loss / d lp in coef (for eco_token_grad). */
+ECO_API int eco_policy_grad(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
+                            const float* old_logp, const float* adv, const float* ref_logp, double low,
+                            double high, double kl_coef, double denom, double gain, float* logp, float* terms,
+                            float* out, const eco_grad_t* grad, eco_stream_t stream);
+ECO_API int eco_policy_tokens(const double* logp64, const int64_t* tokens, const uint8_t* mask, int64_t rows,
+                              int64_t cols, const float* old_logp, const float* adv, const float* ref_logp,
+                              double low, double high, double kl_coef, double denom, float* coef, float* out,
+                              eco_stream_t stream);
+
+/* Preference loss over `pairs` pairs of sequences, the preferred ones first: sequence q has
+ * rows [q seq_len, (q + 1) seq_len), or [cu_seqlens[q], cu_seqlens[q + 1]) where cu_seqlens
+ * (int32 [2 pairs + 1]) is given.  D_q = sum over its counting rows of lp - ref (average: over
+ * their number); h = beta (D_p - D_{p + pairs}).  sigmoid: -(1 - e) log s(h) - e log s(-h);
+ * hinge: max(0, 1 - h); ipo: (h / beta - 1 / (2 beta))^2; out[0] = their sum / denom.
+ * log_ratio [2 pairs] = D, margin [pairs] = h, pair_loss [pairs] (workspace); coef: each
+ * counting row's d loss / d lp (other rows are left as they are). */
+ECO_API int eco_preference_pairs(const double* logp64, const int64_t* tokens, const uint8_t* mask, int64_t rows,
+                                 int64_t cols, const float* ref_logp, const int32_t* cu_seqlens, int64_t seq_len,
+                                 int64_t pairs, int kind, double beta, double label_smoothing, int average,
+                                 double denom, float* coef, float* log_ratio, float* margin, double* pair_loss,
+                                 float* out, eco_stream_t stream);
+
+/* ---------------------------------------- activations kept in eight bits ----------
+ * A row is kept in blocks of ECO_CKPT_BLOCK columns: scale = amax / 127, q = rint(x * (127 /
+ * amax)), each step one fp32 rounding; the block stands for q * scale.  amax < 2^-119: zeros; an
+ * infinity or NaN in the block: NaN throughout.  q rows start on 16 bytes.  Matrices are
+ * ECO_F32, ECO_BF16 or ECO_F16; inputs have any row stride and alignment; outputs have rows
+ * that start on 16 bytes and are padded to whole 16-byte vectors (the padding is written). */
+#define ECO_CKPT_BLOCK 128
+enum { ECO_ACT_SILU = 0, ECO_ACT_GELU = 1 };
+
+typedef struct {
+  int8_t* q;      /* [rows, ld_q], ld_q a multiple of 16 */
+  float* scale;   /* [rows, ld_scale] */
+  int64_t ld_q, ld_scale;
+} eco_saved_i8_t;
+
+ECO_API int eco_ckpt_pack(const void* x, int type, int64_t rows, int64_t cols, int64_t ld,
+                          const eco_saved_i8_t* saved, eco_stream_t stream);
+ECO_API int eco_ckpt_restore(const eco_saved_i8_t* saved, int type, int64_t rows, int64_t cols, void* x,
+                             int64_t ld, eco_stream_t stream);
+
+/* y = act(gate) * up (silu, or gelu by the error function); gate and up are kept in saved_*
+ * (both or neither nullable).  The backward reads them: dup = dy act(gate), dgate = dy up
+ * act'(gate); its outputs may be halves of one matrix (any alignment; nothing past column
+ * `cols` is written). */
+ECO_API int eco_gated_act(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int type, int act,
+                          int64_t rows, int64_t cols, void* y, int64_t ld_y, const eco_saved_i8_t* saved_gate,
+                          const eco_saved_i8_t* saved_up, eco_stream_t stream);
+ECO_API int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int act, int64_t rows, int64_t cols,
+                              const eco_saved_i8_t* saved_gate, const eco_saved_i8_t* saved_up, void* dgate,
+                              int64_t ld_dgate, void* dup, int64_t ld_dup, eco_stream_t stream);
+
+/* y = x rstd w, rstd = 1 / sqrt(mean x^2 + eps) (w nullable: ones; its type fp32 or x's); x is
+ * kept in `saved` and rstd in fp32 [rows] (both nullable).  Backward, with u = kept x * rstd:
+ * dx = rstd (w dy - u mean(w dy u)); dw (nullable, w's type, contiguous) = sum over rows of
+ * dy u.  scratch: eco_rms_norm_bwd_scratch floats on 16 bytes, when dw is wanted. */
+ECO_API int eco_rms_norm(const void* x, int64_t ld, int type, int64_t rows, int64_t cols, const void* w, int w_type,
+                         double eps, void* y, int64_t ld_y, const eco_saved_i8_t* saved, float* rstd,
+                         eco_stream_t stream);
+ECO_API int64_t eco_rms_norm_bwd_scratch(int64_t rows, int64_t cols);
+ECO_API int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t rows, int64_t cols, const void* w,
+                             int w_type, const eco_saved_i8_t* saved, const float* rstd, void* dx, int64_t ld_dx,
+                             void* dw, float* scratch, int64_t scratch_len, eco_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
