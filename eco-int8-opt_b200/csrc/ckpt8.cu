@@ -131,6 +131,20 @@ ECO_DEV float block_amax(const float (&f)[8]) {
   for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
   return m;
 }
+// Gains of N blocks of a half-warp from their maxima, and in lane i (< N) the scale of block i:
+// lane i does block i's two divisions, so that N blocks cost the divisions of one.
+template <int N>
+ECO_DEV float block_gains(const float (&amax)[N], float (&gain)[N]) {
+  const int lane = threadIdx.x & (kLanes - 1);
+  float m = amax[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = lane == i ? amax[i] : m;
+  const bool zero = m < 0x1p-119f;  // false for NaN
+  const float g = zero ? 0.0f : __fdiv_rn(127.0f, m);
+#pragma unroll
+  for (int i = 0; i < N; ++i) gain[i] = N == 1 ? g : __shfl_sync(0xffffffffu, g, i, kLanes);
+  return zero ? 0.0f : (m < INFINITY ? __fdiv_rn(m, 127.0f) : __int_as_float(0x7fc00000));
+}
 // rint(x * gain) of eight values as bytes.  Adding 1.5 * 2^23 rounds to nearest even at the
 // unit, and leaves the whole number's low byte as the sum's low byte.
 ECO_DEV uint2 quant8(const float (&f)[8], float gain) {
@@ -146,27 +160,6 @@ ECO_DEV void dequant8(uint2 q, float (&f)[8]) {
   for (int i = 0; i < 8; ++i)
     f[i] = __uint_as_float(__byte_perm(w[i / 4], 0x4B000000u, 0x7440u | (uint32_t)(i & 3))) - 8388736.0f;
 }
-// Puts eight columns of a block away; all 16 lanes of the block call it.
-ECO_DEV void put8(const float (&f)[8], int n, int8_t* q, int64_t c, float* scale) {
-  const float amax = block_amax(f);
-  const bool zero = amax < 0x1p-119f;  // false for NaN
-  const float gain = zero ? 0.0f : __fdiv_rn(127.0f, amax);
-  if (n > 0) __stcs(reinterpret_cast<uint2*>(q + c), quant8(f, gain));
-  if ((threadIdx.x & (kLanes - 1)) == 0 && n > 0)
-    *scale = zero ? 0.0f : (amax < INFINITY ? __fdiv_rn(amax, 127.0f) : __int_as_float(0x7fc00000));
-}
-ECO_DEV void get8(const int8_t* q, int64_t c, int n, const float* scale, float (&f)[8]) {
-  uint2 w = make_uint2(0u, 0u);
-  float s = 0.0f;
-  if (n > 0) {
-    w = __ldcs(reinterpret_cast<const uint2*>(q + c));
-    s = __ldg(scale);
-  }
-  dequant8(w, f);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] *= s;
-}
-
 // ------------------------------------------------ matrices
 struct Mat {  // rows of any type; two leading dimensions collapse to one
   void* p;
@@ -197,37 +190,88 @@ struct Tile {
     b_step = (int64_t)gridDim.x << bpr_log2;
   }
 };
-// Loops over (row, block) so that both halves of a warp stay in step (the shuffles need all
-// 32 lanes): `body(row, block, first column, columns of this lane)`, no columns past the end.
-template <typename F>
-ECO_DEV void for_blocks(int64_t rows, int64_t cols, int bpr_log2, F body) {
+// Loops over (row, block) in groups of U rows, whose loads are all issued before the first is
+// used (a thread has one or two 16-byte loads per row: alone they would not cover the memory's
+// latency).  Both halves of a warp stay in step (the shuffles need all 32 lanes): lanes past the
+// last row or column get n = 0 columns.  load(r, c, n) -> L;  use(L[U], r[U], n[U], b, c).
+template <int U, typename L, typename Load, typename Use>
+ECO_DEV void for_blocks(int64_t rows, int64_t cols, int bpr_log2, Load load, Use use) {
   const Tile t(cols, bpr_log2);
   const int64_t first = (int64_t)blockIdx.y * (kHalves >> bpr_log2), firstb = (int64_t)blockIdx.x << bpr_log2;
-  for (int64_t r = t.row0, rr = first; rr < rows; r += t.row_step, rr += t.row_step)
+  for (int64_t r0 = t.row0, rr = first; rr < rows; r0 += U * t.row_step, rr += U * t.row_step)
     for (int64_t b = t.b0, bb = firstb; bb < t.blocks; b += t.b_step, bb += t.b_step) {
       const int64_t c = b * kBlock + t.lane * 8;
-      const int n = r < rows && b < t.blocks ? left8(cols, c) : 0;
-      body(r, b, c, n);
+      L l[U];
+      int64_t r[U];
+      int n[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        r[u] = r0 + u * t.row_step;
+        n[u] = r[u] < rows && b < t.blocks ? left8(cols, c) : 0;
+        if (n[u] == 0) r[u] = 0;
+        l[u] = load(r[u], c, n[u]);
+      }
+      use(l, r, n, b, c);
     }
 }
 
 // ------------------------------------------------ put away, bring back
-template <typename T>
+template <typename T, int U>
 __global__ void __launch_bounds__(kThreads) pack_kernel(Mat x, int64_t rows, int64_t cols, Saved S, int bpr_log2) {
-  for_blocks(rows, cols, bpr_log2, [&](int64_t r, int64_t b, int64_t c, int n) {
-    float f[8];
-    unpack8(load8(static_cast<const T*>(x.p) + (n ? r * x.ld : 0), c, n), f);
-    put8(f, n, S.q + r * S.ld_q, c, S.scale + r * S.ld_s + b);
-  });
+  for_blocks<U, Oct<T>>(
+      rows, cols, bpr_log2,
+      [&](int64_t r, int64_t c, int n) { return load8(static_cast<const T*>(x.p) + r * x.ld, c, n); },
+      [&](const Oct<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
+        float f[8], amax[U], gain[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          unpack8(o[u], f);
+          amax[u] = block_amax(f);
+        }
+        const float scale = block_gains(amax, gain);
+        const int lane = threadIdx.x & (kLanes - 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          unpack8(o[u], f);
+          if (n[u] > 0) __stcs(reinterpret_cast<uint2*>(S.q + r[u] * S.ld_q + c), quant8(f, gain[u]));
+          // the scale's lane may lie past the last column: the block's first lane knows
+          const bool live = __shfl_sync(0xffffffffu, n[u], 0, kLanes) > 0;
+          const int64_t row = __shfl_sync(0xffffffffu, (long long)r[u], 0, kLanes);
+          if (lane == u && live) S.scale[row * S.ld_s + b] = scale;
+        }
+      });
 }
 
-template <typename T>
+struct Eights {
+  uint2 q;
+  float s;
+};
+ECO_DEV Eights fetch8(const Saved& S, int64_t r, int64_t c, int n) {
+  Eights e{make_uint2(0u, 0u), 0.0f};
+  if (n > 0) {
+    e.q = __ldcs(reinterpret_cast<const uint2*>(S.q + r * S.ld_q + c));
+    e.s = __ldg(S.scale + r * S.ld_s + c / kBlock);
+  }
+  return e;
+}
+ECO_DEV void values8(const Eights& e, float (&f)[8]) {
+  dequant8(e.q, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] *= e.s;
+}
+
+template <typename T, int U>
 __global__ void __launch_bounds__(kThreads) restore_kernel(Saved S, int64_t rows, int64_t cols, Mat x, int bpr_log2) {
-  for_blocks(rows, cols, bpr_log2, [&](int64_t r, int64_t b, int64_t c, int n) {
-    float f[8];
-    get8(S.q + r * S.ld_q, c, n, S.scale + r * S.ld_s + b, f);
-    if (n > 0) store8(static_cast<T*>(x.p) + r * x.ld, c, n, true, f);
-  });
+  for_blocks<U, Eights>(
+      rows, cols, bpr_log2, [&](int64_t r, int64_t c, int n) { return fetch8(S, r, c, n); },
+      [&](const Eights(&e)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float f[8];
+          values8(e[u], f);
+          if (n[u] > 0) store8(static_cast<T*>(x.p) + r[u] * x.ld, c, n[u], true, f);
+        }
+      });
 }
 
 // ------------------------------------------------ gated activation
@@ -245,64 +289,115 @@ ECO_DEV float act_slope(float g, float s) {
   return s * fmaf(g, 1.0f - s, 1.0f);
 }
 
-template <typename T, bool GELU>
+template <typename T>
+struct OctPair {
+  Oct<T> a, b;
+};
+
+template <typename T, bool GELU, int U>
 __global__ void __launch_bounds__(kThreads)
     gated_fwd_kernel(Mat gate, Mat up, int64_t rows, int64_t cols, Mat y, Saved SG, Saved SU, int bpr_log2) {
-  for_blocks(rows, cols, bpr_log2, [&](int64_t r, int64_t b, int64_t c, int n) {
-    const int64_t rr = n ? r : 0;
-    const Oct<T> go = load8(static_cast<const T*>(gate.p) + rr * gate.ld, c, n);
-    const Oct<T> uo = load8(static_cast<const T*>(up.p) + rr * up.ld, c, n);
-    float g[8], u[8];
-    unpack8(go, g);
-    unpack8(uo, u);
-    if (SG.q) {
-      put8(g, n, SG.q + r * SG.ld_q, c, SG.scale + r * SG.ld_s + b);
-      put8(u, n, SU.q + r * SU.ld_q, c, SU.scale + r * SU.ld_s + b);
-    }
+  for_blocks<U, OctPair<T>>(
+      rows, cols, bpr_log2,
+      [&](int64_t r, int64_t c, int n) {
+        return OctPair<T>{load8(static_cast<const T*>(gate.p) + r * gate.ld, c, n),
+                          load8(static_cast<const T*>(up.p) + r * up.ld, c, n)};
+      },
+      [&](const OctPair<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
+        const int lane = threadIdx.x & (kLanes - 1);
+        if (SG.q) {
+          float f[8], amax[2 * U], gain[2 * U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) g[i] = g[i] * act_over_input<GELU>(g[i]) * u[i];
-    if (n > 0) store8(static_cast<T*>(y.p) + r * y.ld, c, n, true, g);
-  });
+          for (int u = 0; u < U; ++u) {
+            unpack8(o[u].a, f);
+            amax[2 * u] = block_amax(f);
+            unpack8(o[u].b, f);
+            amax[2 * u + 1] = block_amax(f);
+          }
+          const float scale = block_gains(amax, gain);
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            if (n[u] > 0) {
+              unpack8(o[u].a, f);
+              __stcs(reinterpret_cast<uint2*>(SG.q + r[u] * SG.ld_q + c), quant8(f, gain[2 * u]));
+              unpack8(o[u].b, f);
+              __stcs(reinterpret_cast<uint2*>(SU.q + r[u] * SU.ld_q + c), quant8(f, gain[2 * u + 1]));
+            }
+            const bool live = __shfl_sync(0xffffffffu, n[u], 0, kLanes) > 0;
+            const int64_t row = __shfl_sync(0xffffffffu, (long long)r[u], 0, kLanes);
+            if (lane == 2 * u && live) SG.scale[row * SG.ld_s + b] = scale;
+            if (lane == 2 * u + 1 && live) SU.scale[row * SU.ld_s + b] = scale;
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float g[8], v[8];
+          unpack8(o[u].a, g);
+          unpack8(o[u].b, v);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) g[i] = g[i] * act_over_input<GELU>(g[i]) * v[i];
+          if (n[u] > 0) store8(static_cast<T*>(y.p) + r[u] * y.ld, c, n[u], true, g);
+        }
+      });
 }
 
-template <typename T, bool GELU>
+template <typename T>
+struct GatedIn {
+  Oct<T> dy;
+  Eights g, u;
+};
+
+template <typename T, bool GELU, int U>
 __global__ void __launch_bounds__(kThreads)
     gated_bwd_kernel(Mat dy, int64_t rows, int64_t cols, Saved SG, Saved SU, Mat dgate, Mat dup, bool vec_g,
                      bool vec_u, int bpr_log2) {
-  for_blocks(rows, cols, bpr_log2, [&](int64_t r, int64_t b, int64_t c, int n) {
-    const Oct<T> d8 = load8(static_cast<const T*>(dy.p) + (n ? r * dy.ld : 0), c, n);
-    float g[8], u[8], d[8];
-    get8(SG.q + r * SG.ld_q, c, n, SG.scale + r * SG.ld_s + b, g);
-    get8(SU.q + r * SU.ld_q, c, n, SU.scale + r * SU.ld_s + b, u);
-    unpack8(d8, d);
+  for_blocks<U, GatedIn<T>>(
+      rows, cols, bpr_log2,
+      [&](int64_t r, int64_t c, int n) {
+        return GatedIn<T>{load8(static_cast<const T*>(dy.p) + r * dy.ld, c, n), fetch8(SG, r, c, n),
+                          fetch8(SU, r, c, n)};
+      },
+      [&](const GatedIn<T>(&in)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float s = act_over_input<GELU>(g[i]);
-      const float dg = d[i] * u[i] * act_slope<GELU>(g[i], s);
-      u[i] = d[i] * g[i] * s;
-      g[i] = dg;
-    }
-    if (n > 0) {
-      store8(static_cast<T*>(dgate.p) + r * dgate.ld, c, n, vec_g && n == 8, g);
-      store8(static_cast<T*>(dup.p) + r * dup.ld, c, n, vec_u && n == 8, u);
-    }
-  });
+        for (int u = 0; u < U; ++u) {
+          float g[8], v[8], d[8];
+          values8(in[u].g, g);
+          values8(in[u].u, v);
+          unpack8(in[u].dy, d);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float s = act_over_input<GELU>(g[i]);
+            const float dg = d[i] * v[i] * act_slope<GELU>(g[i], s);
+            v[i] = d[i] * g[i] * s;
+            g[i] = dg;
+          }
+          if (n[u] > 0) {
+            store8(static_cast<T*>(dgate.p) + r[u] * dgate.ld, c, n[u], vec_g && n[u] == 8, g);
+            store8(static_cast<T*>(dup.p) + r[u] * dup.ld, c, n[u], vec_u && n[u] == 8, v);
+          }
+        }
+      });
 }
 
 // ------------------------------------------------ rms norm
 // y = x r w,  r = 1 / sqrt(mean x^2 + eps);  with x' = what the eight bits stand for, u = x' r:
 //   dx = r (w dy - u mean(w dy u)),   dw = sum over rows of dy u.
 //
-// NT threads hold a row (CH groups of eight columns each), so a row is read once; the sum is
-// joined over the threads in a fixed order.  Rows wider than that (CH == 0) are read again
-// for the second pass, and their dw sums live in the CTA's own row of `part`.
+// NT threads hold a row, 16 columns each, so a row is read once; the sum is joined over the
+// threads in a fixed order, with one barrier a row.  A CTA walks down its rows, and each thread
+// copies its own columns of the next rows (Stage::kAhead) into shared memory while it works on one
+// (cp.async: no other thread reads them, so no barrier belongs to the copies): the bytes in
+// flight do not depend on how far the row's barrier has come.  Rows that do not start on 16
+// bytes are loaded when they are needed.  Wider rows are read again for the second pass, and
+// their dw sums live in the CTA's own row of `part`.
+constexpr int kCh = 2;      // groups of eight columns per thread
+
 template <int NT>
-ECO_DEV float row_sum(float v, float* sh) {
+ECO_DEV float row_sum(float v, float* sh) {  // sh: this row's buffer (two take turns)
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   if (NT > 32) {
     constexpr int W = NT / 32;
-    __syncthreads();  // sh may still be read for the row before
     if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
     __syncthreads();
     v = sh[threadIdx.x % W];
@@ -312,133 +407,314 @@ ECO_DEV float row_sum(float v, float* sh) {
   return v;
 }
 
-template <typename T, typename WT, int NT, int CH>
-__global__ void __launch_bounds__(NT == 32 ? kThreads : NT)
-    rms_fwd_kernel(Mat x, int64_t rows, int64_t cols, const WT* __restrict__ w, float eps, Mat y, Saved S,
-                   float* rstd) {
-  __shared__ float sh[NT / 32];
-  constexpr int RPC = NT == 32 ? kThreads / NT : 1;  // a wider row has the CTA's barriers to itself
-  const int tid = threadIdx.x % NT;
-  const int64_t span = (int64_t)NT * 8;
-  const int chunks = CH > 0 ? CH : (int)((cols + span - 1) / span);
-  for (int64_t r = (int64_t)blockIdx.x * RPC + threadIdx.x / NT; r < rows; r += (int64_t)gridDim.x * RPC) {
-    const T* row = static_cast<const T*>(x.p) + r * x.ld;
-    Oct<T> keep[CH > 0 ? CH : 1];
-    if constexpr (CH > 0) {
+// cp.async of `bytes` (0 .. N; the rest is zeros) to N bytes of shared memory.
+template <int N>
+ECO_DEV void copy_async(void* dst, const void* src, int bytes) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(N), "r"(bytes) : "memory");
+}
+ECO_DEV void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+ECO_DEV void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// One thread's columns of a row on their way: kCh groups of T (16-byte pieces, a piece of all
+// threads side by side), and for the backward the bytes, scales and the row's rstd.
+template <typename T, bool BWD>
+struct Stage {
+  static constexpr int V = Oct<T>::W / 4;
+  static constexpr int kBytes = kCh * 16 * V + (BWD ? kCh * 12 + 4 : 0);  // per thread
+  // Rows on their way besides the one in work: what 1024 threads' stages leave room for.
+  static constexpr int kAhead = 200 * 1024 / (kBytes * 1024) - 1 > 3 ? 3 : 200 * 1024 / (kBytes * 1024) - 1;
+  ECO_DEV static uint4* piece(char* st, int threads, int i, int v) {
+    return reinterpret_cast<uint4*>(st) + (i * V + v) * threads + threadIdx.x;
+  }
+  ECO_DEV static uint2* bytes(char* st, int threads, int i) {
+    return reinterpret_cast<uint2*>(st + kCh * 16 * V * threads) + i * threads + threadIdx.x;
+  }
+  ECO_DEV static float* word(char* st, int threads, int i) {  // scales, then rstd
+    return reinterpret_cast<float*>(st + kCh * (16 * V + 8) * threads) + i * threads + threadIdx.x;
+  }
+};
+
+// The weight of a thread's columns (ones without a weight, zeros past the end).
+template <typename T>
+ECO_DEV void load_weight(const void* w, bool w_f32, int64_t cols, int64_t c, float (&f)[8]) {
+  const int n = left8(cols, c);
+  if (!w) {
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int64_t c = i * span + tid * 8;
-        keep[i] = load8(row, c, left8(cols, c));
+    for (int k = 0; k < 8; ++k) f[k] = 1.0f;
+  } else if (w_f32) {
+    unpack8(load8(static_cast<const float*>(w), c, n), f);
+  } else {
+    unpack8(load8(static_cast<const T*>(w), c, n), f);
+  }
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, NT == 32 ? 1024 / kThreads : 1024 / NT)
+    rms_fwd_kernel(Mat x, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, float eps, Mat y,
+                   Saved S, float* rstd, bool async) {
+  extern __shared__ __align__(16) char stages[];
+  __shared__ float sh[2][NT / 32];
+  using St = Stage<T, false>;
+  constexpr int THREADS = NT == 32 ? kThreads : NT, RPC = THREADS / NT;
+  constexpr int kStage = St::kBytes * THREADS, kAhead = St::kAhead;
+  const int tid = threadIdx.x % NT;
+  const int64_t step = (int64_t)gridDim.x * RPC;
+  int64_t r = (int64_t)blockIdx.x * RPC + threadIdx.x / NT;
+  auto column = [&](int i) { return ((int64_t)i * NT + tid) * 8; };
+  auto issue = [&](int64_t row, int slot) {
+    if (async && row < rows) {
+      const T* p = static_cast<const T*>(x.p) + row * x.ld;
+#pragma unroll
+      for (int i = 0; i < kCh; ++i) {
+        const int n = left8(cols, column(i)) * (int)sizeof(T);
+#pragma unroll
+        for (int v = 0; v < St::V; ++v) {
+          const int b = n - 16 * v < 0 ? 0 : (n - 16 * v > 16 ? 16 : n - 16 * v);
+          copy_async<16>(St::piece(stages + slot * kStage, THREADS, i, v), b > 0 ? p + column(i) + 4 * v : p, b);
+        }
       }
     }
-    float ss = 0.0f;
-#pragma unroll(CH > 0 ? CH : 1)
-    for (int i = 0; i < chunks; ++i) {
-      const int64_t c = i * span + tid * 8;
-      float f[8];
-      unpack8(CH > 0 ? keep[CH > 0 ? i : 0] : load8(row, c, left8(cols, c)), f);
+    copies_commit();
+  };
+  for (int d = 0; d < kAhead; ++d) issue(r + d * step, d);
+  float wt[kCh][8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) ss = fmaf(f[k], f[k], ss);
+  for (int i = 0; i < kCh; ++i) load_weight<T>(w, w_f32, cols, column(i), wt[i]);
+  for (int k = 0; r < rows; ++k, r += step) {
+    issue(r + kAhead * step, (k + kAhead) % (kAhead + 1));
+    Oct<T> o[kCh];
+    if (async) {
+      copies_wait<kAhead>();
+      char* st = stages + (k % (kAhead + 1)) * kStage;
+#pragma unroll
+      for (int i = 0; i < kCh; ++i)
+#pragma unroll
+        for (int v = 0; v < St::V; ++v) {
+          const uint4 q = *St::piece(st, THREADS, i, v);
+          o[i].w[4 * v] = q.x, o[i].w[4 * v + 1] = q.y, o[i].w[4 * v + 2] = q.z, o[i].w[4 * v + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCh; ++i)
+        o[i] = load8(static_cast<const T*>(x.p) + r * x.ld, column(i), left8(cols, column(i)));
     }
-    ss = row_sum<NT>(ss, sh);
+    float ss = 0.0f, f[kCh][8];
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) {
+      unpack8(o[i], f[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[i][j], f[i][j], ss);
+    }
+    ss = row_sum<NT>(ss, sh[k & 1]);
     const float rs = rsqrtf(ss / (float)cols + eps);
     if (tid == 0 && rstd) rstd[r] = rs;
-#pragma unroll(CH > 0 ? CH : 1)
-    for (int i = 0; i < chunks; ++i) {
-      const int64_t c = i * span + tid * 8;
-      const int n = left8(cols, c);
-      float f[8], g[8];
-      unpack8(CH > 0 ? keep[CH > 0 ? i : 0] : load8(row, c, n), f);
-      if (S.q) put8(f, n, S.q + r * S.ld_q, c, S.scale + r * S.ld_s + c / kBlock);
-      if (w) unpack8(load8(w, c, n), g);
+    if (S.q) {
+      float amax[kCh], gain[kCh];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = w ? f[k] * rs * g[k] : f[k] * rs;
+      for (int i = 0; i < kCh; ++i) amax[i] = block_amax(f[i]);
+      const float scale = block_gains(amax, gain);
+      const int lane = threadIdx.x & (kLanes - 1);
+#pragma unroll
+      for (int i = 0; i < kCh; ++i) {
+        const int64_t c = column(i), c0 = c - 8 * lane;  // the block's first column
+        if (c < cols) __stcs(reinterpret_cast<uint2*>(S.q + r * S.ld_q + c), quant8(f[i], gain[i]));
+        if (lane == i && c0 < cols) S.scale[r * S.ld_s + c0 / kBlock] = scale;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] * rs * wt[i][j];
+      const int n = left8(cols, column(i));
+      if (n > 0) store8(static_cast<T*>(y.p) + r * y.ld, column(i), n, true, f[i]);
+    }
+  }
+}
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, NT == 32 ? 1024 / kThreads : 1024 / NT)
+    rms_bwd_kernel(Mat dy, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, Saved S,
+                   const float* __restrict__ rstd, Mat dx, float* part, int64_t ld_part, bool async) {
+  extern __shared__ __align__(16) char stages[];
+  __shared__ float sh[2][NT / 32];
+  using St = Stage<T, true>;
+  constexpr int THREADS = NT == 32 ? kThreads : NT, RPC = THREADS / NT;
+  constexpr int kStage = St::kBytes * THREADS, kAhead = St::kAhead;
+  const int tid = threadIdx.x % NT;
+  const int64_t step = (int64_t)gridDim.x * RPC;
+  const int64_t group = (int64_t)blockIdx.x * RPC + threadIdx.x / NT;
+  int64_t r = group;
+  auto column = [&](int i) { return ((int64_t)i * NT + tid) * 8; };
+  auto issue = [&](int64_t row, int slot) {
+    if (async && row < rows) {
+      char* st = stages + slot * kStage;
+      const T* p = static_cast<const T*>(dy.p) + row * dy.ld;
+      const int8_t* q = S.q + row * S.ld_q;
+      const float* sc = S.scale + row * S.ld_s;
+#pragma unroll
+      for (int i = 0; i < kCh; ++i) {
+        const int64_t c = column(i);
+        const int n = left8(cols, c) * (int)sizeof(T);
+#pragma unroll
+        for (int v = 0; v < St::V; ++v) {
+          const int b = n - 16 * v < 0 ? 0 : (n - 16 * v > 16 ? 16 : n - 16 * v);
+          copy_async<16>(St::piece(st, THREADS, i, v), b > 0 ? p + c + 4 * v : p, b);
+        }
+        copy_async<8>(St::bytes(st, THREADS, i), n > 0 ? q + c : q, n > 0 ? 8 : 0);
+        copy_async<4>(St::word(st, THREADS, i), n > 0 ? sc + c / kBlock : sc, n > 0 ? 4 : 0);
+      }
+      copy_async<4>(St::word(st, THREADS, kCh), rstd + row, 4);
+    }
+    copies_commit();
+  };
+  for (int d = 0; d < kAhead; ++d) issue(r + d * step, d);
+  float acc[kCh][8] = {};
+  for (int k = 0; r < rows; ++k, r += step) {
+    issue(r + kAhead * step, (k + kAhead) % (kAhead + 1));
+    Oct<T> o[kCh];
+    Eights e[kCh];
+    float rs;
+    if (async) {
+      copies_wait<kAhead>();
+      char* st = stages + (k % (kAhead + 1)) * kStage;
+#pragma unroll
+      for (int i = 0; i < kCh; ++i) {
+#pragma unroll
+        for (int v = 0; v < St::V; ++v) {
+          const uint4 q = *St::piece(st, THREADS, i, v);
+          o[i].w[4 * v] = q.x, o[i].w[4 * v + 1] = q.y, o[i].w[4 * v + 2] = q.z, o[i].w[4 * v + 3] = q.w;
+        }
+        e[i].q = *St::bytes(st, THREADS, i);
+        e[i].s = *St::word(st, THREADS, i);
+      }
+      rs = *St::word(st, THREADS, kCh);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCh; ++i) {
+        const int n = left8(cols, column(i));
+        o[i] = load8(static_cast<const T*>(dy.p) + r * dy.ld, column(i), n);
+        e[i] = fetch8(S, r, column(i), n);
+      }
+      rs = rstd[r];
+    }
+    float dot = 0.0f, d[kCh][8], u[kCh][8];
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) {
+      float wt[8];
+      load_weight<T>(w, w_f32, cols, column(i), wt);  // from L1: registers hold the sums
+      unpack8(o[i], d[i]);
+      e[i].s *= rs;
+      values8(e[i], u[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        acc[i][j] = fmaf(d[i][j], u[i][j], acc[i][j]);
+        d[i][j] *= wt[j];
+        dot = fmaf(d[i][j], u[i][j], dot);
+      }
+    }
+    dot = row_sum<NT>(dot, sh[k & 1]) / (float)cols;
+#pragma unroll
+    for (int i = 0; i < kCh; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) d[i][j] = rs * fmaf(-u[i][j], dot, d[i][j]);
+      const int n = left8(cols, column(i));
+      if (n > 0) store8(static_cast<T*>(dx.p) + r * dx.ld, column(i), n, true, d[i]);
+    }
+  }
+  if (part) {
+#pragma unroll
+    for (int i = 0; i < kCh; ++i)
+      if (left8(cols, column(i)) > 0) store8(part + group * ld_part, column(i), 8, true, acc[i]);
+  }
+}
+
+// ---- rows too wide for a CTA's registers (more than 16384 columns): two passes over the row
+constexpr int kWide = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(kWide)
+    rms_fwd_wide_kernel(Mat x, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, float eps, Mat y,
+                        Saved S, float* rstd) {
+  __shared__ float sh[2][kWide / 32];
+  const int lane = threadIdx.x & (kLanes - 1);
+  int k = 0;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, ++k) {
+    const T* row = static_cast<const T*>(x.p) + r * x.ld;
+    float ss = 0.0f;
+    for (int64_t c = threadIdx.x * 8; c < cols; c += kWide * 8) {
+      float f[8];
+      unpack8(load8(row, c, left8(cols, c)), f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
+    }
+    ss = row_sum<kWide>(ss, sh[k & 1]);
+    const float rs = rsqrtf(ss / (float)cols + eps);
+    if (threadIdx.x == 0 && rstd) rstd[r] = rs;
+    for (int64_t cc = 0; cc < cols; cc += kWide * 8) {  // every lane, for the shuffles
+      const int64_t c = cc + threadIdx.x * 8, c0 = c - 8 * lane;
+      const int n = left8(cols, c);
+      float f[8], wt[8];
+      unpack8(load8(row, c, n), f);
+      if (S.q) {
+        const float amax[1] = {block_amax(f)};
+        float gain[1];
+        const float scale = block_gains(amax, gain);
+        if (n > 0) __stcs(reinterpret_cast<uint2*>(S.q + r * S.ld_q + c), quant8(f, gain[0]));
+        if (lane == 0 && c0 < cols) S.scale[r * S.ld_s + c0 / kBlock] = scale;
+      }
+      load_weight<T>(w, w_f32, cols, c, wt);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = f[j] * rs * wt[j];
       if (n > 0) store8(static_cast<T*>(y.p) + r * y.ld, c, n, true, f);
     }
   }
 }
 
-template <typename T, typename WT, int NT, int CH>
-__global__ void __launch_bounds__(NT == 32 ? kThreads : NT)
-    rms_bwd_kernel(Mat dy, int64_t rows, int64_t cols, const WT* __restrict__ w, Saved S,
-                   const float* __restrict__ rstd, Mat dx, float* part, int64_t ld_part) {
-  __shared__ float sh[NT / 32];
-  constexpr int RPC = NT == 32 ? kThreads / NT : 1;  // a wider row has the CTA's barriers to itself
-  const int tid = threadIdx.x % NT;
-  const int64_t span = (int64_t)NT * 8;
-  const int chunks = CH > 0 ? CH : (int)((cols + span - 1) / span);
-  float acc[CH > 0 ? CH : 1][8] = {};
-  // one row of `part` per row group of the grid
-  float* mine = part ? part + ((int64_t)blockIdx.x * RPC + threadIdx.x / NT) * ld_part : nullptr;
-  if (CH == 0 && mine)
-    for (int i = 0; i < chunks; ++i) {
-      const int64_t c = i * span + tid * 8;
-      if (left8(cols, c) > 0) store8(mine, c, 8, true, acc[0]);
-    }
-  for (int64_t r = (int64_t)blockIdx.x * RPC + threadIdx.x / NT; r < rows; r += (int64_t)gridDim.x * RPC) {
-    const T* drow = static_cast<const T*>(dy.p) + r * dy.ld;
-    const int8_t* qrow = S.q + r * S.ld_q;
-    const float* srow = S.scale + r * S.ld_s;
+template <typename T>
+__global__ void __launch_bounds__(kWide)
+    rms_bwd_wide_kernel(Mat dy, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, Saved S,
+                        const float* __restrict__ rstd, Mat dx, float* part, int64_t ld_part) {
+  __shared__ float sh[2][kWide / 32];
+  float* mine = part ? part + blockIdx.x * ld_part : nullptr;
+  int k = 0;
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, ++k) {
+    const T* row = static_cast<const T*>(dy.p) + r * dy.ld;
     const float rs = rstd[r];
-    Oct<T> keep[CH > 0 ? CH : 1];
-    uint2 bytes[CH > 0 ? CH : 1];
-    float unit[CH > 0 ? CH : 1];  // scale * rstd
-    auto fetch = [&](int64_t c, Oct<T>& o, uint2& q, float& s) {
-      const int n = left8(cols, c);
-      o = load8(drow, c, n);
-      q = make_uint2(0u, 0u);
-      s = 0.0f;
-      if (n > 0) {
-        q = __ldcs(reinterpret_cast<const uint2*>(qrow + c));
-        s = __ldg(srow + c / kBlock) * rs;
-      }
-    };
-    if constexpr (CH > 0) {
-#pragma unroll
-      for (int i = 0; i < CH; ++i) fetch(i * span + tid * 8, keep[i], bytes[i], unit[i]);
-    }
     float dot = 0.0f;
-#pragma unroll(CH > 0 ? CH : 1)
-    for (int i = 0; i < chunks; ++i) {
-      const int64_t c = i * span + tid * 8;
-      const int j = CH > 0 ? i : 0;
-      if (CH == 0) fetch(c, keep[0], bytes[0], unit[0]);
-      float d[8], u[8], g[8];
-      unpack8(keep[j], d);
-      dequant8(bytes[j], u);
-      if (w) unpack8(load8(w, c, left8(cols, c)), g);
-      if (CH == 0 && mine && left8(cols, c) > 0) {  // plain loads: the CTA writes this row itself
+    for (int64_t c = threadIdx.x * 8; c < cols; c += kWide * 8) {
+      const int n = left8(cols, c);
+      float d[8], u[8], wt[8];
+      unpack8(load8(row, c, n), d);
+      Eights e = fetch8(S, r, c, n);
+      e.s *= rs;
+      values8(e, u);
+      load_weight<T>(w, w_f32, cols, c, wt);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) acc[0][k] = mine[c + k];
+      for (int j = 0; j < 8; ++j) {
+        // a thread owns its columns of the CTA's sums: plain loads and stores, no atomics
+        if (mine) mine[c + j] = fmaf(d[j], u[j], k ? mine[c + j] : 0.0f);
+        dot = fmaf(d[j] * wt[j], u[j], dot);
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        u[k] *= unit[j];
-        acc[j][k] = fmaf(d[k], u[k], acc[j][k]);
-        dot = fmaf(w ? d[k] * g[k] : d[k], u[k], dot);
-      }
-      if (CH == 0 && mine && left8(cols, c) > 0) store8(mine, c, 8, true, acc[0]);
     }
-    dot = row_sum<NT>(dot, sh) / (float)cols;
-#pragma unroll(CH > 0 ? CH : 1)
-    for (int i = 0; i < chunks; ++i) {
-      const int64_t c = i * span + tid * 8;
-      const int n = left8(cols, c), j = CH > 0 ? i : 0;
-      if (CH == 0) fetch(c, keep[0], bytes[0], unit[0]);
-      float d[8], u[8], g[8];
-      unpack8(keep[j], d);
-      dequant8(bytes[j], u);
-      if (w) unpack8(load8(w, c, n), g);
+    dot = row_sum<kWide>(dot, sh[k & 1]) / (float)cols;
+    for (int64_t c = threadIdx.x * 8; c < cols; c += kWide * 8) {
+      const int n = left8(cols, c);
+      float d[8], u[8], wt[8];
+      unpack8(load8(row, c, n), d);
+      Eights e = fetch8(S, r, c, n);
+      e.s *= rs;
+      values8(e, u);
+      load_weight<T>(w, w_f32, cols, c, wt);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = rs * fmaf(-u[k] * unit[j], dot, w ? d[k] * g[k] : d[k]);
-      if (n > 0) store8(static_cast<T*>(dx.p) + r * dx.ld, c, n, true, d);
-    }
-  }
-  if (CH > 0 && mine) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int64_t c = i * span + tid * 8;
-      if (left8(cols, c) > 0) store8(mine, c, 8, true, acc[i]);
+      for (int j = 0; j < 8; ++j) d[j] = rs * fmaf(-u[j], dot, d[j] * wt[j]);
+      store8(static_cast<T*>(dx.p) + r * dx.ld, c, n, true, d);
     }
   }
 }
@@ -469,10 +745,12 @@ int bpr_log2_of(int64_t cols) {
   while (l < 4 && (1 << l) < blocks) ++l;
   return l;
 }
-dim3 block_grid(int64_t rows, int64_t cols, int bpr_log2) {
-  const int64_t blocks = (cols + kBlock - 1) / kBlock, rpc = kHalves >> bpr_log2;
+// As many CTAs as are resident (eight of 256 threads per SM), each walking down its rows.
+dim3 block_grid(int64_t rows, int64_t cols, int bpr_log2, int unroll) {
+  const int64_t blocks = (cols + kBlock - 1) / kBlock, rpc = (int64_t)(kHalves >> bpr_log2) * unroll;
   const int64_t gx = std::min<int64_t>((blocks + (1 << bpr_log2) - 1) >> bpr_log2, 65535);
-  const int64_t gy = std::min<int64_t>((rows + rpc - 1) / rpc, 65535);
+  const int64_t most = std::max<int64_t>(1, (int64_t)eco_num_sms() * 8 / gx);
+  const int64_t gy = std::min<int64_t>((rows + rpc - 1) / rpc, std::min<int64_t>(most, 65535));
   return dim3((unsigned)gx, (unsigned)gy);
 }
 
@@ -515,21 +793,39 @@ void by_float(int type, F f) {
   else f((__half*)nullptr);
 }
 
-// Threads and groups of a row: four groups of eight columns per thread as far as a CTA goes.
+// Threads of a row (16 columns each), 0 for the two-pass kernels of wider rows.
+int row_threads(int64_t cols) {
+  int nt = 32;
+  while (nt < 1024 && (int64_t)nt * 8 * kCh < cols) nt *= 2;
+  return (int64_t)nt * 8 * kCh < cols ? 0 : nt;
+}
 template <typename F>
 void by_width(int64_t cols, F f) {
-  if (cols <= 256) f(std::integral_constant<int, 32>{}, std::integral_constant<int, 1>{});
-  else if (cols <= 1024) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 1>{});
-  else if (cols <= 4096) f(std::integral_constant<int, 128>{}, std::integral_constant<int, 4>{});
-  else if (cols <= 8192) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-  else if (cols <= 16384) f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
-  else f(std::integral_constant<int, 512>{}, std::integral_constant<int, 0>{});
+  switch (row_threads(cols)) {
+    case 32: return f(std::integral_constant<int, 32>{});
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    case 256: return f(std::integral_constant<int, 256>{});
+    case 512: return f(std::integral_constant<int, 512>{});
+    case 1024: return f(std::integral_constant<int, 1024>{});
+    default: return f(std::integral_constant<int, 0>{});
+  }
 }
-int row_threads(int64_t cols) { return cols <= 256 ? 32 : cols <= 4096 ? 128 : cols <= 8192 ? 256 : 512; }
-int64_t rms_groups(int64_t rows, int64_t cols) {  // row groups of the backward's grid
-  const int nt = row_threads(cols), threads = nt == 32 ? kThreads : nt, rpc = threads / nt;
-  const int64_t ctas = std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)eco_num_sms() * (1024 / threads));
-  return ctas * rpc;
+// CTAs of the norm's kernels: what is resident at 1024 threads per SM.
+int64_t rms_ctas(int64_t rows, int64_t cols) {
+  const int nt = row_threads(cols);
+  const int threads = nt == 0 ? kWide : nt == 32 ? kThreads : nt, rpc = nt == 32 ? kThreads / 32 : 1;
+  return std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)eco_num_sms() * (1024 / threads));
+}
+int64_t rms_groups(int64_t rows, int64_t cols) {
+  return rms_ctas(rows, cols) * (row_threads(cols) == 32 ? kThreads / 32 : 1);
+}
+// Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device; the
+// attribute is set at each launch that needs it (a host-side store, no synchronisation).
+template <typename K>
+bool allow_smem(K kernel, int bytes) {
+  return bytes <= 47 * 1024 ||  // static arrays count too
+         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess;
 }
 
 }  // namespace
@@ -543,7 +839,8 @@ extern "C" int eco_ckpt_pack(const void* x, int type, int64_t rows, int64_t cols
   const int l = bpr_log2_of(cols);
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    pack_kernel<T><<<block_grid(rows, cols, l), kThreads, 0, eco_stream(stream)>>>(
+    constexpr int U = sizeof(T) == 4 ? 2 : 4;
+    pack_kernel<T, U><<<block_grid(rows, cols, l, U), kThreads, 0, eco_stream(stream)>>>(
         Mat{const_cast<void*>(x), ld}, rows, cols, saved_of(saved), l);
   });
   return eco_launch_check("eco_ckpt_pack");
@@ -558,8 +855,8 @@ extern "C" int eco_ckpt_restore(const eco_saved_i8_t* saved, int type, int64_t r
   const int l = bpr_log2_of(cols);
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    restore_kernel<T><<<block_grid(rows, cols, l), kThreads, 0, eco_stream(stream)>>>(saved_of(saved), rows, cols,
-                                                                                      Mat{x, ld}, l);
+    restore_kernel<T, 4><<<block_grid(rows, cols, l, 4), kThreads, 0, eco_stream(stream)>>>(saved_of(saved), rows,
+                                                                                            cols, Mat{x, ld}, l);
   });
   return eco_launch_check("eco_ckpt_restore");
 }
@@ -579,15 +876,16 @@ extern "C" int eco_gated_act(const void* gate, int64_t ld_gate, const void* up, 
     if (int rc = check_saved(saved_up, rows, cols, "eco_gated_act")) return rc;
   }
   const int l = bpr_log2_of(cols);
-  const dim3 grid = block_grid(rows, cols, l);
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int U = sizeof(T) == 4 ? 1 : 2;
+    const dim3 grid = block_grid(rows, cols, l, U);
     const Mat g{const_cast<void*>(gate), ld_gate}, u{const_cast<void*>(up), ld_up}, o{y, ld_y};
     if (act == ECO_ACT_GELU)
-      gated_fwd_kernel<T, true><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, rows, cols, o, saved_of(saved_gate),
+      gated_fwd_kernel<T, true, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, rows, cols, o, saved_of(saved_gate),
                                                                            saved_of(saved_up), l);
     else
-      gated_fwd_kernel<T, false><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, rows, cols, o, saved_of(saved_gate),
+      gated_fwd_kernel<T, false, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, rows, cols, o, saved_of(saved_gate),
                                                                             saved_of(saved_up), l);
   });
   return eco_launch_check("eco_gated_act");
@@ -609,15 +907,16 @@ extern "C" int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int ac
   const bool vg = rows_on_16(dgate, ld_dgate, rows, type);
   const bool vu = rows_on_16(dup, ld_dup, rows, type);
   const int l = bpr_log2_of(cols);
-  const dim3 grid = block_grid(rows, cols, l);
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
+    constexpr int U = sizeof(T) == 4 ? 1 : 2;
+    const dim3 grid = block_grid(rows, cols, l, U);
     const Mat d{const_cast<void*>(dy), ld_dy}, g{dgate, ld_dgate}, u{dup, ld_dup};
     if (act == ECO_ACT_GELU)
-      gated_bwd_kernel<T, true><<<grid, kThreads, 0, eco_stream(stream)>>>(
+      gated_bwd_kernel<T, true, U><<<grid, kThreads, 0, eco_stream(stream)>>>(
           d, rows, cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
     else
-      gated_bwd_kernel<T, false><<<grid, kThreads, 0, eco_stream(stream)>>>(
+      gated_bwd_kernel<T, false, U><<<grid, kThreads, 0, eco_stream(stream)>>>(
           d, rows, cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
   });
   return eco_launch_check("eco_gated_act_bwd");
@@ -635,21 +934,28 @@ extern "C" int eco_rms_norm(const void* x, int64_t ld, int type, int64_t rows, i
   if (int rc = check_out(y, ld_y, rows, cols, type, "eco_rms_norm")) return rc;
   if (saved)
     if (int rc = check_saved(saved, rows, cols, "eco_rms_norm")) return rc;
+  bool ok = true;
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    by_width(cols, [&](auto nt, auto ch) {
-      constexpr int NT = decltype(nt)::value, CH = decltype(ch)::value;
-      constexpr int threads = NT == 32 ? kThreads : NT, rpc = threads / NT;
-      const unsigned grid = (unsigned)std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)eco_num_sms() * 8);
+    by_width(cols, [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      const unsigned grid = (unsigned)rms_ctas(rows, cols);
       const Mat xi{const_cast<void*>(x), ld}, yo{y, ld_y};
-      if (w && w_type != type)
-        rms_fwd_kernel<T, float, NT, CH><<<grid, threads, 0, eco_stream(stream)>>>(
-            xi, rows, cols, static_cast<const float*>(w), (float)eps, yo, saved_of(saved), rstd);
-      else
-        rms_fwd_kernel<T, T, NT, CH><<<grid, threads, 0, eco_stream(stream)>>>(
-            xi, rows, cols, static_cast<const T*>(w), (float)eps, yo, saved_of(saved), rstd);
+      const bool w_f32 = w_type == ECO_F32;
+      if constexpr (NT == 0) {
+        rms_fwd_wide_kernel<T><<<grid, kWide, 0, eco_stream(stream)>>>(xi, rows, cols, w, w_f32, (float)eps, yo,
+                                                                       saved_of(saved), rstd);
+      } else {
+        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, false>::kBytes * threads * (Stage<T, false>::kAhead + 1);
+        const bool async = rows_on_16(x, ld, rows, type);
+        ok = allow_smem(rms_fwd_kernel<T, NT>, smem);
+        if (ok)
+          rms_fwd_kernel<T, NT><<<grid, threads, async ? smem : 0, eco_stream(stream)>>>(
+              xi, rows, cols, w, w_f32, (float)eps, yo, saved_of(saved), rstd, async);
+      }
     });
   });
+  if (!ok) return eco_fail(ECO_ERR_LAUNCH, "eco_rms_norm: %s", cudaGetErrorString(cudaGetLastError()));
   return eco_launch_check("eco_rms_norm");
 }
 
@@ -678,22 +984,28 @@ extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t
   const int64_t groups = rms_groups(rows, cols), ld_part = (cols + 7) / 8 * 8;
   ECO_REQUIRE(!dw || (scratch && eco_aligned16(scratch) && scratch_len >= groups * ld_part), ECO_ERR_ARG,
               "eco_rms_norm_bwd: scratch too small (eco_rms_norm_bwd_scratch)");
+  bool ok = true;
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    by_width(cols, [&](auto nt, auto ch) {
-      constexpr int NT = decltype(nt)::value, CH = decltype(ch)::value;
-      constexpr int threads = NT == 32 ? kThreads : NT, rpc = threads / NT;
-      const unsigned grid = (unsigned)(groups / rpc);
+    by_width(cols, [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      const unsigned grid = (unsigned)rms_ctas(rows, cols);
       const Mat d{const_cast<void*>(dy), ld_dy}, o{dx, ld_dx};
       float* part = dw ? scratch : nullptr;
-      if (w && w_type != type)
-        rms_bwd_kernel<T, float, NT, CH><<<grid, threads, 0, s>>>(d, rows, cols, static_cast<const float*>(w),
-                                                                  saved_of(saved), rstd, o, part, ld_part);
-      else
-        rms_bwd_kernel<T, T, NT, CH><<<grid, threads, 0, s>>>(d, rows, cols, static_cast<const T*>(w),
-                                                              saved_of(saved), rstd, o, part, ld_part);
+      const bool w_f32 = w_type == ECO_F32;
+      if constexpr (NT == 0) {
+        rms_bwd_wide_kernel<T><<<grid, kWide, 0, s>>>(d, rows, cols, w, w_f32, saved_of(saved), rstd, o, part, ld_part);
+      } else {
+        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, true>::kBytes * threads * (Stage<T, true>::kAhead + 1);
+        const bool async = rows_on_16(dy, ld_dy, rows, type);
+        ok = allow_smem(rms_bwd_kernel<T, NT>, smem);
+        if (ok)
+          rms_bwd_kernel<T, NT><<<grid, threads, async ? smem : 0, s>>>(d, rows, cols, w, w_f32, saved_of(saved), rstd,
+                                                                        o, part, ld_part, async);
+      }
     });
   });
+  if (!ok) return eco_fail(ECO_ERR_LAUNCH, "eco_rms_norm_bwd: %s", cudaGetErrorString(cudaGetLastError()));
   if (dw)
     by_float(w_type, [&](auto* t) {
       using WT = std::remove_pointer_t<decltype(t)>;

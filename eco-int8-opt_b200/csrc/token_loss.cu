@@ -31,23 +31,42 @@ ECO_DEV float ex2(float x) {
   return y;
 }
 
+// exp((x - m) mul) = 2^((x - m) c), c = mul log2 e.  The sum takes c in two parts: rounded to
+// one, it would stretch every difference by the same 2^-26 or so, which 10^5 terms do not
+// average out; the gradient's single probabilities do with one.
+struct Factor {
+  float hi, lo;
+};
 // What is subtracted before the exponential: m, and 0 for -inf alone (whose terms are then 0).
 // x - m comes first and is multiplied after: a row masked to its type's lowest value would
 // leave the fp32 range as x * c, and as x - m is 0 or -inf.
 ECO_DEV float row_off(float m) { return m == -INFINITY ? 0.0f : m; }
-ECO_DEV float term(float x, float off, float c) { return ex2((x - off) * c); }
+ECO_DEV float term(float x, float off, Factor c) {
+  const float d = x - off;
+  return ex2(fmaf(d, c.lo, d * c.hi));
+}
 
 struct MaxSum {
   float m, s;
 };
-ECO_DEV MaxSum join(MaxSum a, MaxSum b, float c) {
-  const float m = fmaxf(a.m, b.m);
-  const float off = row_off(m);
-  return MaxSum{m, a.s * term(a.m, off, c) + b.s * term(b.m, off, c)};
+// Joined over W lanes (a power of two; groups side by side); every lane gets the same bits.
+template <int W>
+ECO_DEV MaxSum lanes_join(MaxSum a, Factor c) {
+  float m = a.m;
+  if (W == 32) {
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(a.m));
+  } else {
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  }
+  float s = a.s * term(a.m, row_off(m), c);
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return MaxSum{m, s};
 }
 
 template <int E>
-ECO_DEV void take(MaxSum& a, const float (&x)[E], float c) {
+ECO_DEV void take(MaxSum& a, const float (&x)[E], Factor c) {
   float vm = x[0];
 #pragma unroll
   for (int k = 1; k < E; ++k) vm = fmaxf(vm, x[k]);
@@ -59,100 +78,121 @@ ECO_DEV void take(MaxSum& a, const float (&x)[E], float c) {
 #pragma unroll
   for (int k = 0; k < E; ++k) a.s += term(x[k], off, c);
 }
-
-// Joined over the NT threads of a row; every thread gets the same bits.
-template <int NT>
-ECO_DEV MaxSum row_join(MaxSum a, float c, MaxSum* sh) {
+// What a row's gradient needs: g_j = -k 2^((x_j - off) c), and coef more at the token.
+struct Slope {
+  float off, c, k, coef;
+  float base;  // 16-bit gradients: log2 |k| - off c, or NaN where that would cost accuracy
+};
+ECO_DEV Slope slope_of(float off, float c, float k, float coef) {
+  const float t = off * c;
+  return Slope{off, c, k, coef, fabsf(t) < 512.0f ? log2f(fabsf(k)) - t : __int_as_float(0x7fc00000)};
+}
+// A vector's logits to the vector of their gradient (without the token's share), stored at g + v E.
+// FOLD, 16 bits: |k| goes into the exponent, so that an element costs one multiply-add, one
+// exponential and half of a pack and a sign flip.  Its rounding is |exponent| 2^-24 and with
+// |off c| < 512 at most 2^-15 of the value, against half a step of 2^-9 or 2^-11.
+template <typename T, bool FOLD>
+ECO_DEV void store_slope(typename RowIo<T>::G* g, int64_t v, const uint4& raw, const Slope& w) {
+  constexpr int E = RowIo<T>::E;
+  float f[E];
+  RowIo<T>::unpack(raw, f);
+  if constexpr (FOLD && sizeof(T) == 2) {
+    if (w.base == w.base) {  // the same for the whole row
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    MaxSum b;
-    b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-    b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-    a = (threadIdx.x & o) ? join(b, a, c) : join(a, b, c);
-  }
-  if (NT > 32) {
-    constexpr int W = NT / 32;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (lane == 0) sh[warp] = a;
-    __syncthreads();
-    a = sh[lane % W];
-#pragma unroll
-    for (int o = W / 2; o > 0; o >>= 1) {
-      MaxSum b;
-      b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-      b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-      a = (lane & o) ? join(b, a, c) : join(a, b, c);
+      for (int i = 0; i < E; ++i) f[i] = ex2(fmaf(f[i], w.c, w.base));
+      uint4 q = RowIo<T>::pack(f);
+      const uint32_t sign = w.k > 0.0f ? 0x80008000u : 0u;
+      q.x ^= sign, q.y ^= sign, q.z ^= sign, q.w ^= sign;
+      __stcs(reinterpret_cast<uint4*>(g) + v, q);
+      return;
     }
   }
-  return a;
+#pragma unroll
+  for (int i = 0; i < E; ++i) f[i] = -w.k * ex2((f[i] - w.off) * w.c);
+  RowIo<T>::store(g, v, f);
+}
+// One element of it, the token's share included.
+ECO_DEV float slope_at(float x, const Slope& w, bool token) {
+  const float e = ex2((x - w.off) * w.c);
+  return token ? fmaf(-w.k, e, w.coef) : -w.k * e;
 }
 
-template <typename T, int NT>
-ECO_DEV MaxSum row_stats(const T* x, int64_t cols, float c, int tid, MaxSum* sh) {
+// N vectors at a time: their maximum first, so that the terms depend on nothing but it (and the
+// sum is rescaled only where the maximum has grown: seldom, after the first few).  ALL: all of
+// them count; else `in` says which.
+template <typename T, bool ALL, int N>
+ECO_DEV void take_vectors(MaxSum& a, const uint4 (&raw)[N], const bool (&in)[N], Factor c) {
   constexpr int E = RowIo<T>::E;
-  const RowSplit sp = RowIo<T>::split(x, cols);
-  MaxSum a{-INFINITY, 0.0f};
-  const T* body = x + sp.head;
-  int64_t v = tid;
-  for (; v + 3 * NT < sp.vecs; v += 4 * NT) {
-    typename RowIo<T>::Raw r[4];
+  float m = a.m;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) r[u] = RowIo<T>::load(body, v + u * NT);
+  for (int p = 0; p < N; ++p) m = ALL || in[p] ? fmaxf(m, RowIo<T>::max(raw[p])) : m;
+  const float off = row_off(m);
+  if (m > a.m) {
+    a.s *= term(a.m, off, c);
+    a.m = m;
+  }
+  float s[2] = {a.s, 0.0f};
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+  for (int p = 0; p < N; ++p) {
+    if (ALL || in[p]) {
       float f[E];
-      RowIo<T>::unpack(r[u], f);
-      take<E>(a, f, c);
+      RowIo<T>::unpack(raw[p], f);
+#pragma unroll
+      for (int k = 0; k < E; ++k) s[k & 1] += term(f[k], off, c);
     }
   }
-  for (; v < sp.vecs; v += NT) {
-    float f[E];
-    RowIo<T>::unpack(RowIo<T>::load(body, v), f);
-    take<E>(a, f, c);
-  }
-  if (tid < sp.head + sp.tail) {
-    const float f[1] = {to_f32(x[sp.edge(tid, cols)])};
-    take<1>(a, f, c);
-  }
-  return row_join<NT>(a, c, sh);
+  a.s = s[0] + s[1];
 }
+// Vectors p, p + step, ... of which `left` (counted in steps, from p on) count; N at a time.
+template <typename T, int N, bool SHARED>
+ECO_DEV void take_run(MaxSum& a, const uint4* p, int step, int left, Factor c) {
+  uint4 raw[N];
+  bool in[N];
+  for (; left >= N; left -= N, p += N * step) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) raw[u] = SHARED ? p[u * step] : __ldg(p + u * step);
+    take_vectors<T, true, N>(a, raw, in, c);
+  }
+  if (left > 0) {
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      in[u] = u < left;
+      raw[u] = in[u] ? (SHARED ? p[u * step] : __ldg(p + u * step)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    take_vectors<T, false, N>(a, raw, in, c);
+  }
+}
+// How many of the vectors tid, tid + NT, ... lie below `vecs`.
+template <int NT>
+ECO_DEV int run_length(int vecs, int tid) { return vecs > tid ? (vecs - tid + NT - 1) / NT : 0; }
 
-// g_j = -k 2^((x_j - off) c) (+ coef at y)
 template <typename T, int NT>
-ECO_DEV void row_grad(const T* x, typename RowIo<T>::G* g, int64_t cols, float c, float off, float k, float coef,
-                      int64_t y, int64_t tid, int64_t v_end) {
+ECO_DEV void row_grad(const T* x, typename RowIo<T>::G* g, int64_t cols, const Slope& w, int64_t y, int64_t tid,
+                      int64_t v_end) {
   constexpr int E = RowIo<T>::E;
+  using G = typename RowIo<T>::G;
   const RowSplit sp = RowIo<T>::split(x, cols);
   const T* body = x + sp.head;
-  typename RowIo<T>::G* gb = g + sp.head;
-  const int64_t yb = y - sp.head;
-  const int64_t vend = v_end < sp.vecs ? v_end : sp.vecs;
-  for (int64_t v0 = tid; v0 < vend; v0 += 4 * NT) {
-    typename RowIo<T>::Raw r[4];
+  G* gb = g + sp.head;
+  const int vend = (int)(v_end < sp.vecs ? v_end : sp.vecs);
+  for (int v0 = (int)tid; v0 < vend; v0 += 4 * NT) {
+    uint4 r[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u)
       if (v0 + u * NT < vend) r[u] = RowIo<T>::load_last(body, v0 + u * NT);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int64_t v = v0 + u * NT;
+      const int v = v0 + u * NT;
       if (v >= vend) break;
-      float f[E];
-      RowIo<T>::unpack(r[u], f);
-#pragma unroll
-      for (int i = 0; i < E; ++i) f[i] = -k * term(f[i], off, c);
-      const int64_t d = yb - v * E;
-      if (d >= 0 && d < E) {
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (d == i) f[i] += coef;
-      }
-      RowIo<T>::store(gb, v, f);
+      store_slope<T, false>(gb, v, r[u], w);
+      const int d = (int)y - sp.head - v * E;
+      // the token's element, by the thread that has just written its vector
+      if (d >= 0 && d < E) gb[v * E + d] = from_f32<G>(slope_at(to_f32(body[v * E + d]), w, true));
     }
   }
   if (tid < sp.head + sp.tail) {  // the threads of the row's first segment
     const int64_t j = sp.edge((int)tid, cols);
-    const float f = -k * term(to_f32(x[j]), off, c) + (j == y ? coef : 0.0f);
-    g[j] = from_f32<typename RowIo<T>::G>(f);
+    g[j] = from_f32<G>(slope_at(to_f32(x[j]), w, j == y));
   }
 }
 
@@ -170,7 +210,7 @@ struct Rows {
   const void* x;
   int64_t rows, n1, s0, s1, cols;
   double mul;
-  float c;  // mul * log2 e
+  Factor c;  // mul * log2 e
   const int64_t* tokens;
   const uint8_t* mask;  // nullable
   const int32_t* cu;    // nullable: rows outside [cu[0], cu[nseq]) do not count
@@ -192,40 +232,21 @@ struct Grad {
   int64_t s0, s1;
 };
 
-// The row's term in double: (raw_y - m) mul - log s.
+// The row's term in double: (raw_y - m) mul - log s.  ex2 gives values that are 5.0e-8 of
+// themselves too small on average (measured over arguments from -1 to -32, where it varies by
+// 0.1e-8; the largest term, 2^0, is exact).  In a sum of many terms that does not average out,
+// and a sequence adds up hundreds of such sums, so the log takes it back.
+constexpr float kEx2Short = 5.0e-8f;
+// The log is that of the mantissa in fp32 (below 0.35 in magnitude, so good to 2^-25) and the
+// exponent's in double: a thread does this once per row in front of a barrier, and the double
+// log's chain of dependent steps took longer than a row of a few thousand columns.
 ECO_DEV double token_logp(float raw_y, MaxSum a, double mul) {
-  return ((double)raw_y - (double)a.m) * mul - log((double)a.s);
-}
-
-// ------------------------------------------------ forward: lp and what the gradient needs
-// One warp per row for short rows, one CTA per row for long ones.
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT < 256 ? 256 : NT)
-    token_logp_kernel(const __grid_constant__ Rows R, float* logp, double* lp64, float2* stats, float* coef0) {
-  __shared__ MaxSum sh[NT > 32 ? NT / 32 : 1];
-  const int tid = threadIdx.x % NT;
-  for (int64_t r = (int64_t)blockIdx.x * (blockDim.x / NT) + threadIdx.x / NT; r < R.rows;
-       r += (int64_t)gridDim.x * (blockDim.x / NT)) {
-    const bool counts = R.counts(r);
-    double lp = 0.0;
-    float2 st = make_float2(0.0f, 0.0f);
-    if (counts) {
-      const T* x = static_cast<const T*>(R.x) + R.at(r, R.s0, R.s1);
-      const float raw_y = tid == 0 ? to_f32(x[R.tokens[r]]) : 0.0f;
-      const MaxSum a = row_stats<T, NT>(x, R.cols, R.c, tid, sh);
-      if (tid == 0) {
-        lp = token_logp(raw_y, a, R.mul);
-        st = make_float2(row_off(a.m), 1.0f / a.s);
-      }
-      if (NT > 32) __syncthreads();  // sh is free again
-    }
-    if (tid == 0) {
-      if (logp) logp[r] = (float)lp;
-      if (lp64) lp64[r] = lp;
-      if (stats) stats[r] = st;
-      if (coef0) coef0[r] = 0.0f;
-    }
-  }
+  const int bits = __float_as_int(a.s) - 0x3f3504f3;  // mantissa in [sqrt 1/2, sqrt 2)
+  const int e = bits >> 23;
+  const float f = a.s > 0.0f && a.s < INFINITY ? __int_as_float((bits & 0x007fffff) + 0x3f3504f3) : a.s;
+  const float small = logf(f) + kEx2Short * (1.0f - __fdividef(1.0f, a.s));
+  const double whole = a.s > 0.0f && a.s < INFINITY ? (double)e * 0.69314718055994530942 : 0.0;
+  return ((double)raw_y - (double)a.m) * mul - (whole + (double)small);
 }
 
 // ------------------------------------------------ gradient from a coefficient per row
@@ -248,7 +269,7 @@ __global__ void __launch_bounds__(256)
     if (k == 0.0f)
       row_zero<T, NT>(x, g, R.cols, v0 + tid, v0 + seg);
     else
-      row_grad<T, NT>(x, g, R.cols, R.c, st.x, k * st.y, k, R.tokens[r], v0 + tid, v0 + seg);
+      row_grad<T, NT>(x, g, R.cols, Slope{st.x, R.c.hi, k * st.y, k, 0.0f}, R.tokens[r], v0 + tid, v0 + seg);
   }
 }
 
@@ -262,10 +283,17 @@ struct Token {
   float loss, kl, coef;
   bool clipped;
 };
+// What a row's terms need besides its logits, loaded before they are needed.
+struct Given {
+  float old, adv, ref;
+};
+ECO_DEV Given given_of(const Policy& P, int64_t r) {
+  return Given{P.old_logp[r], P.adv[r], P.ref ? P.ref[r] : 0.0f};
+}
 // free = -A r, held = -A clip(r); loss = max(free, held) + kl_coef kl; dloss/dlp.
-ECO_DEV Token policy_token(const Policy& P, int64_t r, double lp) {
-  const float A = P.adv[r];
-  const float ratio = expf((float)(lp - (double)P.old_logp[r]));
+ECO_DEV Token policy_token(const Policy& P, const Given& v, double lp) {
+  const float A = v.adv;
+  const float ratio = expf((float)(lp - (double)v.old));
   const float free = -A * ratio, held = -A * fminf(fmaxf(ratio, P.low), P.high);
   Token t;
   t.clipped = free < held;
@@ -273,7 +301,7 @@ ECO_DEV Token policy_token(const Policy& P, int64_t r, double lp) {
   t.coef = t.clipped ? 0.0f : free;
   t.kl = 0.0f;
   if (P.ref) {
-    const float d = (float)((double)P.ref[r] - lp);
+    const float d = (float)((double)v.ref - lp);
     const float e = expm1f(d);
     t.kl = e - d;
     t.loss += P.kl_coef * t.kl;
@@ -282,12 +310,32 @@ ECO_DEV Token policy_token(const Policy& P, int64_t r, double lp) {
   return t;
 }
 
-// How many rows count, at least 1, by the whole CTA (every CTA reads the masks itself: a few
-// bytes per row from L2, against one launch more).
-ECO_DEV double policy_denom(const Rows& R, double given, int* sh) {
+// How many rows count, at least 1, by the whole CTA.  Few rows: every CTA reads the masks
+// itself (a few bytes per row from L2, against one launch more); many: from kCounts partial
+// counts of a launch of its own.
+constexpr int kCounts = 64;
+constexpr int64_t kCountRows = 2048;  // more rows than this are counted beforehand
+
+__global__ void __launch_bounds__(256) count_kernel(const __grid_constant__ Rows R, int* counts) {
+  __shared__ int sh[8];
+  int n = 0;
+  for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < R.rows; r += 256 * kCounts) n += R.counts(r);
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 8; ++w) n += sh[w];
+    counts[blockIdx.x] = n;
+  }
+}
+ECO_DEV double policy_denom(const Rows& R, double given, const int* counts, int* sh) {
   if (given > 0.0) return given;
   int n = 0;
-  for (int64_t r = threadIdx.x; r < R.rows; r += blockDim.x) n += R.counts(r);
+  if (counts) {
+    for (int i = threadIdx.x; i < kCounts; i += blockDim.x) n += counts[i];
+  } else {
+    for (int64_t r = threadIdx.x; r < R.rows; r += blockDim.x) n += R.counts(r);
+  }
   n = __reduce_add_sync(0xffffffffu, n);
   if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = n;
   __syncthreads();
@@ -296,6 +344,8 @@ ECO_DEV double policy_denom(const Rows& R, double given, int* sh) {
   __syncthreads();
   return all > 0 ? (double)all : 1.0;
 }
+// A coefficient over the denominator (its reciprocal, taken once), times the caller's factor.
+ECO_DEV float over(float coef, double inv_denom, float gain) { return (float)((double)coef * inv_denom) * gain; }
 
 struct Terms {  // per row: loss, kl, clipped
   float *loss, *kl, *clip;
@@ -306,53 +356,451 @@ ECO_DEV void put(const Terms& t, int64_t r, float loss, float kl, float clip) {
   t.clip[r] = clip;
 }
 
-// The whole policy loss of a row: statistics, coefficient, gradient.  The second pass finds
-// the row in L2 (148 SMs x rows in flight of up to 512 KB against 126 MB).
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT < 256 ? 256 : NT)
-    policy_row_kernel(const __grid_constant__ Rows R, const __grid_constant__ Policy P, float gain, float* logp,
-                      const __grid_constant__ Terms terms, const __grid_constant__ Grad G) {
+// ------------------------------------------------ rows held on the chip
+// Rows of up to kPieces vectors per thread stay in shared memory between the pass that sums
+// them and the pass that writes their gradient.  A CTA walks down its rows; each thread copies
+// the vectors it will work on itself (cp.async, kRows rows' worth of places), so no barrier
+// belongs to the copies: while a row's sums are joined and its gradient is written, the next
+// two rows are on their way.  Row i + 1 is summed before row i's gradient is written, so that
+// the scalar work of row i (logarithm, loss terms: one thread) runs behind it; one CTA barrier a
+// row.  A forward alone needs no place for a row once it is summed, and has three on their way.
+//
+// Vectors are counted from the 16-byte boundary at or before the row's start: the first and
+// last may hold neighbours' elements, which are read (they share 16 bytes with the row) and
+// left out.
+constexpr int kPieces = 8;  // vectors per thread and row
+constexpr int kRows = 3;    // rows in the ring
+constexpr int kHeld = 512;  // threads per SM that the ring has room for
+
+struct RowOut {  // what a row leaves besides its gradient; all nullable
+  float* logp;
+  double* lp64;
+  float2* stats;
+  float* coef0;
+  Terms terms;
+};
+template <bool GRAD>
+ECO_DEV void row_out(const RowOut& O, int64_t r, double lp, float2 st, const Token& t) {
+  if (O.logp) O.logp[r] = (float)lp;
+  if (O.lp64) O.lp64[r] = lp;
+  if (O.stats) O.stats[r] = st;
+  if (O.coef0) O.coef0[r] = 0.0f;
+  if (GRAD) put(O.terms, r, t.loss, t.kl, t.clipped ? 1.0f : 0.0f);
+}
+
+// Offsets of every step-th row without a division per row.
+struct Cursor {
+  int r, i, n1, step, step_i;
+  int64_t off, step_off, carry;
+  ECO_DEV Cursor(const Rows& R, int first, int step_, int64_t s0, int64_t s1) {
+    n1 = (int)R.n1;
+    r = first;
+    step = step_;
+    const int o = n1 == (int)R.rows ? 0 : first / n1, so = n1 == (int)R.rows ? 0 : step / n1;
+    i = first - o * n1;
+    step_i = step - so * n1;
+    off = o * s0 + i * s1;
+    step_off = so * s0 + step_i * s1;
+    carry = n1 == (int)R.rows ? 0 : s0 - n1 * s1;
+  }
+  ECO_DEV void next() {
+    r += step;
+    i += step_i;
+    off += step_off;
+    if (i >= n1) {
+      i -= n1;
+      off += carry;
+    }
+  }
+};
+
+template <typename T, int NT, bool GRAD>
+__global__ void __launch_bounds__(NT, kHeld / NT)
+    held_rows_kernel(const __grid_constant__ Rows R, const __grid_constant__ Policy P, const int* counts, float gain,
+                     const __grid_constant__ RowOut O, const __grid_constant__ Grad G) {
   using GT = typename RowIo<T>::G;
-  __shared__ MaxSum sh[NT > 32 ? NT / 32 : 1];
-  __shared__ int counts_sh[32];
-  __shared__ float coef_sh;
-  const double denom = policy_denom(R, P.denom, counts_sh);
-  const int tid = threadIdx.x % NT;
-  for (int64_t r = (int64_t)blockIdx.x * (blockDim.x / NT) + threadIdx.x / NT; r < R.rows;
-       r += (int64_t)gridDim.x * (blockDim.x / NT)) {
-    const T* x = static_cast<const T*>(R.x) + R.at(r, R.s0, R.s1);
-    GT* g = static_cast<GT*>(G.g) + R.at(r, G.s0, G.s1);
-    if (!R.counts(r)) {
-      row_zero<T, NT>(x, g, R.cols, tid, INT64_MAX);
-      if (tid == 0) {
-        logp[r] = 0.0f;
-        put(terms, r, 0.0f, 0.0f, 0.0f);
+  constexpr int E = RowIo<T>::E, W = NT / 32;
+  extern __shared__ __align__(16) uint4 ring[];  // [kRows][kPieces][NT]
+  __shared__ MaxSum warp_part[2][W];
+  __shared__ Slope row_sh[2];
+  __shared__ int counts_sh[W];
+  const int tid = threadIdx.x, cols = (int)R.cols, rows = (int)R.rows, step = (int)gridDim.x;
+  const double inv_denom = GRAD ? 1.0 / policy_denom(R, P.denom, counts, counts_sh) : 1.0;
+  uint4* const mine = ring + tid;
+  const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
+
+  // A row on its way: its token (-1: it does not count) and the element its first vector
+  // starts at (0 .. E - 1 before the row).
+  struct Row {
+    int y, skew;
+  };
+  Cursor xc(R, blockIdx.x, step, R.s0, R.s1);  // the next row to be issued
+  // Its token and mask, loaded an iteration before they are looked at: no wait for them.
+  int64_t token;
+  bool kept;
+  auto look = [&](int r) {
+    token = -1;
+    kept = false;
+    if (r < rows) {
+      token = R.tokens[r];
+      kept = (!R.mask || R.mask[r]) && (!R.cu || (r >= R.cu[0] && r < R.cu[R.nseq]));
+    }
+  };
+  auto issue = [&](int slot) {
+    Row w{-1, 0};
+    if (kept && token >= 0 && token < cols) {
+      const T* x = static_cast<const T*>(R.x) + xc.off;
+      w.y = (int)token;
+      w.skew = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
+      const uint4* src = reinterpret_cast<const uint4*>(x - w.skew) + tid;
+      const int left = (w.skew + cols + E - 1) / E - tid;  // vectors from mine on
+      const uint32_t d = mine_s + slot * (kPieces * NT * 16);
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+        if (p * NT < left)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + p * NT * 16), "l"(src + p * NT) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    xc.next();
+    look(xc.r);
+    return w;
+  };
+  // The row's vectors [first, whole) lie within it; one before and one behind may hold others'
+  // elements and are worked on by the thread that has them, one element at a time.
+  auto sum = [&](int slot, Row w) {
+    MaxSum a{-INFINITY, 0.0f};
+    if (w.y < 0) return a;
+    const uint4* at = mine + slot * (kPieces * NT);
+    const int first = w.skew > 0, end = w.skew + cols, whole = end / E - tid;
+#pragma unroll
+    for (int q = 0; q < kPieces; q += 4) {
+      if (q * NT < whole) {
+        uint4 raw[4];
+        bool in[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          in[p] = (q + p) * NT < whole && (q + p) * NT + tid >= first;
+          raw[p] = at[(q + p) * NT];
+        }
+        if (in[0] && in[3])
+          take_vectors<T, true, 4>(a, raw, in, R.c);
+        else
+          take_vectors<T, false, 4>(a, raw, in, R.c);
       }
-      continue;
     }
-    const int64_t y = R.tokens[r];
-    const float raw_y = tid == 0 ? to_f32(x[y]) : 0.0f;
-    const MaxSum a = row_stats<T, NT>(x, R.cols, R.c, tid, sh);
-    float coef = 0.0f;
+    if (w.skew > 0 || end % E) {
+      const int last = end / E;
+#pragma unroll 1
+      for (int k = 0; k < 2; ++k) {
+        const int v = k ? last : 0;
+        if (k ? (end % E == 0 || (last == 0 && w.skew > 0)) : w.skew == 0) continue;
+        if (v % NT != tid) continue;
+        float f[E];
+        RowIo<T>::unpack(at[v / NT * NT], f);
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (v * E + i < w.skew || v * E + i >= end) f[i] = -INFINITY;
+        take<E>(a, f, R.c);
+      }
+    }
+    return a;
+  };
+  // Warps' parts of a row to its scalars (warp 0): the row's results, and for the gradient what
+  // every thread needs.
+  auto finish = [&](int par, int r, int y, float raw_y, const Given& v) {
+    MaxSum a = warp_part[par][tid % W];
+    if (W > 1) a = lanes_join<W>(a, R.c);
     if (tid == 0) {
-      const double lp = token_logp(raw_y, a, R.mul);
-      const Token t = policy_token(P, r, lp);
-      logp[r] = (float)lp;
-      put(terms, r, t.loss, t.kl, t.clipped ? 1.0f : 0.0f);
-      coef = (float)((double)t.coef / denom) * gain;
-      if (NT > 32) coef_sh = coef;
+      double lp = 0.0;
+      float inv = 0.0f, off = 0.0f, coef = 0.0f;
+      Token t{0.0f, 0.0f, 0.0f, false};
+      if (y >= 0) {
+        lp = token_logp(raw_y, a, R.mul);
+        off = row_off(a.m);
+        inv = 1.0f / a.s;
+        if (GRAD) {
+          t = policy_token(P, v, lp);
+          coef = over(t.coef, inv_denom, gain);
+        }
+      }
+      if (GRAD) row_sh[par] = slope_of(off, R.c.hi, coef * inv, coef);
+      row_out<GRAD>(O, r, lp, make_float2(off, inv), t);
     }
-    if (NT > 32) {
-      __syncthreads();
-      coef = coef_sh;
-      __syncthreads();  // coef_sh and sh are free again
+  };
+  auto raw_token = [&](const T* x, int y) { return tid == 0 && y >= 0 ? to_f32(x[y]) : 0.0f; };
+  auto given = [&](int r, int y) {
+    return GRAD && tid == 0 && y >= 0 ? given_of(P, r) : Given{0.0f, 0.0f, 0.0f};
+  };
+
+  look(blockIdx.x);
+  Cursor gc(R, blockIdx.x, step, GRAD ? G.s0 : R.s0, GRAD ? G.s1 : R.s1);  // the row in work
+  Cursor rc(R, blockIdx.x, step, R.s0, R.s1);                             // its logits, for the token's own
+  Row w0 = issue(0), w1 = issue(1), w2 = issue(2), w3{-1, 0};
+  float raw0 = raw_token(static_cast<const T*>(R.x) + rc.off, w0.y), raw1 = 0.0f;
+  Given v0 = given(rc.r, w0.y), v1{0.0f, 0.0f, 0.0f};
+  if (gc.r < rows) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kRows - 1) : "memory");
+    const MaxSum a = lanes_join<32>(sum(0, w0), R.c);
+    if (!GRAD) w3 = issue(0);
+    if ((tid & 31) == 0) warp_part[0][tid >> 5] = a;
+    if (W > 1) __syncthreads(); else __syncwarp();
+  }
+  int slot = 0;
+  for (int par = 0; gc.r < rows; par ^= 1) {
+    const int slot1 = slot == kRows - 1 ? 0 : slot + 1;
+    if (tid < 32) finish(par, gc.r, w0.y, raw0, v0);
+    rc.next();
+    if (rc.r < rows) {
+      raw1 = raw_token(static_cast<const T*>(R.x) + rc.off, w1.y);
+      v1 = given(rc.r, w1.y);
+      asm volatile("cp.async.wait_group %0;" ::"n"(GRAD ? kRows - 2 : kRows - 1) : "memory");
+      const MaxSum a = lanes_join<32>(sum(slot1, w1), R.c);
+      if ((tid & 31) == 0) warp_part[par ^ 1][tid >> 5] = a;
+    }
+    if (W > 1) __syncthreads(); else __syncwarp();  // row i's scalars, row i + 1's warps
+    Row w4{-1, 0};
+    if (GRAD) {
+      const Slope c = row_sh[par];
+      GT* g = static_cast<GT*>(G.g) + gc.off;
+      // a row that does not count was not looked at: its gradient starts as its logits do
+      const int skew = (int)((reinterpret_cast<uintptr_t>(g) / sizeof(GT)) & (E - 1));
+      const bool zero = w0.y < 0 || c.coef == 0.0f;
+      const uint4* at = mine + slot * (kPieces * NT);
+      const int first = skew > 0, end = skew + cols, whole = end / E - tid;
+      GT* gv = g - skew + tid * E;
+      if (zero) {
+        const float f[E] = {};
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+          if (p * NT < whole && p * NT + tid >= first) RowIo<T>::store(gv, p * NT, f);
+      } else {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p)
+          if (p * NT < whole && p * NT + tid >= first) store_slope<T, true>(gv, p * NT, at[p * NT], c);
+      }
+      if (skew > 0 || end % E) {
+        const int last = end / E;
+#pragma unroll 1
+        for (int k = 0; k < 2; ++k) {
+          const int v = k ? last : 0;
+          if (k ? (end % E == 0 || (last == 0 && skew > 0)) : skew == 0) continue;
+          if (v % NT != tid) continue;
+          const T* xs = reinterpret_cast<const T*>(at + v / NT * NT);
+#pragma unroll 1
+          for (int i = 0; i < E; ++i)
+            if (v * E + i >= skew && v * E + i < end)
+              g[v * E + i - skew] = from_f32<GT>(zero ? 0.0f : slope_at(to_f32(xs[i]), c, false));
+        }
+      }
+      if (!zero) {  // the token's element, by the thread that has written its vector
+        const int v = (w0.y + skew) / E;
+        if (v % NT == tid) {
+          const float xy = to_f32(reinterpret_cast<const T*>(at + v / NT * NT)[(w0.y + skew) % E]);
+          g[w0.y] = from_f32<GT>(slope_at(xy, c, true));
+        }
+      }
+      w3 = issue(slot);
     } else {
-      coef = __shfl_sync(0xffffffffu, coef, 0);
+      w4 = issue(slot1);
     }
-    if (coef == 0.0f)
-      row_zero<T, NT>(x, g, R.cols, tid, INT64_MAX);
-    else
-      row_grad<T, NT>(x, g, R.cols, R.c, row_off(a.m), coef * (1.0f / a.s), coef, y, tid, INT64_MAX);
+    slot = slot1;
+    gc.next();
+    w0 = w1, w1 = w2, w2 = w3, w3 = w4;
+    raw0 = raw1;
+    v0 = v1;
+  }
+}
+
+// ------------------------------------------------ wider rows
+// The forward alone: one CTA per row.
+constexpr int kWide = 512;
+
+template <typename T>
+__global__ void __launch_bounds__(kWide, 3)
+    wide_logp_kernel(const __grid_constant__ Rows R, const __grid_constant__ RowOut O) {
+  __shared__ MaxSum sh[kWide / 32];
+  const int tid = threadIdx.x;
+  for (int64_t r = blockIdx.x; r < R.rows; r += gridDim.x) {
+    double lp = 0.0;
+    float2 st = make_float2(0.0f, 0.0f);
+    if (R.counts(r)) {
+      const T* x = static_cast<const T*>(R.x) + R.at(r, R.s0, R.s1);
+      const float raw_y = tid == 0 ? to_f32(x[R.tokens[r]]) : 0.0f;
+      const RowSplit sp = RowIo<T>::split(x, R.cols);
+      const float f[1] = {tid < sp.head + sp.tail ? to_f32(x[sp.edge(tid, R.cols)]) : -INFINITY};
+      MaxSum a{-INFINITY, 0.0f};
+      take_run<T, 4, false>(a, reinterpret_cast<const uint4*>(x + sp.head) + tid, kWide,
+                            run_length<kWide>((int)sp.vecs, tid), R.c);
+      if (tid < sp.head + sp.tail) take<1>(a, f, R.c);
+      a = lanes_join<32>(a, R.c);
+      if ((tid & 31) == 0) sh[tid >> 5] = a;
+      __syncthreads();
+      if (tid < 32) a = lanes_join<kWide / 32>(sh[tid % (kWide / 32)], R.c);
+      if (tid == 0) {
+        lp = token_logp(raw_y, a, R.mul);
+        st = make_float2(row_off(a.m), 1.0f / a.s);
+      }
+      __syncthreads();  // sh is free again
+    }
+    if (tid == 0) row_out<false>(O, r, lp, st, Token{});
+  }
+}
+
+// The whole policy loss.  The first kPlaces vectors per thread of a row stay in shared memory, the rest is read again
+// for the gradient, from L2: the launch lets no more rows be in work than L2 holds the rests of.
+// As soon as a place has been used for the last time, the next row's vector is copied there
+// (cp.async by the thread that will use it), so memory is read while the end of a row is
+// summed, joined and written.
+constexpr int kPlaces = 12;
+constexpr int kBatch = 4;  // vectors read again at a time
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT)
+    wide_rows_kernel(const __grid_constant__ Rows R, const __grid_constant__ Policy P, const int* counts, float gain,
+                     const __grid_constant__ RowOut O, const __grid_constant__ Grad G) {
+  using GT = typename RowIo<T>::G;
+  using Io = RowIo<T>;
+  constexpr int E = Io::E, W = NT / 32;
+  extern __shared__ __align__(16) uint4 places[];  // [kPlaces][NT]
+  __shared__ MaxSum sh[W];
+  __shared__ Slope row_sh;
+  __shared__ int counts_sh[W];
+  const int tid = threadIdx.x, cols = (int)R.cols, rows = (int)R.rows, step = (int)gridDim.x;
+  const double inv_denom = 1.0 / policy_denom(R, P.denom, counts, counts_sh);
+  uint4* const mine = places + tid;
+  const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
+  Cursor xc(R, blockIdx.x, step, R.s0, R.s1);  // one row ahead of gc after the first fill
+  Cursor gc(R, blockIdx.x, step, G.s0, G.s1);
+  int64_t token = -1;
+  bool kept = false;
+  auto look = [&](int r) {  // loads only; looked at when the row's copies start
+    token = -1;
+    kept = false;
+    if (r < rows) {
+      token = R.tokens[r];
+      kept = (!R.mask || R.mask[r]) && (!R.cu || (r >= R.cu[0] && r < R.cu[R.nseq]));
+    }
+  };
+  struct Row {
+    const T* x;
+    int y, vecs, head;
+  };
+  auto next_row = [&]() {  // the row xc stands at
+    Row w{static_cast<const T*>(R.x) + xc.off, -1, 0, 0};
+    if (kept && token >= 0 && token < cols) {
+      const RowSplit sp = Io::split(w.x, cols);
+      w.y = (int)token;
+      w.vecs = (int)sp.vecs;
+      w.head = sp.head;
+    }
+    return w;
+  };
+  auto copy = [&](const Row& w, int p) {
+    if (p * NT + tid < w.vecs)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine_s + p * NT * 16),
+                   "l"(reinterpret_cast<const uint4*>(w.x + w.head) + p * NT + tid)
+                   : "memory");
+  };
+  look(xc.r);
+  Row w = next_row();
+#pragma unroll
+  for (int p = 0; p < kPlaces; ++p) copy(w, p);
+  asm volatile("cp.async.commit_group;" ::: "memory");
+  xc.next();
+  look(xc.r);
+  for (; gc.r < rows; gc.next()) {
+    const int tail = cols - w.head - w.vecs * E, edges = w.y < 0 ? 0 : w.head + tail;
+    const T* body = w.x + w.head;
+    float raw_y = 0.0f, edge = 0.0f;
+    Given v{0.0f, 0.0f, 0.0f};
+    const int edge_at = tid < w.head ? tid : cols - tail + tid - w.head;
+    if (w.y >= 0) {
+      if (tid == 0) {
+        raw_y = to_f32(w.x[w.y]);
+        v = given_of(P, gc.r);
+      }
+      if (tid < edges) edge = to_f32(w.x[edge_at]);
+    }
+    const Row nw = next_row();
+    MaxSum a{-INFINITY, 0.0f};
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (w.y >= 0) {
+      const int run = run_length<NT>(w.vecs, tid), here = run < kPlaces ? run : kPlaces;
+      take_run<T, kBatch, true>(a, mine, NT, here, R.c);
+      take_run<T, kBatch, false>(a, reinterpret_cast<const uint4*>(body) + kPlaces * NT + tid, NT, run - kPlaces, R.c);
+      if (tid < edges) {
+        const float f[1] = {edge};
+        take<1>(a, f, R.c);
+      }
+    }
+    xc.next();
+    look(xc.r);
+    a = lanes_join<32>(a, R.c);
+    if ((tid & 31) == 0) sh[tid >> 5] = a;
+    __syncthreads();
+    if (tid < 32) {
+      a = lanes_join<W>(sh[tid % W], R.c);
+      if (tid == 0) {
+        double lp = 0.0;
+        float inv = 0.0f, off = 0.0f, coef = 0.0f;
+        Token t{0.0f, 0.0f, 0.0f, false};
+        if (w.y >= 0) {
+          lp = token_logp(raw_y, a, R.mul);
+          off = row_off(a.m);
+          inv = 1.0f / a.s;
+          t = policy_token(P, v, lp);
+          coef = over(t.coef, inv_denom, gain);
+        }
+        row_sh = slope_of(off, R.c.hi, coef * inv, coef);
+        row_out<true>(O, gc.r, lp, make_float2(off, inv), t);
+      }
+    }
+    __syncthreads();  // row_sh, and sh is free again
+    {
+      const Slope c = row_sh;
+      GT* g = static_cast<GT*>(G.g) + gc.off;
+      const bool zero = w.y < 0 || c.coef == 0.0f;
+      // a row that does not count was not split: its gradient starts as its logits do
+      const RowSplit sp = Io::split(w.x, cols);
+      GT* gb = g + sp.head;
+      const int vecs = (int)sp.vecs;
+      const int run = run_length<NT>(vecs, tid);
+      GT* gp = gb + tid * E;
+      if (zero) {
+        const float f[E] = {};
+        for (int p = 0; p < run; ++p, gp += NT * E) Io::store(gp, 0, f);
+#pragma unroll
+        for (int p = 0; p < kPlaces; ++p) copy(nw, p);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      } else {
+#pragma unroll
+        for (int p = 0; p < kPlaces; ++p) {
+          if (p < run) store_slope<T, true>(gp, p * NT, mine[p * NT], c);
+          copy(nw, p);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const uint4* xp = reinterpret_cast<const uint4*>(body) + kPlaces * NT + tid;
+        gp += kPlaces * NT * E;
+        for (int left = run - kPlaces; left > 0; left -= kBatch, xp += kBatch * NT, gp += kBatch * NT * E) {
+          uint4 raw[kBatch];
+#pragma unroll
+          for (int p = 0; p < kBatch; ++p)
+            if (p < left) raw[p] = __ldcs(xp + p * NT);
+#pragma unroll
+          for (int p = 0; p < kBatch; ++p) {
+            if (p < left) store_slope<T, true>(gp, p * NT, raw[p], c);
+          }
+        }
+      }
+      if (tid < sp.head + sp.tail) {
+        const int j = (int)sp.edge(tid, cols);
+        g[j] = from_f32<GT>(zero ? 0.0f : slope_at(edge, c, j == w.y));
+      }
+      const int yv = w.y - sp.head;  // the token's element, by the thread that has written its vector
+      if (!zero && yv >= 0 && yv / E < vecs && yv / E % NT == tid)
+        g[w.y] = from_f32<GT>(slope_at(to_f32(w.x[w.y]), c, true));
+    }
+    w = nw;
   }
 }
 
@@ -370,10 +818,10 @@ ECO_DEV double cta_sum(double v, double* sh) {
 
 // loss, kl and clip fraction from the rows' terms (one CTA, fixed order, sums in double).
 __global__ void __launch_bounds__(1024) policy_finish_kernel(const __grid_constant__ Rows R, const Terms terms,
-                                                              double denom, float* out) {
+                                                              double denom, const int* counts, float* out) {
   __shared__ double sh[32];
   __shared__ int counts_sh[32];
-  const double n = policy_denom(R, denom, counts_sh);
+  const double n = policy_denom(R, denom, counts, counts_sh);
   double a = 0.0, b = 0.0, d = 0.0;
   for (int64_t r = threadIdx.x; r < R.rows; r += blockDim.x) {
     a += terms.loss[r];
@@ -396,16 +844,16 @@ __global__ void __launch_bounds__(1024) policy_tokens_kernel(const __grid_consta
                                                               float* coef, float* out) {
   __shared__ double sh[32];
   __shared__ int counts_sh[32];
-  const double n = policy_denom(R, P.denom, counts_sh);
+  const double n = policy_denom(R, P.denom, nullptr, counts_sh), inv = 1.0 / n;
   double a = 0.0, b = 0.0, d = 0.0;
   for (int64_t r = threadIdx.x; r < R.rows; r += blockDim.x) {
     float k = 0.0f;
     if (R.counts(r)) {
-      const Token t = policy_token(P, r, lp64[r]);
+      const Token t = policy_token(P, given_of(P, r), lp64[r]);
       a += t.loss;
       b += t.kl;
       d += t.clipped ? 1.0 : 0.0;
-      k = (float)((double)t.coef / n);
+      k = over(t.coef, inv, 1.0f);
     }
     coef[r] = k;
   }
@@ -502,7 +950,10 @@ Rows rows_of(const eco_logits_t& L, const int64_t* tokens, const uint8_t* mask, 
   R.s1 = L.s1;
   R.cols = L.cols;
   R.mul = L.mul;
-  R.c = (float)(L.mul * 1.4426950408889634);
+  const double c = L.mul * 1.4426950408889634;
+  R.c.hi = std::nextafter((float)c, 0.0f);  // below c: the rest is positive, and -inf times it is -inf
+  if ((double)R.c.hi >= c) R.c.hi = std::nextafter(R.c.hi, 0.0f);
+  R.c.lo = (float)(c - (double)R.c.hi);
   R.tokens = tokens;
   R.mask = mask;
   R.cu = cu;
@@ -525,26 +976,20 @@ int check_logits(const eco_logits_t* L, const int64_t* tokens, const char* who) 
   return ECO_OK;
 }
 
-// A gradient row starts at the logits row's address modulo 16 bytes (so 16-byte vectors of
-// both hold the same elements), and on 16 bytes for int8 logits.
+// A 16-byte vector of logits and the vector of as many gradient elements hold the same
+// elements: every gradient row starts as many elements behind such a boundary as its logits row.
 int check_grad(const eco_logits_t& L, const eco_grad_t* G, const char* who) {
   ECO_REQUIRE(G && G->g && G->s0 >= 0 && G->s1 >= 0 && (L.n1 <= 1 || G->s1 >= L.cols) &&
                   (L.n0 <= 1 || G->s0 >= L.cols),
               ECO_ERR_ARG, "%s: bad gradient layout", who);
-  const int64_t es = esize(L.type);
-  const int64_t base = reinterpret_cast<uintptr_t>(G->g);
-  bool ok;
-  if (L.type == ECO_I8)
-    ok = base % 16 == 0 && (L.n0 <= 1 || G->s0 % 4 == 0) && (L.n1 <= 1 || G->s1 % 4 == 0);
-  else
-    ok = (base - (int64_t) reinterpret_cast<uintptr_t>(L.x)) % 16 == 0 &&
-         (L.n0 <= 1 || (G->s0 - L.s0) * es % 16 == 0) && (L.n1 <= 1 || (G->s1 - L.s1) * es % 16 == 0);
-  ECO_REQUIRE(ok, ECO_ERR_MISALIGNED, "%s: gradient rows must start like the logits rows modulo 16 bytes", who);
+  const int64_t es = esize(L.type), ges = es == 1 ? 4 : es, per = 16 / es;
+  const int64_t xb = (int64_t) reinterpret_cast<uintptr_t>(L.x), gb = (int64_t) reinterpret_cast<uintptr_t>(G->g);
+  ECO_REQUIRE(gb % ges == 0 && (gb / ges - xb / es) % per == 0 && (L.n0 <= 1 || (G->s0 - L.s0) % per == 0) &&
+                  (L.n1 <= 1 || (G->s1 - L.s1) % per == 0),
+              ECO_ERR_MISALIGNED, "%s: gradient rows must start like the logits rows, modulo %d elements", who,
+              (int)per);
   return ECO_OK;
 }
-
-// Threads per row: a warp up to 1024 columns (no barrier; eight rows per CTA), a CTA beyond.
-int row_threads(int64_t cols) { return cols <= 1024 ? 32 : cols <= 8192 ? 128 : 512; }
 
 template <typename F>
 int by_type(int type, F f) {
@@ -556,20 +1001,51 @@ int by_type(int type, F f) {
   }
 }
 
-template <typename T, int NT>
-void launch_logp(const Rows& R, float* logp, double* lp64, float2* stats, float* coef0, cudaStream_t s) {
-  constexpr int threads = NT == 32 ? 256 : NT;
-  const int64_t grid = std::min<int64_t>((R.rows + threads / NT - 1) / (threads / NT), 1 << 20);
-  token_logp_kernel<T, NT><<<(unsigned)grid, threads, 0, s>>>(R, logp, lp64, stats, coef0);
+template <typename T, int NT, bool GRAD>
+bool launch_held(const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O, const Grad& G,
+                 cudaStream_t s) {
+  const auto kernel = held_rows_kernel<T, NT, GRAD>;
+  constexpr int smem = kRows * kPieces * NT * 16;
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return false;
+  const int64_t grid = std::min<int64_t>(R.rows, (int64_t)eco_num_sms() * (kHeld / NT));
+  kernel<<<(unsigned)grid, NT, smem, s>>>(R, P, counts, gain, O, G);
+  return true;
+}
+
+// Threads per CTA by the vectors of a row (at whatever alignment it starts): as few as hold it,
+// so that a row's fixed work is shared by as many of its elements as possible.
+constexpr int64_t kHeldVecs = 256 * kPieces;
+template <typename T>
+int64_t row_vecs(const Rows& R) {
+  constexpr int64_t E = RowIo<T>::E;
+  const bool on_16 = eco_aligned16(R.x) && (R.rows == R.n1 || R.s0 % E == 0) && (R.n1 <= 1 || R.s1 % E == 0);
+  return (R.cols + (on_16 ? 0 : E - 1) + E - 1) / E;
+}
+template <typename T, bool GRAD>
+bool by_vecs(int64_t vecs, const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O,
+             const Grad& G, cudaStream_t s) {
+  if (vecs <= 32 * kPieces) return launch_held<T, 32, GRAD>(R, P, counts, gain, O, G, s);
+  if (vecs <= 64 * kPieces) return launch_held<T, 64, GRAD>(R, P, counts, gain, O, G, s);
+  if (vecs <= 128 * kPieces) return launch_held<T, 128, GRAD>(R, P, counts, gain, O, G, s);
+  return launch_held<T, 256, GRAD>(R, P, counts, gain, O, G, s);
 }
 
 template <typename T, int NT>
-void launch_policy(const Rows& R, const Policy& P, float gain, float* logp, const Terms& t, const Grad& G,
-                   cudaStream_t s) {
-  constexpr int threads = NT == 32 ? 256 : NT;
-  const int64_t cap = (int64_t)eco_num_sms() * (1536 / threads);
-  const int64_t grid = std::min<int64_t>((R.rows + threads / NT - 1) / (threads / NT), cap);
-  policy_row_kernel<T, NT><<<(unsigned)grid, threads, 0, s>>>(R, P, gain, logp, t, G);
+bool launch_wide(const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O, const Grad& G,
+                 cudaStream_t s) {
+  const auto kernel = wide_rows_kernel<T, NT>;
+  constexpr int smem = kPlaces * NT * 16;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return false;
+  const int64_t grid = std::min<int64_t>(R.rows, (int64_t)eco_num_sms() * (1024 / NT));
+  kernel<<<(unsigned)grid, NT, smem, s>>>(R, P, counts, gain, O, G);
+  return true;
+}
+// Whether what the rows in work leave to L2 fits there: half of its 126 MB, since either die
+// keeps its own copy of what its SMs read.
+bool rests_fit(int64_t vecs, int threads) {
+  const int64_t rest = std::max<int64_t>(0, vecs - (int64_t)kPlaces * threads) * 16;
+  return rest * eco_num_sms() * (1024 / threads) <= (int64_t)56 << 20;
 }
 
 template <typename T>
@@ -580,7 +1056,7 @@ void launch_grad(const Rows& R, const float2* stats, const float* coef, const fl
     const int64_t grid = std::min<int64_t>((R.rows + 7) / 8, 1 << 20);
     token_grad_kernel<T, 32><<<(unsigned)grid, 256, 0, s>>>(R, stats, coef, scale, gain, G, INT64_MAX / 2);
   } else {
-    // segments of 2048 vectors (32 KB of logits), eight loads of each thread
+    // segments of 2048 vectors (32 kBatch of logits), eight loads of each thread
     const int64_t seg = 2048;
     const dim3 grid((unsigned)std::min<int64_t>(R.rows, 1 << 20), (unsigned)((vecs + seg - 1) / seg));
     token_grad_kernel<T, 256><<<grid, 256, 0, s>>>(R, stats, coef, scale, gain, G, seg);
@@ -598,14 +1074,18 @@ extern "C" int eco_token_logp(const eco_logits_t* logits, const int64_t* tokens,
   if (R.rows == 0) return ECO_OK;
   ECO_REQUIRE(logp || logp64, ECO_ERR_ARG, "eco_token_logp: no output");
   float2* st = reinterpret_cast<float2*>(row_stats);
+  bool ok = true;
   by_type(logits->type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int nt = row_threads(R.cols);
-    if (nt == 32) launch_logp<T, 32>(R, logp, logp64, st, coef_zero, eco_stream(stream));
-    else if (nt == 128) launch_logp<T, 128>(R, logp, logp64, st, coef_zero, eco_stream(stream));
-    else launch_logp<T, 512>(R, logp, logp64, st, coef_zero, eco_stream(stream));
+    const int64_t vecs = row_vecs<T>(R);
+    const RowOut O{logp, logp64, st, coef_zero, Terms{}};
+    if (vecs <= kHeldVecs)
+      ok = by_vecs<T, false>(vecs, R, Policy{}, nullptr, 0.0f, O, Grad{}, eco_stream(stream));
+    else
+      wide_logp_kernel<T><<<(unsigned)std::min<int64_t>(R.rows, 1 << 20), kWide, 0, eco_stream(stream)>>>(R, O);
     return 0;
   });
+  if (!ok) return eco_fail(ECO_ERR_LAUNCH, "eco_token_logp: %s", cudaGetErrorString(cudaGetLastError()));
   return eco_launch_check("eco_token_logp");
 }
 
@@ -653,15 +1133,25 @@ extern "C" int eco_policy_grad(const eco_logits_t* logits, const int64_t* tokens
   if (int rc = check_grad(*logits, grad, "eco_policy_grad")) return rc;
   const Grad G{grad->g, grad->s0, grad->s1};
   const Terms t{terms, terms + R.rows, terms + 2 * R.rows};
+  int* counts = nullptr;
+  if (!(denom > 0.0) && R.rows > kCountRows) {
+    counts = reinterpret_cast<int*>(terms + 3 * R.rows);
+    count_kernel<<<kCounts, 256, 0, s>>>(R, counts);
+  }
+  bool ok = true;
   by_type(logits->type, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    const int nt = row_threads(R.cols);
-    if (nt == 32) launch_policy<T, 32>(R, P, (float)gain, logp, t, G, s);
-    else if (nt == 128) launch_policy<T, 128>(R, P, (float)gain, logp, t, G, s);
-    else launch_policy<T, 512>(R, P, (float)gain, logp, t, G, s);
+    const int64_t vecs = row_vecs<T>(R);
+    const RowOut O{logp, nullptr, nullptr, nullptr, t};
+    if (vecs <= kHeldVecs)
+      ok = by_vecs<T, true>(vecs, R, P, counts, (float)gain, O, G, s);
+    else
+      ok = rests_fit(vecs, 512) ? launch_wide<T, 512>(R, P, counts, (float)gain, O, G, s)
+                                : launch_wide<T, 1024>(R, P, counts, (float)gain, O, G, s);
     return 0;
   });
-  policy_finish_kernel<<<1, 1024, 0, s>>>(R, t, denom, out);
+  if (!ok) return eco_fail(ECO_ERR_LAUNCH, "eco_policy_grad: %s", cudaGetErrorString(cudaGetLastError()));
+  policy_finish_kernel<<<1, 1024, 0, s>>>(R, t, denom, counts, out);
   return eco_launch_check("eco_policy_grad");
 }
 

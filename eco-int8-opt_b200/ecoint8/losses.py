@@ -19,8 +19,8 @@ row strides (``logits[:, :-1]`` is read in place) as long as the vocabulary is c
 Rows with a false ``mask`` or a token outside ``[0, vocab)`` (such as -100) do not count: their
 logits are not read and may hold anything, and their gradient is zero.  Sums over rows are
 taken in fp64 and in a fixed order: the same call gives the same bits.  A row of infinities or
-NaN that counts makes its results NaN.  The gradient of ``logits[b, t]`` starts at the same
-address modulo 16 bytes as that row, so gradients may come with padded strides.
+NaN that counts makes its results NaN.  A gradient row starts as far
+behind a vector boundary as its logits row does, so gradients may come with padded strides.
 """
 
 from __future__ import annotations
@@ -112,14 +112,12 @@ class _Rows:
         return t.contiguous()
 
     def new_grad(self):
-        """``(tensor, eco_grad_t)``: rows that start like the logits' rows modulo 16 bytes."""
+        """``(tensor, eco_grad_t)``: rows that start like the logits' rows, modulo a 16-byte vector of those."""
         x, cols = self.x, self.x.shape[-1]
         n0, n1 = self.spec.n0, self.spec.n1
-        if x.dtype == torch.int8:
-            dtype, per, want0, want1, skew = torch.float32, 4, 0, 0, 0
-        else:
-            dtype, per = x.dtype, 16 // x.element_size()
-            want0, want1, skew = self.spec.s0, self.spec.s1, x.data_ptr() % 16 // x.element_size()
+        dtype = torch.float32 if x.dtype == torch.int8 else x.dtype
+        es = x.element_size()
+        per, skew, want0, want1 = 16 // es, x.data_ptr() % 16 // es, self.spec.s0, self.spec.s1
         s1 = cols + (want1 - cols) % per
         s0 = n1 * s1 + (want0 - n1 * s1) % per if n0 > 1 else n1 * s1
         if skew == 0 and s1 == cols and s0 == n1 * s1:
@@ -234,7 +232,7 @@ def policy_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch
     keep, args = _policy_args(rows, old_logp, advantages, ref_logp, clip_low, clip_high, kl_coef, denom)
     with nat.on_device(rows.dev):
         g, spec = rows.new_grad()
-        logp, terms, out = rows.new(*rows.lead), rows.new(3, rows.rows), rows.new(3)
+        logp, terms, out = rows.new(*rows.lead), rows.new(3 * rows.rows + 64), rows.new(3)
         nat.call("eco_policy_grad", ctypes.byref(rows.spec), rows.tokens.data_ptr(), nat.ptr(rows.mask), *args,
                  rows.gain, logp.data_ptr(), terms.data_ptr(), out.data_ptr(), ctypes.byref(spec), nat.stream())
     loss, kl, clipped = out.unbind()

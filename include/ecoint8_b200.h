@@ -459,8 +459,8 @@ typedef struct {
 } eco_logits_t;
 
 /* The gradient's rows: the logits' type (fp32 for int8 logits), row strides in elements.
- * Every row has to start where the logits' row starts modulo 16 bytes (on 16 bytes for int8
- * logits). */
+ * Every row has to start as many elements behind a boundary of 16 / sizeof(logit) elements as
+ * the logits' row does (the same address modulo 16 bytes; four times that modulo 64 for int8). */
 typedef struct {
   void* g;
   int64_t s0, s1;
@@ -484,8 +484,8 @@ ECO_API int eco_token_grad(const eco_logits_t* logits, const int64_t* tokens, co
  *   r = exp(lp - old);  l = max(-A r, -A clip(r, low, high)) + kl_coef k
  *   k = exp(ref - lp) - (ref - lp) - 1  (0 without ref_logp)
  * out[0..2] = sum l / denom, sum k / denom, share of rows whose clipped term is the larger.
- * eco_policy_grad does all of it from the logits in two launches: logp [rows], terms float
- * [3, rows] (workspace), the gradient times gain.  eco_policy_tokens starts from fp64
+ * eco_policy_grad does all of it from the logits: logp [rows], terms float [3 rows + 64]
+ * (workspace), the gradient times gain.  eco_policy_tokens starts from fp64
  * log-probabilities and leaves each row's d loss / d lp in coef (for eco_token_grad). */
 ECO_API int eco_policy_grad(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
                             const float* old_logp, const float* adv, const float* ref_logp, double low,

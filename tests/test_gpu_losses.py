@@ -62,7 +62,8 @@ def _fp64(x, temperature=1.0):
 def _check_grad(got, want, x, coef, coef_err, unit, note=""):
     """|got - want| against the module's bound; ``coef`` fp64 per row, ``coef_err`` its absolute error."""
     p = torch.softmax(torch.nan_to_num(x), -1)
-    e = _err(x)[..., None]
+    # a 16-bit gradient's exponent takes in the coefficient: below 2^9 + 2^7 in size, rounded twice
+    e = _err(x)[..., None] + (2.0 ** -14 if got.dtype != torch.float32 else 0.0)
     c, ce = coef.abs()[..., None], coef_err[..., None]
     tiny = torch.finfo(got.dtype).tiny * torch.finfo(got.dtype).eps  # half of the smallest subnormal step, and ftz
     tol = want.abs() * _half_step(got.dtype) + (c * e * unit + ce * unit) * (p + (want.abs() > c * 0.5 * unit)) + \

@@ -134,9 +134,9 @@ def test_token_objectives_refuse_bad_arguments():
     call = lambda g, **how: lib.eco_token_grad(_logits_spec(**how), 8192, 8192, 8192, None, 1.0, g, None)  # noqa: E731
     _refused(call(grad(None, 0, 64)), -1, "gradient layout")
     _refused(call(grad(8192, 0, 32)), -1, "gradient layout")
-    _refused(call(grad(8194, 0, 64)), -2, "modulo 16")
-    _refused(call(grad(8192, 0, 65)), -2, "modulo 16")
-    _refused(call(grad(8196, 0, 64), type=nat.I8), -2, "modulo 16")
+    _refused(call(grad(8194, 0, 64)), -2, "modulo 8 elements")
+    _refused(call(grad(8192, 0, 65)), -2, "modulo 8 elements")
+    _refused(call(grad(8196, 0, 64), type=nat.I8), -2, "modulo 16 elements")
     _refused(lib.eco_token_grad(_logits_spec(), 8192, None, 8192, None, 1.0, grad(8192, 0, 64), None), -1, "statistics")
     policy = lambda lo, hi, kl, old=8192, dn=0.0: lib.eco_policy_grad(  # noqa: E731
         _logits_spec(), 8192, None, old, 8192, None, lo, hi, kl, dn, 1.0, 8192, 8192, 8192, grad(8192, 0, 64), None)
