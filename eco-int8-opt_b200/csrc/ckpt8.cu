@@ -33,53 +33,51 @@ struct Oct {
 };
 
 // Columns [c, c + n) of a row, n in [0, 8]; the others are zeros.  A row that does not start
-// on 16 bytes is read by the 16-byte words that hold its eight columns, shifted into place
-// (each of them holds at least one of the eight, so none lies outside the row's memory).
+// on 16 bytes (32 for fp32) is read by the 16-byte words that hold its columns, shifted into
+// place (each word that is read holds at least one of them, so none lies outside the row's memory).
 template <typename T>
 ECO_DEV Oct<T> load8(const T* row, int64_t c, int n) {
-  constexpr int V = Oct<T>::W / 4;  // 16-byte words
+  constexpr int W = Oct<T>::W, V = W / 4;  // 32-bit words, 16-byte words
   Oct<T> o;
-  if (n == 8) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
-    const uint4* p = reinterpret_cast<const uint4*>(a & ~uintptr_t(15));
-    const uint32_t skew = (uint32_t)a & 15;
-    if (skew == 0) {
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        const uint4 t = __ldg(p + v);
-        o.w[4 * v] = t.x, o.w[4 * v + 1] = t.y, o.w[4 * v + 2] = t.z, o.w[4 * v + 3] = t.w;
-      }
-      return o;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
+  if (n == 8 && (a & (16 * V - 1)) == 0) {
+    if constexpr (V == 2) {
+      asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+          : "=r"(o.w[0]), "=r"(o.w[1]), "=r"(o.w[2]), "=r"(o.w[3]), "=r"(o.w[4]), "=r"(o.w[5]), "=r"(o.w[6]), "=r"(o.w[7])
+          : "l"(row + c));
+    } else {
+      const uint4 t = __ldg(reinterpret_cast<const uint4*>(row + c));
+      o.w[0] = t.x, o.w[1] = t.y, o.w[2] = t.z, o.w[3] = t.w;
     }
-    uint32_t w[4 * V + 4];
-#pragma unroll
-    for (int v = 0; v <= V; ++v) {
-      const uint4 t = __ldg(p + v);
-      w[4 * v] = t.x, w[4 * v + 1] = t.y, w[4 * v + 2] = t.z, w[4 * v + 3] = t.w;
-    }
-    if (skew & 8) {
-#pragma unroll
-      for (int i = 0; i < 4 * V + 2; ++i) w[i] = w[i + 2];
-    }
-    if (skew & 4) {
-#pragma unroll
-      for (int i = 0; i < 4 * V + 1; ++i) w[i] = w[i + 1];
-    }
-    const uint32_t bits = (skew & 3) * 8;
-#pragma unroll
-    for (int i = 0; i < 4 * V; ++i) o.w[i] = __funnelshift_r(w[i], w[i + 1], bits);
     return o;
   }
+  const uint4* p = reinterpret_cast<const uint4*>(a & ~uintptr_t(15));
+  const uint32_t skew = (uint32_t)a & 15;
+  const int end = n > 0 ? (int)skew + n * (int)sizeof(T) : 0;  // bytes that are needed, from p on
+  uint32_t w[W + 4];
 #pragma unroll
-  for (int i = 0; i < Oct<T>::W; ++i) o.w[i] = 0u;
+  for (int v = 0; v <= V; ++v) {
+    uint4 t = make_uint4(0u, 0u, 0u, 0u);
+    if (16 * v < end) t = __ldg(p + v);
+    w[4 * v] = t.x, w[4 * v + 1] = t.y, w[4 * v + 2] = t.z, w[4 * v + 3] = t.w;
+  }
+  if (skew & 8) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) {
-      if constexpr (sizeof(T) == 4)
-        o.w[i] = __float_as_uint(row[c + i]);
-      else
-        o.w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(row + c + i)) << (16 * (i & 1));
-    }
+    for (int i = 0; i < W + 2; ++i) w[i] = w[i + 2];
+  }
+  if (skew & 4) {
+#pragma unroll
+    for (int i = 0; i < W + 1; ++i) w[i] = w[i + 1];
+  }
+  const uint32_t bits = (skew & 3) * 8;
+#pragma unroll
+  for (int i = 0; i < W; ++i) {  // columns past the n-th are the row's neighbours: zeros here
+    o.w[i] = __funnelshift_r(w[i], w[i + 1], bits);
+    if constexpr (sizeof(T) == 4)
+      o.w[i] = i < n ? o.w[i] : 0u;
+    else
+      o.w[i] = 2 * i + 1 < n ? o.w[i] : (2 * i < n ? o.w[i] & 0xffffu : 0u);
+  }
   return o;
 }
 
@@ -96,18 +94,17 @@ ECO_DEV void unpack8(const Oct<T>& o, float (&f)[8]) {
   }
 }
 
-// Eight columns of an output row: whole vectors where the row starts on 16 bytes (its
-// padding takes the rest of a last vector), else n single stores.
+// Eight columns of an output row: whole where eight columns of the row start on a boundary of
+// their size (its padding takes the rest of the last eight), else n single stores.
 template <typename T>
 ECO_DEV void store8(T* row, int64_t c, int n, bool vec, const float (&f)[8]) {
   if (vec) {
-    uint4* p = reinterpret_cast<uint4*>(row + c);
     if constexpr (sizeof(T) == 4) {
-      const float a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
-      p[0] = RowIo<T>::pack(a);
-      if (n > 4) p[1] = RowIo<T>::pack(b);
+      asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c), "f"(f[0]), "f"(f[1]),
+                   "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                   : "memory");
     } else {
-      p[0] = RowIo<T>::pack(f);
+      *reinterpret_cast<uint4*>(row + c) = RowIo<T>::pack(f);
     }
     return;
   }
@@ -122,14 +119,27 @@ ECO_DEV float max_nan(float a, float b) {  // NaN if either is
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
   return d;
 }
-// max |x| of a block over its 16 lanes.
-ECO_DEV float block_amax(const float (&f)[8]) {
-  float m = fabsf(f[0]);
+// max |x| of a block over its 16 lanes.  Without their signs, numbers order like their bits, NaN
+// above infinity: an integer maximum, two 16-bit numbers at a time.
+template <typename T>
+ECO_DEV float block_amax(const Oct<T>& o) {
+  if constexpr (sizeof(T) == 4) {
+    float m = fabsf(__uint_as_float(o.w[0]));
 #pragma unroll
-  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(f[i]));
+    for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(__uint_as_float(o.w[i])));
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
+    for (int s = 8; s > 0; s >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, s));
+    return m;
+  } else {
+    uint32_t m = o.w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = __vmaxu2(m, o.w[i] & 0x7fff7fffu);
+#pragma unroll
+    for (int s = 8; s > 0; s >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, s));
+    m = max(m & 0xffffu, m >> 16);
+    if constexpr (std::is_same_v<T, __nv_bfloat16>) return __uint_as_float(m << 16);
+    else return __half2float(__ushort_as_half((unsigned short)m));
+  }
 }
 // Gains of N blocks of a half-warp from their maxima, and in lane i (< N) the scale of block i:
 // lane i does block i's two divisions, so that N blocks cost the divisions of one.
@@ -193,7 +203,8 @@ struct Tile {
 // Loops over (row, block) in groups of U rows, whose loads are all issued before the first is
 // used (a thread has one or two 16-byte loads per row: alone they would not cover the memory's
 // latency).  Both halves of a warp stay in step (the shuffles need all 32 lanes): lanes past the
-// last row or column get n = 0 columns.  load(r, c, n) -> L;  use(L[U], r[U], n[U], b, c).
+// last row or column get n = 0 columns, blocks past the last row or block `live` = false.
+// load(r, c, n) -> L;  use(L[U], r[U], n[U], live[U], b, c).
 template <int U, typename L, typename Load, typename Use>
 ECO_DEV void for_blocks(int64_t rows, int64_t cols, int bpr_log2, Load load, Use use) {
   const Tile t(cols, bpr_log2);
@@ -204,14 +215,17 @@ ECO_DEV void for_blocks(int64_t rows, int64_t cols, int bpr_log2, Load load, Use
       L l[U];
       int64_t r[U];
       int n[U];
+      bool live[U];
+      const int most = b < t.blocks ? left8(cols, c) : 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         r[u] = r0 + u * t.row_step;
-        n[u] = r[u] < rows && b < t.blocks ? left8(cols, c) : 0;
-        if (n[u] == 0) r[u] = 0;
+        live[u] = r[u] < rows && b < t.blocks;
+        n[u] = live[u] ? most : 0;
+        if (!live[u]) r[u] = 0;
         l[u] = load(r[u], c, n[u]);
       }
-      use(l, r, n, b, c);
+      use(l, r, n, live, b, c);
     }
 }
 
@@ -221,23 +235,17 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(Mat x, int64_t rows, int
   for_blocks<U, Oct<T>>(
       rows, cols, bpr_log2,
       [&](int64_t r, int64_t c, int n) { return load8(static_cast<const T*>(x.p) + r * x.ld, c, n); },
-      [&](const Oct<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
+      [&](const Oct<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
         float f[8], amax[U], gain[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          unpack8(o[u], f);
-          amax[u] = block_amax(f);
-        }
+        for (int u = 0; u < U; ++u) amax[u] = block_amax(o[u]);
         const float scale = block_gains(amax, gain);
         const int lane = threadIdx.x & (kLanes - 1);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           unpack8(o[u], f);
           if (n[u] > 0) __stcs(reinterpret_cast<uint2*>(S.q + r[u] * S.ld_q + c), quant8(f, gain[u]));
-          // the scale's lane may lie past the last column: the block's first lane knows
-          const bool live = __shfl_sync(0xffffffffu, n[u], 0, kLanes) > 0;
-          const int64_t row = __shfl_sync(0xffffffffu, (long long)r[u], 0, kLanes);
-          if (lane == u && live) S.scale[row * S.ld_s + b] = scale;
+          if (lane == u && live[u]) S.scale[r[u] * S.ld_s + b] = scale;
         }
       });
 }
@@ -264,7 +272,7 @@ template <typename T, int U>
 __global__ void __launch_bounds__(kThreads) restore_kernel(Saved S, int64_t rows, int64_t cols, Mat x, int bpr_log2) {
   for_blocks<U, Eights>(
       rows, cols, bpr_log2, [&](int64_t r, int64_t c, int n) { return fetch8(S, r, c, n); },
-      [&](const Eights(&e)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
+      [&](const Eights(&e)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float f[8];
@@ -303,16 +311,14 @@ __global__ void __launch_bounds__(kThreads)
         return OctPair<T>{load8(static_cast<const T*>(gate.p) + r * gate.ld, c, n),
                           load8(static_cast<const T*>(up.p) + r * up.ld, c, n)};
       },
-      [&](const OctPair<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
+      [&](const OctPair<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
         const int lane = threadIdx.x & (kLanes - 1);
         if (SG.q) {
           float f[8], amax[2 * U], gain[2 * U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
-            unpack8(o[u].a, f);
-            amax[2 * u] = block_amax(f);
-            unpack8(o[u].b, f);
-            amax[2 * u + 1] = block_amax(f);
+            amax[2 * u] = block_amax(o[u].a);
+            amax[2 * u + 1] = block_amax(o[u].b);
           }
           const float scale = block_gains(amax, gain);
 #pragma unroll
@@ -323,10 +329,8 @@ __global__ void __launch_bounds__(kThreads)
               unpack8(o[u].b, f);
               __stcs(reinterpret_cast<uint2*>(SU.q + r[u] * SU.ld_q + c), quant8(f, gain[2 * u + 1]));
             }
-            const bool live = __shfl_sync(0xffffffffu, n[u], 0, kLanes) > 0;
-            const int64_t row = __shfl_sync(0xffffffffu, (long long)r[u], 0, kLanes);
-            if (lane == 2 * u && live) SG.scale[row * SG.ld_s + b] = scale;
-            if (lane == 2 * u + 1 && live) SU.scale[row * SU.ld_s + b] = scale;
+            if (lane == 2 * u && live[u]) SG.scale[r[u] * SG.ld_s + b] = scale;
+            if (lane == 2 * u + 1 && live[u]) SU.scale[r[u] * SU.ld_s + b] = scale;
           }
         }
 #pragma unroll
@@ -357,7 +361,7 @@ __global__ void __launch_bounds__(kThreads)
         return GatedIn<T>{load8(static_cast<const T*>(dy.p) + r * dy.ld, c, n), fetch8(SG, r, c, n),
                           fetch8(SU, r, c, n)};
       },
-      [&](const GatedIn<T>(&in)[U], const int64_t(&r)[U], const int(&n)[U], int64_t b, int64_t c) {
+      [&](const GatedIn<T>(&in)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float g[8], v[8], d[8];
@@ -518,7 +522,7 @@ __global__ void __launch_bounds__(NT == 32 ? kThreads : NT, NT == 32 ? 1024 / kT
     if (S.q) {
       float amax[kCh], gain[kCh];
 #pragma unroll
-      for (int i = 0; i < kCh; ++i) amax[i] = block_amax(f[i]);
+      for (int i = 0; i < kCh; ++i) amax[i] = block_amax(o[i]);
       const float scale = block_gains(amax, gain);
       const int lane = threadIdx.x & (kLanes - 1);
 #pragma unroll
@@ -549,8 +553,7 @@ __global__ void __launch_bounds__(NT == 32 ? kThreads : NT, NT == 32 ? 1024 / kT
   constexpr int kStage = St::kBytes * THREADS, kAhead = St::kAhead;
   const int tid = threadIdx.x % NT;
   const int64_t step = (int64_t)gridDim.x * RPC;
-  const int64_t group = (int64_t)blockIdx.x * RPC + threadIdx.x / NT;
-  int64_t r = group;
+  int64_t r = (int64_t)blockIdx.x * RPC + threadIdx.x / NT;
   auto column = [&](int i) { return ((int64_t)i * NT + tid) * 8; };
   auto issue = [&](int64_t row, int slot) {
     if (async && row < rows) {
@@ -629,9 +632,28 @@ __global__ void __launch_bounds__(NT == 32 ? kThreads : NT, NT == 32 ? 1024 / kT
     }
   }
   if (part) {
+    if constexpr (NT == 32) {  // the CTA's eight rows of sums to one, in order
+      constexpr int kSpan = kCh * NT * 8;
+      static_assert(RPC * kSpan * 4 <= kStage * (kAhead + 1), "the stages hold the rows of sums");
+      float* joined = reinterpret_cast<float*>(stages);
+      copies_wait<0>();
+      __syncthreads();  // no stage is in use
 #pragma unroll
-    for (int i = 0; i < kCh; ++i)
-      if (left8(cols, column(i)) > 0) store8(part + group * ld_part, column(i), 8, true, acc[i]);
+      for (int i = 0; i < kCh; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) joined[threadIdx.x / NT * kSpan + column(i) + j] = acc[i][j];
+      __syncthreads();
+      for (int c = threadIdx.x; c < cols; c += THREADS) {
+        float v = joined[c];
+#pragma unroll
+        for (int w8 = 1; w8 < RPC; ++w8) v += joined[w8 * kSpan + c];
+        part[(int64_t)blockIdx.x * ld_part + c] = v;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCh; ++i)
+        if (left8(cols, column(i)) > 0) store8(part + (int64_t)blockIdx.x * ld_part, column(i), 8, true, acc[i]);
+    }
   }
 }
 
@@ -661,9 +683,10 @@ __global__ void __launch_bounds__(kWide)
       const int64_t c = cc + threadIdx.x * 8, c0 = c - 8 * lane;
       const int n = left8(cols, c);
       float f[8], wt[8];
-      unpack8(load8(row, c, n), f);
+      const Oct<T> o = load8(row, c, n);
+      unpack8(o, f);
       if (S.q) {
-        const float amax[1] = {block_amax(f)};
+        const float amax[1] = {block_amax(o)};
         float gain[1];
         const float scale = block_gains(amax, gain);
         if (n > 0) __stcs(reinterpret_cast<uint2*>(S.q + r * S.ld_q + c), quant8(f, gain[0]));
@@ -696,12 +719,15 @@ __global__ void __launch_bounds__(kWide)
       e.s *= rs;
       values8(e, u);
       load_weight<T>(w, w_f32, cols, c, wt);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        // a thread owns its columns of the CTA's sums: plain loads and stores, no atomics
-        if (mine) mine[c + j] = fmaf(d[j], u[j], k ? mine[c + j] : 0.0f);
-        dot = fmaf(d[j] * wt[j], u[j], dot);
+      if (mine) {  // a thread owns its columns of the CTA's sums: plain loads and stores, no atomics
+        float4* at = reinterpret_cast<float4*>(mine + c);
+        float4 s0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), s1 = s0;
+        if (k) s0 = at[0], s1 = at[1];
+        at[0] = make_float4(fmaf(d[0], u[0], s0.x), fmaf(d[1], u[1], s0.y), fmaf(d[2], u[2], s0.z), fmaf(d[3], u[3], s0.w));
+        at[1] = make_float4(fmaf(d[4], u[4], s1.x), fmaf(d[5], u[5], s1.y), fmaf(d[6], u[6], s1.z), fmaf(d[7], u[7], s1.w));
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dot = fmaf(d[j] * wt[j], u[j], dot);
     }
     dot = row_sum<kWide>(dot, sh[k & 1]) / (float)cols;
     for (int64_t c = threadIdx.x * 8; c < cols; c += kWide * 8) {
@@ -719,23 +745,32 @@ __global__ void __launch_bounds__(kWide)
   }
 }
 
-// dw = column sums of the `n` partial rows, in double and in order: 32 columns x 8 rows of
-// threads per CTA.
+// dw = column sums of the `n` partial rows, in double and in a fixed order: 32 columns x 32
+// rows of threads per CTA, four rows' loads at a time (a thread's chain of loads is what
+// takes the time).
 template <typename WT>
-__global__ void __launch_bounds__(256) rms_dw_kernel(const float* __restrict__ part, int64_t n, int64_t ld_part,
-                                                      int64_t cols, WT* dw) {
-  __shared__ double sh[8][33];
+__global__ void __launch_bounds__(1024) rms_dw_kernel(const float* __restrict__ part, int64_t n, int64_t ld_part,
+                                                       int64_t cols, WT* dw) {
+  __shared__ double sh[32][33];
   const int lane = threadIdx.x & 31, q = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   double v = 0.0;
-  if (c < cols)
-    for (int64_t i = q; i < n; i += 8) v += part[i * ld_part + c];
+  if (c < cols) {
+    int64_t i = q;
+    for (; i + 96 < n; i += 128) {
+      const float a = part[i * ld_part + c], b = part[(i + 32) * ld_part + c];
+      const float d = part[(i + 64) * ld_part + c], e = part[(i + 96) * ld_part + c];
+      v += (double)a + (double)b + ((double)d + (double)e);
+    }
+    for (; i < n; i += 32) v += part[i * ld_part + c];
+  }
   sh[q][lane] = v;
   __syncthreads();
-  if (q == 0 && c < cols) {
-    for (int i = 1; i < 8; ++i) v += sh[i][lane];
-    dw[c] = from_f32<WT>((float)v);
-  }
+  v = sh[lane][q];  // warp q joins column q
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int64_t cq = (int64_t)blockIdx.x * 32 + q;
+  if (lane == 0 && cq < cols) dw[cq] = from_f32<WT>((float)v);
 }
 
 // ------------------------------------------------ host side
@@ -768,16 +803,19 @@ bool good_type(int t) { return t == ECO_F32 || t == ECO_BF16 || t == ECO_F16; }
 bool rows_on_16(const void* p, int64_t ld, int64_t rows, int type) {
   return eco_aligned16(p) && (rows <= 1 || ld * es_of(type) % 16 == 0);
 }
+// Eight columns of every row start on a boundary of their size: 32 bytes for fp32, else 16.
+bool rows_on_8(const void* p, int64_t ld, int64_t rows, int type) {
+  return reinterpret_cast<uintptr_t>(p) % (uintptr_t)(8 * es_of(type)) == 0 && (rows <= 1 || ld % 8 == 0);
+}
 int check_in(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const char* who) {
   ECO_REQUIRE(p && (rows <= 1 || ld >= 0) && reinterpret_cast<uintptr_t>(p) % (uintptr_t)es_of(type) == 0, ECO_ERR_ARG,
               "%s: bad input", who);
   return ECO_OK;
 }
-// Outputs have rows that start on 16 bytes and room for whole vectors behind the last column.
+// Outputs have rows of whole groups of eight columns that start on a boundary of their size.
 int check_out(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const char* who) {
-  const int64_t per = 16 / es_of(type);
-  ECO_REQUIRE(p && ld >= (cols + per - 1) / per * per, ECO_ERR_ARG, "%s: output rows too short", who);
-  ECO_REQUIRE(rows_on_16(p, ld, 2, type), ECO_ERR_MISALIGNED, "%s: output rows do not start on 16 bytes", who);
+  ECO_REQUIRE(p && ld >= (cols + 7) / 8 * 8, ECO_ERR_ARG, "%s: output rows too short", who);
+  ECO_REQUIRE(rows_on_8(p, ld, 2, type), ECO_ERR_MISALIGNED, "%s: output rows do not start on eight elements", who);
   return ECO_OK;
 }
 int check_shape(int64_t rows, int64_t cols, int type, const char* who) {
@@ -816,9 +854,6 @@ int64_t rms_ctas(int64_t rows, int64_t cols) {
   const int nt = row_threads(cols);
   const int threads = nt == 0 ? kWide : nt == 32 ? kThreads : nt, rpc = nt == 32 ? kThreads / 32 : 1;
   return std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)eco_num_sms() * (1024 / threads));
-}
-int64_t rms_groups(int64_t rows, int64_t cols) {
-  return rms_ctas(rows, cols) * (row_threads(cols) == 32 ? kThreads / 32 : 1);
 }
 // Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device; the
 // attribute is set at each launch that needs it (a host-side store, no synchronisation).
@@ -903,9 +938,9 @@ extern "C" int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int ac
   ECO_REQUIRE(dgate && dup && (rows <= 1 || (ld_dgate >= cols && ld_dup >= cols)), ECO_ERR_ARG,
               "eco_gated_act_bwd: bad outputs");
   // A half of one packed output has no padding of its own: the last columns, fewer than eight,
-  // are stored one by one, and so is a half whose rows do not start on 16 bytes.
-  const bool vg = rows_on_16(dgate, ld_dgate, rows, type);
-  const bool vu = rows_on_16(dup, ld_dup, rows, type);
+  // are stored one by one, and so is a half whose rows do not start on eight elements.
+  const bool vg = rows_on_8(dgate, ld_dgate, rows, type);
+  const bool vu = rows_on_8(dup, ld_dup, rows, type);
   const int l = bpr_log2_of(cols);
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
@@ -961,7 +996,7 @@ extern "C" int eco_rms_norm(const void* x, int64_t ld, int type, int64_t rows, i
 
 extern "C" int64_t eco_rms_norm_bwd_scratch(int64_t rows, int64_t cols) {
   if (rows <= 0 || cols <= 0) return 0;
-  return rms_groups(rows, cols) * ((cols + 7) / 8 * 8);
+  return rms_ctas(rows, cols) * ((cols + 7) / 8 * 8);
 }
 
 extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t rows, int64_t cols, const void* w,
@@ -981,15 +1016,15 @@ extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t
   if (int rc = check_saved(saved, rows, cols, "eco_rms_norm_bwd")) return rc;
   if (int rc = check_out(dx, ld_dx, rows, cols, type, "eco_rms_norm_bwd")) return rc;
   ECO_REQUIRE(rstd, ECO_ERR_ARG, "eco_rms_norm_bwd: null rstd");
-  const int64_t groups = rms_groups(rows, cols), ld_part = (cols + 7) / 8 * 8;
-  ECO_REQUIRE(!dw || (scratch && eco_aligned16(scratch) && scratch_len >= groups * ld_part), ECO_ERR_ARG,
+  const int64_t ctas = rms_ctas(rows, cols), ld_part = (cols + 7) / 8 * 8;
+  ECO_REQUIRE(!dw || (scratch && eco_aligned16(scratch) && scratch_len >= ctas * ld_part), ECO_ERR_ARG,
               "eco_rms_norm_bwd: scratch too small (eco_rms_norm_bwd_scratch)");
   bool ok = true;
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     by_width(cols, [&](auto nt) {
       constexpr int NT = decltype(nt)::value;
-      const unsigned grid = (unsigned)rms_ctas(rows, cols);
+      const unsigned grid = (unsigned)ctas;
       const Mat d{const_cast<void*>(dy), ld_dy}, o{dx, ld_dx};
       float* part = dw ? scratch : nullptr;
       const bool w_f32 = w_type == ECO_F32;
@@ -1000,7 +1035,7 @@ extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t
         const bool async = rows_on_16(dy, ld_dy, rows, type);
         ok = allow_smem(rms_bwd_kernel<T, NT>, smem);
         if (ok)
-          rms_bwd_kernel<T, NT><<<grid, threads, async ? smem : 0, s>>>(d, rows, cols, w, w_f32, saved_of(saved), rstd,
+          rms_bwd_kernel<T, NT><<<grid, threads, async || NT == 32 ? smem : 0, s>>>(d, rows, cols, w, w_f32, saved_of(saved), rstd,
                                                                         o, part, ld_part, async);
       }
     });
@@ -1009,7 +1044,7 @@ extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t
   if (dw)
     by_float(w_type, [&](auto* t) {
       using WT = std::remove_pointer_t<decltype(t)>;
-      rms_dw_kernel<WT><<<(unsigned)((cols + 31) / 32), 256, 0, s>>>(scratch, groups, ld_part, cols,
+      rms_dw_kernel<WT><<<(unsigned)((cols + 31) / 32), 1024, 0, s>>>(scratch, ctas, ld_part, cols,
                                                                      static_cast<WT*>(dw));
     });
   return eco_launch_check("eco_rms_norm_bwd");

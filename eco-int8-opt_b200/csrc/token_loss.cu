@@ -119,7 +119,8 @@ ECO_DEV float slope_at(float x, const Slope& w, bool token) {
 
 // N vectors at a time: their maximum first, so that the terms depend on nothing but it (and the
 // sum is rescaled only where the maximum has grown: seldom, after the first few).  ALL: all of
-// them count; else `in` says which.
+// them count; else `in` says which, and the others are worked on for nothing (lanes of a warp
+// differ in it: a branch would run both ways).
 template <typename T, bool ALL, int N>
 ECO_DEV void take_vectors(MaxSum& a, const uint4 (&raw)[N], const bool (&in)[N], Factor c) {
   constexpr int E = RowIo<T>::E;
@@ -131,17 +132,14 @@ ECO_DEV void take_vectors(MaxSum& a, const uint4 (&raw)[N], const bool (&in)[N],
     a.s *= term(a.m, off, c);
     a.m = m;
   }
-  float s[2] = {a.s, 0.0f};
 #pragma unroll
   for (int p = 0; p < N; ++p) {
-    if (ALL || in[p]) {
-      float f[E];
-      RowIo<T>::unpack(raw[p], f);
+    float f[E], s[2] = {0.0f, 0.0f};
+    RowIo<T>::unpack(raw[p], f);
 #pragma unroll
-      for (int k = 0; k < E; ++k) s[k & 1] += term(f[k], off, c);
-    }
+    for (int k = 0; k < E; ++k) s[k & 1] += term(f[k], off, c);
+    a.s += ALL || in[p] ? s[0] + s[1] : 0.0f;
   }
-  a.s = s[0] + s[1];
 }
 // Vectors p, p + step, ... of which `left` (counted in steps, from p on) count; N at a time.
 template <typename T, int N, bool SHARED>
@@ -482,10 +480,7 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
           in[p] = (q + p) * NT < whole && (q + p) * NT + tid >= first;
           raw[p] = at[(q + p) * NT];
         }
-        if (in[0] && in[3])
-          take_vectors<T, true, 4>(a, raw, in, R.c);
-        else
-          take_vectors<T, false, 4>(a, raw, in, R.c);
+        take_vectors<T, false, 4>(a, raw, in, R.c);
       }
     }
     if (w.skew > 0 || end % E) {

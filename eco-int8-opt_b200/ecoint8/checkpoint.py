@@ -13,7 +13,7 @@ one fp32 rounding), and the backward kernels read the eight bits in place:
 
 Tensors are fp32, bf16 or fp16 of any shape whose last dimension is the row.  A block whose
 largest value is below 2^-119 comes back as zeros; one that holds an infinity or NaN comes
-back as NaN.  Outputs whose rows are no multiple of 16 bytes have padded row strides.
+back as NaN.  Outputs whose rows are no multiple of eight columns have padded row strides.
 """
 
 from __future__ import annotations
@@ -43,11 +43,10 @@ def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
 
 
 def _empty_rows(rows: int, cols: int, dtype, dev) -> torch.Tensor:
-    """``[rows, cols]`` whose rows start on 16 bytes."""
-    per = 16 // dtype.itemsize
-    if cols % per == 0:
+    """``[rows, cols]`` whose rows start on a multiple of eight elements."""
+    if cols % 8 == 0:
         return torch.empty((rows, cols), dtype=dtype, device=dev)
-    return torch.empty((rows, (cols + per - 1) // per * per), dtype=dtype, device=dev)[:, :cols]
+    return torch.empty((rows, (cols + 7) // 8 * 8), dtype=dtype, device=dev)[:, :cols]
 
 
 class _Eight:

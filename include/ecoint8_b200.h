@@ -514,7 +514,7 @@ ECO_API int eco_preference_pairs(const double* logp64, const int64_t* tokens, co
  * amax)), each step one fp32 rounding; the block stands for q * scale.  amax < 2^-119: zeros; an
  * infinity or NaN in the block: NaN throughout.  q rows start on 16 bytes.  Matrices are
  * ECO_F32, ECO_BF16 or ECO_F16; inputs have any row stride and alignment; outputs have rows
- * that start on 16 bytes and are padded to whole 16-byte vectors (the padding is written). */
+ * that start on a multiple of eight elements and are padded to one (the padding is written). */
 #define ECO_CKPT_BLOCK 128
 enum { ECO_ACT_SILU = 0, ECO_ACT_GELU = 1 };
 

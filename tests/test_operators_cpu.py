@@ -165,7 +165,7 @@ def test_eight_bit_activations_refuse_bad_arguments():
                   (8192, 8192, 64, 0)):
         _refused(lib.eco_ckpt_pack(8192, 0, 4, 64, 64, ctypes.byref(nat.SavedI8(*saved)), None), -1, "eight-bit")
     _refused(lib.eco_ckpt_restore(ok, 1, 4, 63, 8192, 63, None), -1, "too short")
-    _refused(lib.eco_ckpt_restore(ok, 1, 4, 64, 8200, 64, None), -2, "16 bytes")
+    _refused(lib.eco_ckpt_restore(ok, 1, 4, 64, 8200, 64, None), -2, "eight elements")
     _refused(lib.eco_gated_act(8192, 64, 8192, 64, 0, 2, 4, 64, 8192, 64, ok, ok, None), -1, "activation")
     _refused(lib.eco_gated_act(8192, 64, 8192, 64, 0, 0, 4, 64, 8192, 64, ok, None, None), -1, "missing")
     _refused(lib.eco_gated_act_bwd(8192, 64, 0, 0, 4, 64, ok, ok, 8192, 32, 8192, 64, None), -1, "outputs")
