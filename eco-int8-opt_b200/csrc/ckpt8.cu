@@ -36,13 +36,15 @@ struct Oct {
 // on 16 bytes (32 for fp32) is read by the 16-byte words that hold its columns, shifted into
 // place (each word that is read holds at least one of them, so none lies outside the row's memory).
 template <typename T>
-ECO_DEV Oct<T> load8(const T* row, int64_t c, int n) {
+ECO_DEV Oct<T> load8(const T* row, int c, int n) {
   constexpr int W = Oct<T>::W, V = W / 4;  // 32-bit words, 16-byte words
   Oct<T> o;
   const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
   if (n == 8 && (a & (16 * V - 1)) == 0) {
     if constexpr (V == 2) {
-      asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      // volatile: without it the load counts as a pure function of the address, free to move in
+      // front of the conditions that say the address is good
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
           : "=r"(o.w[0]), "=r"(o.w[1]), "=r"(o.w[2]), "=r"(o.w[3]), "=r"(o.w[4]), "=r"(o.w[5]), "=r"(o.w[6]), "=r"(o.w[7])
           : "l"(row + c));
     } else {
@@ -97,7 +99,7 @@ ECO_DEV void unpack8(const Oct<T>& o, float (&f)[8]) {
 // Eight columns of an output row: whole where eight columns of the row start on a boundary of
 // their size (its padding takes the rest of the last eight), else n single stores.
 template <typename T>
-ECO_DEV void store8(T* row, int64_t c, int n, bool vec, const float (&f)[8]) {
+ECO_DEV void store8(T* row, int c, int n, bool vec, const float (&f)[8]) {
   if (vec) {
     if constexpr (sizeof(T) == 4) {
       asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c), "f"(f[0]), "f"(f[1]),
@@ -163,79 +165,64 @@ ECO_DEV uint2 quant8(const float (&f)[8], float gain) {
   for (int i = 0; i < 8; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[i], gain), 12582912.0f));
   return make_uint2(pack4(b[0], b[1], b[2], b[3]), pack4(b[4], b[5], b[6], b[7]));
 }
-// The bytes as floats: byte + 128 in the low mantissa bits of 2^23, less 2^23 + 128.
+// The bytes as floats, by the conversion unit, which has nothing else to do here.
 ECO_DEV void dequant8(uint2 q, float (&f)[8]) {
-  const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    f[i] = __uint_as_float(__byte_perm(w[i / 4], 0x4B000000u, 0x7440u | (uint32_t)(i & 3))) - 8388736.0f;
+  for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
 }
 // ------------------------------------------------ matrices
-struct Mat {  // rows of any type; two leading dimensions collapse to one
+struct Mat {  // rows of any type
   void* p;
-  int64_t ld;
+  int ld;
 };
 struct Saved {  // q [rows, ld_q] int8 (ld_q a multiple of 16), scale [rows, ld_s] fp32
   int8_t* q;
   float* scale;
-  int64_t ld_q, ld_s;
+  int ld_q, ld_s;
 };
 
-ECO_DEV int left8(int64_t cols, int64_t c) { return cols - c >= 8 ? 8 : (cols > c ? (int)(cols - c) : 0); }
+ECO_DEV int left8(int cols, int c) { return max(0, min(8, cols - c)); }
 
-// Where a half-warp works: blocks of one row side by side, rows below each other.  bpr
-// (blocks of a row in a CTA, a power of two up to 16) times rows in a CTA = 16.
-struct Tile {
-  int64_t row0, row_step;
-  int64_t b0, b_step, blocks;
-  int lane;
-  ECO_DEV Tile(int64_t cols, int bpr_log2) {
-    const int half = threadIdx.x / kLanes;
-    lane = threadIdx.x & (kLanes - 1);
-    blocks = (cols + kBlock - 1) / kBlock;
-    const int rows = kHalves >> bpr_log2;
-    row0 = (int64_t)blockIdx.y * rows + (half >> bpr_log2);
-    row_step = (int64_t)gridDim.y * rows;
-    b0 = ((int64_t)blockIdx.x << bpr_log2) + (half & ((1 << bpr_log2) - 1));
-    b_step = (int64_t)gridDim.x << bpr_log2;
-  }
-};
-// Loops over (row, block) in groups of U rows, whose loads are all issued before the first is
-// used (a thread has one or two 16-byte loads per row: alone they would not cover the memory's
-// latency).  Both halves of a warp stay in step (the shuffles need all 32 lanes): lanes past the
-// last row or column get n = 0 columns, blocks past the last row or block `live` = false.
+// Where a half-warp works: blocks of one row side by side, rows below each other.  2^l blocks of
+// a row in a CTA (up to 16) and 16 / 2^l rows.  Loops over (row, block) in groups of U rows,
+// whose loads are all issued before the first is used (a thread has one or two 16-byte loads per
+// row: alone they would not cover the memory's latency).  Both halves of a warp stay in step
+// (the shuffles need all 32 lanes): lanes past the last row or column get n = 0 columns, blocks
+// past the last row or block `live` = false.
 // load(r, c, n) -> L;  use(L[U], r[U], n[U], live[U], b, c).
 template <int U, typename L, typename Load, typename Use>
-ECO_DEV void for_blocks(int64_t rows, int64_t cols, int bpr_log2, Load load, Use use) {
-  const Tile t(cols, bpr_log2);
-  const int64_t first = (int64_t)blockIdx.y * (kHalves >> bpr_log2), firstb = (int64_t)blockIdx.x << bpr_log2;
-  for (int64_t r0 = t.row0, rr = first; rr < rows; r0 += U * t.row_step, rr += U * t.row_step)
-    for (int64_t b = t.b0, bb = firstb; bb < t.blocks; b += t.b_step, bb += t.b_step) {
-      const int64_t c = b * kBlock + t.lane * 8;
-      L l[U];
+ECO_DEV void for_blocks(int rows, int cols, int l, Load load, Use use) {
+  const int half = threadIdx.x / kLanes, lane = threadIdx.x & (kLanes - 1);
+  const int blocks = (cols + kBlock - 1) / kBlock, per = kHalves >> l;
+  const int row_step = (int)gridDim.y * per, b_step = (int)gridDim.x << l;
+  for (int64_t rr = (int64_t)blockIdx.y * per; rr < rows; rr += (int64_t)U * row_step)
+    for (int bb = (int)blockIdx.x << l; bb < blocks; bb += b_step) {
+      const int b = bb + (half & ((1 << l) - 1)), c = b * kBlock + lane * 8;
+      const int64_t r0 = rr + (half >> l);
+      L in[U];
       int64_t r[U];
       int n[U];
       bool live[U];
-      const int most = b < t.blocks ? left8(cols, c) : 0;
+      const int most = b < blocks ? left8(cols, c) : 0;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        r[u] = r0 + u * t.row_step;
-        live[u] = r[u] < rows && b < t.blocks;
+        r[u] = r0 + (int64_t)u * row_step;
+        live[u] = r[u] < rows && b < blocks;
         n[u] = live[u] ? most : 0;
         if (!live[u]) r[u] = 0;
-        l[u] = load(r[u], c, n[u]);
+        in[u] = load(r[u], c, n[u]);
       }
-      use(l, r, n, live, b, c);
+      use(in, r, n, live, b, c);
     }
 }
 
 // ------------------------------------------------ put away, bring back
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) pack_kernel(Mat x, int64_t rows, int64_t cols, Saved S, int bpr_log2) {
+__global__ void __launch_bounds__(kThreads) pack_kernel(Mat x, int rows, int cols, Saved S, int bpr_log2) {
   for_blocks<U, Oct<T>>(
       rows, cols, bpr_log2,
-      [&](int64_t r, int64_t c, int n) { return load8(static_cast<const T*>(x.p) + r * x.ld, c, n); },
-      [&](const Oct<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
+      [&](int64_t r, int c, int n) { return load8(static_cast<const T*>(x.p) + r * x.ld, c, n); },
+      [&](const Oct<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
         float f[8], amax[U], gain[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) amax[u] = block_amax(o[u]);
@@ -254,7 +241,7 @@ struct Eights {
   uint2 q;
   float s;
 };
-ECO_DEV Eights fetch8(const Saved& S, int64_t r, int64_t c, int n) {
+ECO_DEV Eights fetch8(const Saved& S, int64_t r, int c, int n) {
   Eights e{make_uint2(0u, 0u), 0.0f};
   if (n > 0) {
     e.q = __ldcs(reinterpret_cast<const uint2*>(S.q + r * S.ld_q + c));
@@ -269,10 +256,10 @@ ECO_DEV void values8(const Eights& e, float (&f)[8]) {
 }
 
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) restore_kernel(Saved S, int64_t rows, int64_t cols, Mat x, int bpr_log2) {
+__global__ void __launch_bounds__(kThreads) restore_kernel(Saved S, int rows, int cols, Mat x, int bpr_log2) {
   for_blocks<U, Eights>(
-      rows, cols, bpr_log2, [&](int64_t r, int64_t c, int n) { return fetch8(S, r, c, n); },
-      [&](const Eights(&e)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
+      rows, cols, bpr_log2, [&](int64_t r, int c, int n) { return fetch8(S, r, c, n); },
+      [&](const Eights(&e)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float f[8];
@@ -286,15 +273,33 @@ __global__ void __launch_bounds__(kThreads) restore_kernel(Saved S, int64_t rows
 // h = act(gate) up;  d up = dh act(gate),  d gate = dh up act'(gate)
 //   silu: act(g) = g s, s = 1 / (1 + e^-g);       act'(g) = s (1 + g (1 - s))
 //   gelu: act(g) = g F(g), F the normal's distribution;   act'(g) = F(g) + g f(g), f its density
+// The normal's distribution by the rational approximation 7.1.26 of Abramowitz and Stegun,
+// Handbook of Mathematical Functions: with z = |g| / sqrt 2 and t = 1 / (1 + 0.3275911 z),
+//   F(-|g|) = 1/2 (a1 t + ... + a5 t^5) exp(-z^2),  to 7.5e-8,
+// whose exponential is the density's too (one exponential and one reciprocal per element for
+// both; erff took as much again as all the rest).
+struct Act {
+  float over, dens;  // act(g) / g; gelu: the density at g
+};
 template <bool GELU>
-ECO_DEV float act_over_input(float g) {
-  if (GELU) return 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-  return __fdividef(1.0f, 1.0f + __expf(-g));
+ECO_DEV Act act_of(float g) {
+  if (GELU) {
+    const float a = fabsf(g);
+    const float t = __fdividef(1.0f, fmaf(a, 0.3275911f * 0.70710678118654752f, 1.0f));
+    const float e = __expf(-0.5f * g * g);
+    float p = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    p = fmaf(p, t, 0.5f * 1.421413741f);
+    p = fmaf(p, t, 0.5f * -0.284496736f);
+    p = fmaf(p, t, 0.5f * 0.254829592f);
+    const float low = p * t * e;
+    return Act{g < 0.0f ? low : 1.0f - low, e * 0.39894228040143268f};
+  }
+  return Act{__fdividef(1.0f, 1.0f + __expf(-g)), 0.0f};
 }
 template <bool GELU>
-ECO_DEV float act_slope(float g, float s) {
-  if (GELU) return fmaf(g * 0.39894228040143268f, __expf(-0.5f * g * g), s);
-  return s * fmaf(g, 1.0f - s, 1.0f);
+ECO_DEV float act_slope(float g, Act a) {
+  if (GELU) return fmaf(g, a.dens, a.over);
+  return a.over * fmaf(g, 1.0f - a.over, 1.0f);
 }
 
 template <typename T>
@@ -304,14 +309,14 @@ struct OctPair {
 
 template <typename T, bool GELU, int U>
 __global__ void __launch_bounds__(kThreads)
-    gated_fwd_kernel(Mat gate, Mat up, int64_t rows, int64_t cols, Mat y, Saved SG, Saved SU, int bpr_log2) {
+    gated_fwd_kernel(Mat gate, Mat up, int rows, int cols, Mat y, Saved SG, Saved SU, int bpr_log2) {
   for_blocks<U, OctPair<T>>(
       rows, cols, bpr_log2,
-      [&](int64_t r, int64_t c, int n) {
+      [&](int64_t r, int c, int n) {
         return OctPair<T>{load8(static_cast<const T*>(gate.p) + r * gate.ld, c, n),
                           load8(static_cast<const T*>(up.p) + r * up.ld, c, n)};
       },
-      [&](const OctPair<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
+      [&](const OctPair<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
         const int lane = threadIdx.x & (kLanes - 1);
         if (SG.q) {
           float f[8], amax[2 * U], gain[2 * U];
@@ -339,7 +344,7 @@ __global__ void __launch_bounds__(kThreads)
           unpack8(o[u].a, g);
           unpack8(o[u].b, v);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] = g[i] * act_over_input<GELU>(g[i]) * v[i];
+          for (int i = 0; i < 8; ++i) g[i] = g[i] * act_of<GELU>(g[i]).over * v[i];
           if (n[u] > 0) store8(static_cast<T*>(y.p) + r[u] * y.ld, c, n[u], true, g);
         }
       });
@@ -353,15 +358,15 @@ struct GatedIn {
 
 template <typename T, bool GELU, int U>
 __global__ void __launch_bounds__(kThreads)
-    gated_bwd_kernel(Mat dy, int64_t rows, int64_t cols, Saved SG, Saved SU, Mat dgate, Mat dup, bool vec_g,
+    gated_bwd_kernel(Mat dy, int rows, int cols, Saved SG, Saved SU, Mat dgate, Mat dup, bool vec_g,
                      bool vec_u, int bpr_log2) {
   for_blocks<U, GatedIn<T>>(
       rows, cols, bpr_log2,
-      [&](int64_t r, int64_t c, int n) {
+      [&](int64_t r, int c, int n) {
         return GatedIn<T>{load8(static_cast<const T*>(dy.p) + r * dy.ld, c, n), fetch8(SG, r, c, n),
                           fetch8(SU, r, c, n)};
       },
-      [&](const GatedIn<T>(&in)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int64_t b, int64_t c) {
+      [&](const GatedIn<T>(&in)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           float g[8], v[8], d[8];
@@ -370,9 +375,9 @@ __global__ void __launch_bounds__(kThreads)
           unpack8(in[u].dy, d);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float s = act_over_input<GELU>(g[i]);
+            const Act s = act_of<GELU>(g[i]);
             const float dg = d[i] * v[i] * act_slope<GELU>(g[i], s);
-            v[i] = d[i] * g[i] * s;
+            v[i] = d[i] * g[i] * s.over;
             g[i] = dg;
           }
           if (n[u] > 0) {
@@ -387,14 +392,13 @@ __global__ void __launch_bounds__(kThreads)
 // y = x r w,  r = 1 / sqrt(mean x^2 + eps);  with x' = what the eight bits stand for, u = x' r:
 //   dx = r (w dy - u mean(w dy u)),   dw = sum over rows of dy u.
 //
-// NT threads hold a row, 16 columns each, so a row is read once; the sum is joined over the
+// NT threads hold a row, CH groups of eight columns each, so a row is read once; the sum is joined over the
 // threads in a fixed order, with one barrier a row.  A CTA walks down its rows, and each thread
 // copies its own columns of the next rows (Stage::kAhead) into shared memory while it works on one
 // (cp.async: no other thread reads them, so no barrier belongs to the copies): the bytes in
-// flight do not depend on how far the row's barrier has come.  Rows that do not start on 16
-// bytes are loaded when they are needed.  Wider rows are read again for the second pass, and
+// flight do not depend on how far the row's barrier has come.  Wider rows are read again for the second pass, and
 // their dw sums live in the CTA's own row of `part`.
-constexpr int kCh = 2;      // groups of eight columns per thread
+constexpr int kRmsThreads = 512;  // per SM: 128 registers each, and what the stages have room for
 
 template <int NT>
 ECO_DEV float row_sum(float v, float* sh) {  // sh: this row's buffer (two take turns)
@@ -411,14 +415,13 @@ ECO_DEV float row_sum(float v, float* sh) {  // sh: this row's buffer (two take 
   return v;
 }
 
-// cp.async of `bytes` (0 .. N; the rest is zeros) to N bytes of shared memory.
 template <int N>
-ECO_DEV void copy_async(void* dst, const void* src, int bytes) {
+ECO_DEV void copy_async(void* dst, const void* src) {  // N bytes to shared memory
   const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
   if constexpr (N == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(d), "l"(src), "n"(N), "r"(bytes) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(N) : "memory");
 }
 ECO_DEV void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -426,233 +429,262 @@ ECO_DEV void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// One thread's columns of a row on their way: kCh groups of T (16-byte pieces, a piece of all
+// One thread's columns of a row on their way: CH groups of T (16-byte pieces, a piece of all
 // threads side by side), and for the backward the bytes, scales and the row's rstd.
-template <typename T, bool BWD>
+template <typename T, int CH, bool BWD>
 struct Stage {
   static constexpr int V = Oct<T>::W / 4;
-  static constexpr int kBytes = kCh * 16 * V + (BWD ? kCh * 12 + 4 : 0);  // per thread
-  // Rows on their way besides the one in work: what 1024 threads' stages leave room for.
-  static constexpr int kAhead = 200 * 1024 / (kBytes * 1024) - 1 > 3 ? 3 : 200 * 1024 / (kBytes * 1024) - 1;
+  static constexpr int kBytes = CH * 16 * V + (BWD ? CH * 12 + 4 : 0);  // per thread
+  // Rows on their way besides the one in work: what an SM's stages have room for.
+  static constexpr int kRoom = 200 * 1024 / (kBytes * kRmsThreads) - 1;
+  static constexpr int kAhead = kRoom > 3 ? 3 : kRoom;
   ECO_DEV static uint4* piece(char* st, int threads, int i, int v) {
     return reinterpret_cast<uint4*>(st) + (i * V + v) * threads + threadIdx.x;
   }
   ECO_DEV static uint2* bytes(char* st, int threads, int i) {
-    return reinterpret_cast<uint2*>(st + kCh * 16 * V * threads) + i * threads + threadIdx.x;
+    return reinterpret_cast<uint2*>(st + CH * 16 * V * threads) + i * threads + threadIdx.x;
   }
   ECO_DEV static float* word(char* st, int threads, int i) {  // scales, then rstd
-    return reinterpret_cast<float*>(st + kCh * (16 * V + 8) * threads) + i * threads + threadIdx.x;
+    return reinterpret_cast<float*>(st + CH * (16 * V + 8) * threads) + i * threads + threadIdx.x;
   }
 };
 
-// The weight of a thread's columns (ones without a weight, zeros past the end).
-template <typename T>
-ECO_DEV void load_weight(const void* w, bool w_f32, int64_t cols, int64_t c, float (&f)[8]) {
-  const int n = left8(cols, c);
-  if (!w) {
+// The weight: nothing (ones), fp32 or x's type.  WHOLE: groups of eight columns on 16 bytes.
+struct Weight {
+  const void* p;
+  bool f32;
+};
+template <typename T, bool WHOLE>
+ECO_DEV void load_weight(const Weight& w, int c, int n, float (&f)[8]) {
+  if (!w.p || n == 0) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) f[k] = 1.0f;
-  } else if (w_f32) {
-    unpack8(load8(static_cast<const float*>(w), c, n), f);
+  } else if constexpr (WHOLE) {
+    if (sizeof(T) == 4 || w.f32) {
+      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w.p) + c);
+      const float4 a = __ldg(p), b = __ldg(p + 1);
+      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    } else if constexpr (sizeof(T) == 2) {
+      const uint4 t = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w.p) + c));
+      const Oct<T> o{t.x, t.y, t.z, t.w};
+      unpack8(o, f);
+    }
+  } else if (w.f32) {
+    unpack8(load8(static_cast<const float*>(w.p), c, n), f);
   } else {
-    unpack8(load8(static_cast<const T*>(w), c, n), f);
+    unpack8(load8(static_cast<const T*>(w.p), c, n), f);
   }
 }
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, NT == 32 ? 1024 / kThreads : 1024 / NT)
-    rms_fwd_kernel(Mat x, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, float eps, Mat y,
-                   Saved S, float* rstd, bool async) {
+// WHOLE: rows start on 16 bytes and consist of whole groups of eight columns, and so does the
+// weight; else a row is loaded when it is needed.
+template <typename T, int NT, int CH, bool WHOLE>
+__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, kRmsThreads / (NT == 32 ? kThreads : NT))
+    rms_fwd_kernel(Mat x, int rows, int cols, const Weight w, float eps, Mat y, Saved S, float* rstd) {
   extern __shared__ __align__(16) char stages[];
   __shared__ float sh[2][NT / 32];
-  using St = Stage<T, false>;
+  using St = Stage<T, CH, false>;
   constexpr int THREADS = NT == 32 ? kThreads : NT, RPC = THREADS / NT;
   constexpr int kStage = St::kBytes * THREADS, kAhead = St::kAhead;
-  const int tid = threadIdx.x % NT;
-  const int64_t step = (int64_t)gridDim.x * RPC;
-  int64_t r = (int64_t)blockIdx.x * RPC + threadIdx.x / NT;
-  auto column = [&](int i) { return ((int64_t)i * NT + tid) * 8; };
-  auto issue = [&](int64_t row, int slot) {
-    if (async && row < rows) {
-      const T* p = static_cast<const T*>(x.p) + row * x.ld;
+  const int tid = threadIdx.x % NT, step = (int)gridDim.x * RPC, lane = threadIdx.x & (kLanes - 1);
+  int r = (int)blockIdx.x * RPC + threadIdx.x / NT;
+  const float inv_cols = 1.0f / (float)cols;
+  // groups of eight columns c, c + NT * 8, ...: how many columns each
+  const int c = tid * 8;
+  int n[CH];
 #pragma unroll
-      for (int i = 0; i < kCh; ++i) {
-        const int n = left8(cols, column(i)) * (int)sizeof(T);
+  for (int i = 0; i < CH; ++i) n[i] = left8(cols, c + i * NT * 8);
+  int ahead = r;  // the next row to be copied
+  auto issue = [&](int slot) {
+    if (WHOLE && ahead < rows) {
+      const T* src = static_cast<const T*>(x.p) + (int64_t)ahead * x.ld + c;
 #pragma unroll
-        for (int v = 0; v < St::V; ++v) {
-          const int b = n - 16 * v < 0 ? 0 : (n - 16 * v > 16 ? 16 : n - 16 * v);
-          copy_async<16>(St::piece(stages + slot * kStage, THREADS, i, v), b > 0 ? p + column(i) + 4 * v : p, b);
+      for (int i = 0; i < CH; ++i)
+        if (n[i] > 0) {
+#pragma unroll
+          for (int v = 0; v < St::V; ++v)
+            copy_async<16>(St::piece(stages + slot * kStage, THREADS, i, v), src + i * NT * 8 + v * (16 / (int)sizeof(T)));
         }
-      }
     }
     copies_commit();
+    ahead += step;
   };
-  for (int d = 0; d < kAhead; ++d) issue(r + d * step, d);
-  float wt[kCh][8];
-#pragma unroll
-  for (int i = 0; i < kCh; ++i) load_weight<T>(w, w_f32, cols, column(i), wt[i]);
-  for (int k = 0; r < rows; ++k, r += step) {
-    issue(r + kAhead * step, (k + kAhead) % (kAhead + 1));
-    Oct<T> o[kCh];
-    if (async) {
+  for (int d = 0; d < kAhead; ++d) issue(d);
+  int slot = 0, par = 0;
+  for (; r < rows; r += step) {
+    issue(slot == 0 ? kAhead : slot - 1);
+    Oct<T> o[CH];
+    if constexpr (WHOLE) {
       copies_wait<kAhead>();
-      char* st = stages + (k % (kAhead + 1)) * kStage;
+      char* st = stages + slot * kStage;
 #pragma unroll
-      for (int i = 0; i < kCh; ++i)
+      for (int i = 0; i < CH; ++i)
 #pragma unroll
         for (int v = 0; v < St::V; ++v) {
-          const uint4 q = *St::piece(st, THREADS, i, v);
-          o[i].w[4 * v] = q.x, o[i].w[4 * v + 1] = q.y, o[i].w[4 * v + 2] = q.z, o[i].w[4 * v + 3] = q.w;
+          uint4 t = make_uint4(0u, 0u, 0u, 0u);
+          if (n[i] > 0) t = *St::piece(st, THREADS, i, v);
+          o[i].w[4 * v] = t.x, o[i].w[4 * v + 1] = t.y, o[i].w[4 * v + 2] = t.z, o[i].w[4 * v + 3] = t.w;
         }
     } else {
 #pragma unroll
-      for (int i = 0; i < kCh; ++i)
-        o[i] = load8(static_cast<const T*>(x.p) + r * x.ld, column(i), left8(cols, column(i)));
+      for (int i = 0; i < CH; ++i)
+        o[i] = load8(static_cast<const T*>(x.p) + (int64_t)r * x.ld, c + i * NT * 8, n[i]);
     }
-    float ss = 0.0f, f[kCh][8];
+    slot = slot == kAhead ? 0 : slot + 1;
+    float ss = 0.0f, f[CH][8];
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) {
+    for (int i = 0; i < CH; ++i) {
       unpack8(o[i], f[i]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(f[i][j], f[i][j], ss);
     }
-    ss = row_sum<NT>(ss, sh[k & 1]);
-    const float rs = rsqrtf(ss / (float)cols + eps);
-    if (tid == 0 && rstd) rstd[r] = rs;
-    if (S.q) {
-      float amax[kCh], gain[kCh];
+    if (S.q) {  // in front of the row's barrier: it needs no sum
+      float amax[CH], gain[CH];
 #pragma unroll
-      for (int i = 0; i < kCh; ++i) amax[i] = block_amax(o[i]);
+      for (int i = 0; i < CH; ++i) amax[i] = block_amax(o[i]);
       const float scale = block_gains(amax, gain);
-      const int lane = threadIdx.x & (kLanes - 1);
+      int8_t* q = S.q + (int64_t)r * S.ld_q + c;
+      float* sc = S.scale + (int64_t)r * S.ld_s + c / kBlock;
 #pragma unroll
-      for (int i = 0; i < kCh; ++i) {
-        const int64_t c = column(i), c0 = c - 8 * lane;  // the block's first column
-        if (c < cols) __stcs(reinterpret_cast<uint2*>(S.q + r * S.ld_q + c), quant8(f[i], gain[i]));
-        if (lane == i && c0 < cols) S.scale[r * S.ld_s + c0 / kBlock] = scale;
+      for (int i = 0; i < CH; ++i) {
+        if (n[i] > 0) __stcs(reinterpret_cast<uint2*>(q + i * NT * 8), quant8(f[i], gain[i]));
+        if (lane == i && c - 8 * lane + i * NT * 8 < cols) sc[i * (NT * 8 / kBlock)] = scale;
       }
     }
+    ss = row_sum<NT>(ss, sh[par]);
+    par ^= 1;
+    const float rs = rsqrtf(fmaf(ss, inv_cols, eps));
+    if (tid == 0 && rstd) rstd[r] = rs;
+    T* out = static_cast<T*>(y.p) + (int64_t)r * y.ld + c;
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) {
+    for (int i = 0; i < CH; ++i) {
+      float wt[8];
+      load_weight<T, WHOLE>(w, c + i * NT * 8, n[i], wt);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] * rs * wt[i][j];
-      const int n = left8(cols, column(i));
-      if (n > 0) store8(static_cast<T*>(y.p) + r * y.ld, column(i), n, true, f[i]);
+      for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] * rs * wt[j];
+      if (n[i] > 0) store8(out, i * NT * 8, n[i], true, f[i]);
     }
   }
 }
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, NT == 32 ? 1024 / kThreads : 1024 / NT)
-    rms_bwd_kernel(Mat dy, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, Saved S,
-                   const float* __restrict__ rstd, Mat dx, float* part, int64_t ld_part, bool async) {
+template <typename T, int NT, int CH, bool WHOLE>
+__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, kRmsThreads / (NT == 32 ? kThreads : NT))
+    rms_bwd_kernel(Mat dy, int rows, int cols, const Weight w, Saved S, const float* __restrict__ rstd, Mat dx,
+                   float* part, int64_t ld_part) {
   extern __shared__ __align__(16) char stages[];
   __shared__ float sh[2][NT / 32];
-  using St = Stage<T, true>;
+  using St = Stage<T, CH, true>;
   constexpr int THREADS = NT == 32 ? kThreads : NT, RPC = THREADS / NT;
   constexpr int kStage = St::kBytes * THREADS, kAhead = St::kAhead;
-  const int tid = threadIdx.x % NT;
-  const int64_t step = (int64_t)gridDim.x * RPC;
-  int64_t r = (int64_t)blockIdx.x * RPC + threadIdx.x / NT;
-  auto column = [&](int i) { return ((int64_t)i * NT + tid) * 8; };
-  auto issue = [&](int64_t row, int slot) {
-    if (async && row < rows) {
+  const int tid = threadIdx.x % NT, step = (int)gridDim.x * RPC;
+  int r = (int)blockIdx.x * RPC + threadIdx.x / NT;
+  const float inv_cols = 1.0f / (float)cols;
+  const int c = tid * 8;
+  int n[CH];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) n[i] = left8(cols, c + i * NT * 8);
+  int ahead = r;
+  auto issue = [&](int slot) {
+    if (WHOLE && ahead < rows) {
       char* st = stages + slot * kStage;
-      const T* p = static_cast<const T*>(dy.p) + row * dy.ld;
-      const int8_t* q = S.q + row * S.ld_q;
-      const float* sc = S.scale + row * S.ld_s;
+      const T* src = static_cast<const T*>(dy.p) + (int64_t)ahead * dy.ld + c;
+      const int8_t* q = S.q + (int64_t)ahead * S.ld_q + c;
+      const float* sc = S.scale + (int64_t)ahead * S.ld_s + c / kBlock;
 #pragma unroll
-      for (int i = 0; i < kCh; ++i) {
-        const int64_t c = column(i);
-        const int n = left8(cols, c) * (int)sizeof(T);
+      for (int i = 0; i < CH; ++i) {
+        const int at = i * NT * 8;
+        if (n[i] > 0) {
 #pragma unroll
-        for (int v = 0; v < St::V; ++v) {
-          const int b = n - 16 * v < 0 ? 0 : (n - 16 * v > 16 ? 16 : n - 16 * v);
-          copy_async<16>(St::piece(st, THREADS, i, v), b > 0 ? p + c + 4 * v : p, b);
+          for (int v = 0; v < St::V; ++v)
+            copy_async<16>(St::piece(st, THREADS, i, v), src + at + v * (16 / (int)sizeof(T)));
+          copy_async<8>(St::bytes(st, THREADS, i), q + at);
+          copy_async<4>(St::word(st, THREADS, i), sc + at / kBlock);
         }
-        copy_async<8>(St::bytes(st, THREADS, i), n > 0 ? q + c : q, n > 0 ? 8 : 0);
-        copy_async<4>(St::word(st, THREADS, i), n > 0 ? sc + c / kBlock : sc, n > 0 ? 4 : 0);
       }
-      copy_async<4>(St::word(st, THREADS, kCh), rstd + row, 4);
+      copy_async<4>(St::word(st, THREADS, CH), rstd + ahead);
     }
     copies_commit();
+    ahead += step;
   };
-  for (int d = 0; d < kAhead; ++d) issue(r + d * step, d);
-  float acc[kCh][8] = {};
-  for (int k = 0; r < rows; ++k, r += step) {
-    issue(r + kAhead * step, (k + kAhead) % (kAhead + 1));
-    Oct<T> o[kCh];
-    Eights e[kCh];
-    float rs;
-    if (async) {
-      copies_wait<kAhead>();
-      char* st = stages + (k % (kAhead + 1)) * kStage;
+  for (int d = 0; d < kAhead; ++d) issue(d);
+  float acc[CH][8] = {};
+  int slot = 0, par = 0;
+  for (; r < rows; r += step) {
+    issue(slot == 0 ? kAhead : slot - 1);
+    if constexpr (WHOLE) copies_wait<kAhead>();
+    char* st = stages + slot * kStage;
+    slot = slot == kAhead ? 0 : slot + 1;
+    const float rs = WHOLE ? *St::word(st, THREADS, CH) : rstd[r];
+    // u = byte * scale * rstd: the factor, one per group, goes where it is used once
+    float dot = 0.0f, d[CH][8], k[CH];
+    uint2 bytes[CH];
 #pragma unroll
-      for (int i = 0; i < kCh; ++i) {
+    for (int i = 0; i < CH; ++i) {
+      Oct<T> o;
+      Eights e{make_uint2(0u, 0u), 0.0f};
+      if constexpr (WHOLE) {
 #pragma unroll
         for (int v = 0; v < St::V; ++v) {
-          const uint4 q = *St::piece(st, THREADS, i, v);
-          o[i].w[4 * v] = q.x, o[i].w[4 * v + 1] = q.y, o[i].w[4 * v + 2] = q.z, o[i].w[4 * v + 3] = q.w;
+          uint4 t = make_uint4(0u, 0u, 0u, 0u);
+          if (n[i] > 0) t = *St::piece(st, THREADS, i, v);
+          o.w[4 * v] = t.x, o.w[4 * v + 1] = t.y, o.w[4 * v + 2] = t.z, o.w[4 * v + 3] = t.w;
         }
-        e[i].q = *St::bytes(st, THREADS, i);
-        e[i].s = *St::word(st, THREADS, i);
+        if (n[i] > 0) e = Eights{*St::bytes(st, THREADS, i), *St::word(st, THREADS, i)};
+      } else {
+        o = load8(static_cast<const T*>(dy.p) + (int64_t)r * dy.ld, c + i * NT * 8, n[i]);
+        e = fetch8(S, r, c + i * NT * 8, n[i]);
       }
-      rs = *St::word(st, THREADS, kCh);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kCh; ++i) {
-        const int n = left8(cols, column(i));
-        o[i] = load8(static_cast<const T*>(dy.p) + r * dy.ld, column(i), n);
-        e[i] = fetch8(S, r, column(i), n);
-      }
-      rs = rstd[r];
-    }
-    float dot = 0.0f, d[kCh][8], u[kCh][8];
-#pragma unroll
-    for (int i = 0; i < kCh; ++i) {
-      float wt[8];
-      load_weight<T>(w, w_f32, cols, column(i), wt);  // from L1: registers hold the sums
-      unpack8(o[i], d[i]);
-      e[i].s *= rs;
-      values8(e[i], u[i]);
+      float wt[8], u[8], part_dot = 0.0f;
+      load_weight<T, WHOLE>(w, c + i * NT * 8, n[i], wt);  // from L1: registers hold the sums
+      unpack8(o, d[i]);
+      dequant8(e.q, u);
+      bytes[i] = e.q;
+      k[i] = e.s * rs;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        acc[i][j] = fmaf(d[i][j], u[i][j], acc[i][j]);
+        acc[i][j] = fmaf(d[i][j] * k[i], u[j], acc[i][j]);
         d[i][j] *= wt[j];
-        dot = fmaf(d[i][j], u[i][j], dot);
+        part_dot = fmaf(d[i][j], u[j], part_dot);
       }
+      dot = fmaf(part_dot, k[i], dot);
     }
-    dot = row_sum<NT>(dot, sh[k & 1]) / (float)cols;
+    dot = row_sum<NT>(dot, sh[par]) * inv_cols;
+    par ^= 1;
+    T* out = static_cast<T*>(dx.p) + (int64_t)r * dx.ld + c;
 #pragma unroll
-    for (int i = 0; i < kCh; ++i) {
+    for (int i = 0; i < CH; ++i) {
+      const float kd = k[i] * dot;
+      float u[8];
+      asm volatile("" : "+r"(bytes[i].x), "+r"(bytes[i].y));  // converted again: the bytes take a quarter of the room
+      dequant8(bytes[i], u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[i][j] = rs * fmaf(-u[i][j], dot, d[i][j]);
-      const int n = left8(cols, column(i));
-      if (n > 0) store8(static_cast<T*>(dx.p) + r * dx.ld, column(i), n, true, d[i]);
+      for (int j = 0; j < 8; ++j) d[i][j] = rs * fmaf(-u[j], kd, d[i][j]);
+      if (n[i] > 0) store8(out, i * NT * 8, n[i], true, d[i]);
     }
   }
   if (part) {
+    float* mine = part + (int64_t)blockIdx.x * ld_part;
     if constexpr (NT == 32) {  // the CTA's eight rows of sums to one, in order
-      constexpr int kSpan = kCh * NT * 8;
+      constexpr int kSpan = CH * NT * 8;
       static_assert(RPC * kSpan * 4 <= kStage * (kAhead + 1), "the stages hold the rows of sums");
       float* joined = reinterpret_cast<float*>(stages);
       copies_wait<0>();
       __syncthreads();  // no stage is in use
 #pragma unroll
-      for (int i = 0; i < kCh; ++i)
+      for (int i = 0; i < CH; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) joined[threadIdx.x / NT * kSpan + column(i) + j] = acc[i][j];
+        for (int j = 0; j < 8; ++j) joined[threadIdx.x / NT * kSpan + c + i * NT * 8 + j] = acc[i][j];
       __syncthreads();
-      for (int c = threadIdx.x; c < cols; c += THREADS) {
-        float v = joined[c];
+      for (int at = threadIdx.x; at < cols; at += THREADS) {
+        float v = joined[at];
 #pragma unroll
-        for (int w8 = 1; w8 < RPC; ++w8) v += joined[w8 * kSpan + c];
-        part[(int64_t)blockIdx.x * ld_part + c] = v;
+        for (int w8 = 1; w8 < RPC; ++w8) v += joined[w8 * kSpan + at];
+        mine[at] = v;
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < kCh; ++i)
-        if (left8(cols, column(i)) > 0) store8(part + (int64_t)blockIdx.x * ld_part, column(i), 8, true, acc[i]);
+      for (int i = 0; i < CH; ++i)
+        if (n[i] > 0) store8(mine, c + i * NT * 8, 8, true, acc[i]);
     }
   }
 }
@@ -662,7 +694,7 @@ constexpr int kWide = 512;
 
 template <typename T>
 __global__ void __launch_bounds__(kWide)
-    rms_fwd_wide_kernel(Mat x, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, float eps, Mat y,
+    rms_fwd_wide_kernel(Mat x, int rows, int cols, const Weight w, float eps, Mat y,
                         Saved S, float* rstd) {
   __shared__ float sh[2][kWide / 32];
   const int lane = threadIdx.x & (kLanes - 1);
@@ -670,7 +702,7 @@ __global__ void __launch_bounds__(kWide)
   for (int64_t r = blockIdx.x; r < rows; r += gridDim.x, ++k) {
     const T* row = static_cast<const T*>(x.p) + r * x.ld;
     float ss = 0.0f;
-    for (int64_t c = threadIdx.x * 8; c < cols; c += kWide * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kWide * 8) {
       float f[8];
       unpack8(load8(row, c, left8(cols, c)), f);
 #pragma unroll
@@ -679,8 +711,8 @@ __global__ void __launch_bounds__(kWide)
     ss = row_sum<kWide>(ss, sh[k & 1]);
     const float rs = rsqrtf(ss / (float)cols + eps);
     if (threadIdx.x == 0 && rstd) rstd[r] = rs;
-    for (int64_t cc = 0; cc < cols; cc += kWide * 8) {  // every lane, for the shuffles
-      const int64_t c = cc + threadIdx.x * 8, c0 = c - 8 * lane;
+    for (int cc = 0; cc < cols; cc += kWide * 8) {  // every lane, for the shuffles
+      const int c = cc + threadIdx.x * 8, c0 = c - 8 * lane;
       const int n = left8(cols, c);
       float f[8], wt[8];
       const Oct<T> o = load8(row, c, n);
@@ -692,7 +724,7 @@ __global__ void __launch_bounds__(kWide)
         if (n > 0) __stcs(reinterpret_cast<uint2*>(S.q + r * S.ld_q + c), quant8(f, gain[0]));
         if (lane == 0 && c0 < cols) S.scale[r * S.ld_s + c0 / kBlock] = scale;
       }
-      load_weight<T>(w, w_f32, cols, c, wt);
+      load_weight<T, false>(w, c, n, wt);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = f[j] * rs * wt[j];
       if (n > 0) store8(static_cast<T*>(y.p) + r * y.ld, c, n, true, f);
@@ -702,7 +734,7 @@ __global__ void __launch_bounds__(kWide)
 
 template <typename T>
 __global__ void __launch_bounds__(kWide)
-    rms_bwd_wide_kernel(Mat dy, int64_t rows, int64_t cols, const void* __restrict__ w, bool w_f32, Saved S,
+    rms_bwd_wide_kernel(Mat dy, int rows, int cols, const Weight w, Saved S,
                         const float* __restrict__ rstd, Mat dx, float* part, int64_t ld_part) {
   __shared__ float sh[2][kWide / 32];
   float* mine = part ? part + blockIdx.x * ld_part : nullptr;
@@ -711,14 +743,14 @@ __global__ void __launch_bounds__(kWide)
     const T* row = static_cast<const T*>(dy.p) + r * dy.ld;
     const float rs = rstd[r];
     float dot = 0.0f;
-    for (int64_t c = threadIdx.x * 8; c < cols; c += kWide * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kWide * 8) {
       const int n = left8(cols, c);
       float d[8], u[8], wt[8];
       unpack8(load8(row, c, n), d);
       Eights e = fetch8(S, r, c, n);
       e.s *= rs;
       values8(e, u);
-      load_weight<T>(w, w_f32, cols, c, wt);
+      load_weight<T, false>(w, c, n, wt);
       if (mine) {  // a thread owns its columns of the CTA's sums: plain loads and stores, no atomics
         float4* at = reinterpret_cast<float4*>(mine + c);
         float4 s0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), s1 = s0;
@@ -730,14 +762,14 @@ __global__ void __launch_bounds__(kWide)
       for (int j = 0; j < 8; ++j) dot = fmaf(d[j] * wt[j], u[j], dot);
     }
     dot = row_sum<kWide>(dot, sh[k & 1]) / (float)cols;
-    for (int64_t c = threadIdx.x * 8; c < cols; c += kWide * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kWide * 8) {
       const int n = left8(cols, c);
       float d[8], u[8], wt[8];
       unpack8(load8(row, c, n), d);
       Eights e = fetch8(S, r, c, n);
       e.s *= rs;
       values8(e, u);
-      load_weight<T>(w, w_f32, cols, c, wt);
+      load_weight<T, false>(w, c, n, wt);
 #pragma unroll
       for (int j = 0; j < 8; ++j) d[j] = rs * fmaf(-u[j], dot, d[j] * wt[j]);
       store8(static_cast<T*>(dx.p) + r * dx.ld, c, n, true, d);
@@ -790,13 +822,14 @@ dim3 block_grid(int64_t rows, int64_t cols, int bpr_log2, int unroll) {
 }
 
 int check_saved(const eco_saved_i8_t* S, int64_t rows, int64_t cols, const char* who) {
-  ECO_REQUIRE(S && S->q && S->scale && S->ld_q >= cols && S->ld_q % 16 == 0 && eco_aligned16(S->q) &&
-                  S->ld_scale >= (cols + kBlock - 1) / kBlock,
+  ECO_REQUIRE(S && S->q && S->scale && S->ld_q >= cols && S->ld_q <= INT32_MAX && S->ld_q % 16 == 0 && eco_aligned16(S->q) &&
+                  S->ld_scale >= (cols + kBlock - 1) / kBlock && S->ld_scale <= INT32_MAX,
               ECO_ERR_ARG, "%s: bad eight-bit buffers", who);
   return ECO_OK;
 }
+Mat mat(const void* p, int64_t ld) { return Mat{const_cast<void*>(p), (int)ld}; }
 Saved saved_of(const eco_saved_i8_t* S) {
-  return S ? Saved{S->q, S->scale, S->ld_q, S->ld_scale} : Saved{nullptr, nullptr, 0, 0};
+  return S ? Saved{S->q, S->scale, (int)S->ld_q, (int)S->ld_scale} : Saved{nullptr, nullptr, 0, 0};
 }
 int es_of(int type) { return type == ECO_F32 ? 4 : 2; }
 bool good_type(int t) { return t == ECO_F32 || t == ECO_BF16 || t == ECO_F16; }
@@ -808,18 +841,19 @@ bool rows_on_8(const void* p, int64_t ld, int64_t rows, int type) {
   return reinterpret_cast<uintptr_t>(p) % (uintptr_t)(8 * es_of(type)) == 0 && (rows <= 1 || ld % 8 == 0);
 }
 int check_in(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const char* who) {
-  ECO_REQUIRE(p && (rows <= 1 || ld >= 0) && reinterpret_cast<uintptr_t>(p) % (uintptr_t)es_of(type) == 0, ECO_ERR_ARG,
+  ECO_REQUIRE(p && (rows <= 1 || (ld >= 0 && ld <= INT32_MAX)) && reinterpret_cast<uintptr_t>(p) % (uintptr_t)es_of(type) == 0, ECO_ERR_ARG,
               "%s: bad input", who);
   return ECO_OK;
 }
 // Outputs have rows of whole groups of eight columns that start on a boundary of their size.
 int check_out(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const char* who) {
-  ECO_REQUIRE(p && ld >= (cols + 7) / 8 * 8, ECO_ERR_ARG, "%s: output rows too short", who);
+  ECO_REQUIRE(p && ld >= (cols + 7) / 8 * 8 && ld <= INT32_MAX, ECO_ERR_ARG, "%s: output rows too short", who);
   ECO_REQUIRE(rows_on_8(p, ld, 2, type), ECO_ERR_MISALIGNED, "%s: output rows do not start on eight elements", who);
   return ECO_OK;
 }
 int check_shape(int64_t rows, int64_t cols, int type, const char* who) {
-  ECO_REQUIRE(rows >= 0 && cols > 0 && cols <= (int64_t)1 << 28, ECO_ERR_ARG, "%s: bad shape", who);
+  ECO_REQUIRE(rows >= 0 && cols > 0 && rows <= (int64_t)1 << 30 && cols <= (int64_t)1 << 28, ECO_ERR_ARG,
+              "%s: bad shape", who);
   ECO_REQUIRE(good_type(type), ECO_ERR_ARG, "%s: unknown type %d", who, type);
   return ECO_OK;
 }
@@ -831,29 +865,34 @@ void by_float(int type, F f) {
   else f((__half*)nullptr);
 }
 
-// Threads of a row (16 columns each), 0 for the two-pass kernels of wider rows.
-int row_threads(int64_t cols) {
-  int nt = 32;
-  while (nt < 1024 && (int64_t)nt * 8 * kCh < cols) nt *= 2;
-  return (int64_t)nt * 8 * kCh < cols ? 0 : nt;
-}
+// Threads of a row and groups of eight columns per thread: a warp up to 1024 columns, four groups
+// per thread beyond; (0, 0): the two-pass kernels of wider rows.
 template <typename F>
 void by_width(int64_t cols, F f) {
-  switch (row_threads(cols)) {
-    case 32: return f(std::integral_constant<int, 32>{});
-    case 64: return f(std::integral_constant<int, 64>{});
-    case 128: return f(std::integral_constant<int, 128>{});
-    case 256: return f(std::integral_constant<int, 256>{});
-    case 512: return f(std::integral_constant<int, 512>{});
-    case 1024: return f(std::integral_constant<int, 1024>{});
-    default: return f(std::integral_constant<int, 0>{});
-  }
+  using std::integral_constant;
+  if (cols <= 256) f(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+  else if (cols <= 512) f(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+  else if (cols <= 1024) f(integral_constant<int, 32>{}, integral_constant<int, 4>{});
+  else if (cols <= 2048) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  else if (cols <= 4096) f(integral_constant<int, 128>{}, integral_constant<int, 4>{});
+  else if (cols <= 8192) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  else if (cols <= 16384) f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
+  else f(integral_constant<int, 0>{}, integral_constant<int, 0>{});
 }
-// CTAs of the norm's kernels: what is resident at 1024 threads per SM.
+// Rows of whole groups of eight columns on 16 bytes, and a weight on 16 bytes.
+bool whole_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const void* w) {
+  return rows_on_16(p, ld, rows, type) && cols % 8 == 0 && eco_aligned16(w);
+}
+// CTAs of the norm's kernels: what is resident.
 int64_t rms_ctas(int64_t rows, int64_t cols) {
-  const int nt = row_threads(cols);
-  const int threads = nt == 0 ? kWide : nt == 32 ? kThreads : nt, rpc = nt == 32 ? kThreads / 32 : 1;
-  return std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)eco_num_sms() * (1024 / threads));
+  int64_t n = 0;
+  by_width(cols, [&](auto nt, auto) {
+    constexpr int NT = decltype(nt)::value;
+    constexpr int threads = NT == 0 ? kWide : NT == 32 ? kThreads : NT, rpc = NT == 32 ? kThreads / 32 : 1;
+    const int per_sm = NT == 0 ? 1024 / kWide : kRmsThreads / threads;
+    n = std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)eco_num_sms() * per_sm);
+  });
+  return n;
 }
 // Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device; the
 // attribute is set at each launch that needs it (a host-side store, no synchronisation).
@@ -876,7 +915,7 @@ extern "C" int eco_ckpt_pack(const void* x, int type, int64_t rows, int64_t cols
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int U = sizeof(T) == 4 ? 2 : 4;
     pack_kernel<T, U><<<block_grid(rows, cols, l, U), kThreads, 0, eco_stream(stream)>>>(
-        Mat{const_cast<void*>(x), ld}, rows, cols, saved_of(saved), l);
+        mat(x, ld), (int)rows, (int)cols, saved_of(saved), l);
   });
   return eco_launch_check("eco_ckpt_pack");
 }
@@ -890,8 +929,8 @@ extern "C" int eco_ckpt_restore(const eco_saved_i8_t* saved, int type, int64_t r
   const int l = bpr_log2_of(cols);
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    restore_kernel<T, 4><<<block_grid(rows, cols, l, 4), kThreads, 0, eco_stream(stream)>>>(saved_of(saved), rows,
-                                                                                            cols, Mat{x, ld}, l);
+    restore_kernel<T, 4><<<block_grid(rows, cols, l, 4), kThreads, 0, eco_stream(stream)>>>(
+        saved_of(saved), (int)rows, (int)cols, mat(x, ld), l);
   });
   return eco_launch_check("eco_ckpt_restore");
 }
@@ -915,12 +954,12 @@ extern "C" int eco_gated_act(const void* gate, int64_t ld_gate, const void* up, 
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int U = sizeof(T) == 4 ? 1 : 2;
     const dim3 grid = block_grid(rows, cols, l, U);
-    const Mat g{const_cast<void*>(gate), ld_gate}, u{const_cast<void*>(up), ld_up}, o{y, ld_y};
+    const Mat g = mat(gate, ld_gate), u = mat(up, ld_up), o = mat(y, ld_y);
     if (act == ECO_ACT_GELU)
-      gated_fwd_kernel<T, true, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, rows, cols, o, saved_of(saved_gate),
+      gated_fwd_kernel<T, true, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, (int)rows, (int)cols, o, saved_of(saved_gate),
                                                                            saved_of(saved_up), l);
     else
-      gated_fwd_kernel<T, false, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, rows, cols, o, saved_of(saved_gate),
+      gated_fwd_kernel<T, false, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, (int)rows, (int)cols, o, saved_of(saved_gate),
                                                                             saved_of(saved_up), l);
   });
   return eco_launch_check("eco_gated_act");
@@ -935,7 +974,7 @@ extern "C" int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int ac
   if (int rc = check_in(dy, ld_dy, rows, cols, type, "eco_gated_act_bwd")) return rc;
   if (int rc = check_saved(saved_gate, rows, cols, "eco_gated_act_bwd")) return rc;
   if (int rc = check_saved(saved_up, rows, cols, "eco_gated_act_bwd")) return rc;
-  ECO_REQUIRE(dgate && dup && (rows <= 1 || (ld_dgate >= cols && ld_dup >= cols)), ECO_ERR_ARG,
+  ECO_REQUIRE(dgate && dup && (rows <= 1 || (ld_dgate >= cols && ld_dup >= cols && ld_dgate <= INT32_MAX && ld_dup <= INT32_MAX)), ECO_ERR_ARG,
               "eco_gated_act_bwd: bad outputs");
   // A half of one packed output has no padding of its own: the last columns, fewer than eight,
   // are stored one by one, and so is a half whose rows do not start on eight elements.
@@ -946,13 +985,13 @@ extern "C" int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int ac
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int U = sizeof(T) == 4 ? 1 : 2;
     const dim3 grid = block_grid(rows, cols, l, U);
-    const Mat d{const_cast<void*>(dy), ld_dy}, g{dgate, ld_dgate}, u{dup, ld_dup};
+    const Mat d = mat(dy, ld_dy), g = mat(dgate, ld_dgate), u = mat(dup, ld_dup);
     if (act == ECO_ACT_GELU)
       gated_bwd_kernel<T, true, U><<<grid, kThreads, 0, eco_stream(stream)>>>(
-          d, rows, cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
+          d, (int)rows, (int)cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
     else
       gated_bwd_kernel<T, false, U><<<grid, kThreads, 0, eco_stream(stream)>>>(
-          d, rows, cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
+          d, (int)rows, (int)cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
   });
   return eco_launch_check("eco_gated_act_bwd");
 }
@@ -972,21 +1011,22 @@ extern "C" int eco_rms_norm(const void* x, int64_t ld, int type, int64_t rows, i
   bool ok = true;
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    by_width(cols, [&](auto nt) {
-      constexpr int NT = decltype(nt)::value;
+    by_width(cols, [&](auto nt, auto ch) {
+      constexpr int NT = decltype(nt)::value, CH = decltype(ch)::value;
       const unsigned grid = (unsigned)rms_ctas(rows, cols);
-      const Mat xi{const_cast<void*>(x), ld}, yo{y, ld_y};
-      const bool w_f32 = w_type == ECO_F32;
+      const Mat xi = mat(x, ld), yo = mat(y, ld_y);
+      const Weight wt{w, w_type == ECO_F32};
       if constexpr (NT == 0) {
-        rms_fwd_wide_kernel<T><<<grid, kWide, 0, eco_stream(stream)>>>(xi, rows, cols, w, w_f32, (float)eps, yo,
+        rms_fwd_wide_kernel<T><<<grid, kWide, 0, eco_stream(stream)>>>(xi, (int)rows, (int)cols, wt, (float)eps, yo,
                                                                        saved_of(saved), rstd);
       } else {
-        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, false>::kBytes * threads * (Stage<T, false>::kAhead + 1);
-        const bool async = rows_on_16(x, ld, rows, type);
-        ok = allow_smem(rms_fwd_kernel<T, NT>, smem);
-        if (ok)
-          rms_fwd_kernel<T, NT><<<grid, threads, async ? smem : 0, eco_stream(stream)>>>(
-              xi, rows, cols, w, w_f32, (float)eps, yo, saved_of(saved), rstd, async);
+        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, CH, false>::kBytes * threads * (Stage<T, CH, false>::kAhead + 1);
+        if (!whole_rows(x, ld, rows, cols, type, w))
+          rms_fwd_kernel<T, NT, CH, false><<<grid, threads, 0, eco_stream(stream)>>>(xi, (int)rows, (int)cols, wt, (float)eps,
+                                                                                 yo, saved_of(saved), rstd);
+        else if ((ok = allow_smem(rms_fwd_kernel<T, NT, CH, true>, smem)))
+          rms_fwd_kernel<T, NT, CH, true><<<grid, threads, smem, eco_stream(stream)>>>(xi, (int)rows, (int)cols, wt,
+                                                                                   (float)eps, yo, saved_of(saved), rstd);
       }
     });
   });
@@ -1022,21 +1062,23 @@ extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t
   bool ok = true;
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    by_width(cols, [&](auto nt) {
-      constexpr int NT = decltype(nt)::value;
+    by_width(cols, [&](auto nt, auto ch) {
+      constexpr int NT = decltype(nt)::value, CH = decltype(ch)::value;
       const unsigned grid = (unsigned)ctas;
-      const Mat d{const_cast<void*>(dy), ld_dy}, o{dx, ld_dx};
+      const Mat d = mat(dy, ld_dy), o = mat(dx, ld_dx);
       float* part = dw ? scratch : nullptr;
-      const bool w_f32 = w_type == ECO_F32;
+      const Weight wt{w, w_type == ECO_F32};
       if constexpr (NT == 0) {
-        rms_bwd_wide_kernel<T><<<grid, kWide, 0, s>>>(d, rows, cols, w, w_f32, saved_of(saved), rstd, o, part, ld_part);
+        rms_bwd_wide_kernel<T><<<grid, kWide, 0, s>>>(d, (int)rows, (int)cols, wt, saved_of(saved), rstd, o, part,
+                                                           ld_part);
       } else {
-        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, true>::kBytes * threads * (Stage<T, true>::kAhead + 1);
-        const bool async = rows_on_16(dy, ld_dy, rows, type);
-        ok = allow_smem(rms_bwd_kernel<T, NT>, smem);
+        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, CH, true>::kBytes * threads * (Stage<T, CH, true>::kAhead + 1);
+        const bool whole = whole_rows(dy, ld_dy, rows, cols, type, w);
+        const auto kernel = whole ? rms_bwd_kernel<T, NT, CH, true> : rms_bwd_kernel<T, NT, CH, false>;
+        const int bytes = whole || NT == 32 ? smem : 0;
+        ok = allow_smem(kernel, bytes);
         if (ok)
-          rms_bwd_kernel<T, NT><<<grid, threads, async || NT == 32 ? smem : 0, s>>>(d, rows, cols, w, w_f32, saved_of(saved), rstd,
-                                                                        o, part, ld_part, async);
+          kernel<<<grid, threads, bytes, s>>>(d, (int)rows, (int)cols, wt, saved_of(saved), rstd, o, part, ld_part);
       }
     });
   });

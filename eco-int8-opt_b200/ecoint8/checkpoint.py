@@ -39,7 +39,7 @@ def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
     if t.shape[-1] == 0:
         raise AssertionError(f"{name} has empty rows")
     m = t.reshape(-1, t.shape[-1])
-    return m if m.stride(1) == 1 or m.shape[1] == 1 else m.contiguous()
+    return m if (m.stride(1) == 1 or m.shape[1] == 1) and m.stride(0) < 1 << 31 else m.contiguous()
 
 
 def _empty_rows(rows: int, cols: int, dtype, dev) -> torch.Tensor:

@@ -236,8 +236,9 @@ def test_gated_activation(act, name, rows, cols, packed):
     def err(v):
         return (v.abs().clamp(max=104) * 2 + 32) * U
 
-    # erf near -1 cancels: gelu's F has the absolute error 2^-24
-    low = (lambda v: v.abs() * 2.0 ** -23) if act == "gelu" else (lambda v: v.abs() * 2.0 ** -126)
+    # gelu's distribution is a rational approximation with the absolute error 7.5e-8, evaluated in
+    # fp32 from terms below 1 (2^-24 more): together below 2^-22
+    low = (lambda v: v.abs() * 2.0 ** -22) if act == "gelu" else (lambda v: v.abs() * 2.0 ** -126)
     tol = wy.abs() * (_half(dtype) + err(g)) + low(g) * u.abs() + 2.0 ** -126
     if dtype == torch.float16:
         tol = tol + 2.0 ** -25
@@ -247,7 +248,7 @@ def test_gated_activation(act, name, rows, cols, packed):
     tol = wu.abs() * (_half(dtype) + err(kg)) + low(kg) * d + extra
     assert ((du.double() - wu).abs() <= tol).all()
     # act' sums terms of either sign, each below 1 + |g|
-    tol = wg.abs() * _half(dtype) + d * ku.abs() * (1 + kg.abs()) * err(kg) + extra
+    tol = wg.abs() * _half(dtype) + d * ku.abs() * ((1 + kg.abs()) * err(kg) + (2.0 ** -22 if act == "gelu" else 0)) + extra
     assert dg.dtype == dtype and ((dg.double() - wg).abs() <= tol).all()
 
 
