@@ -26,21 +26,21 @@ constexpr int kThreads = 256;
 constexpr int kHalves = kThreads / kLanes;  // blocks a CTA works on at a time
 
 // ------------------------------------------------ eight columns of a row
-template <typename T>
-struct Oct {
-  static constexpr int W = 2 * (int)sizeof(T);  // 32-bit words
+template <typename T, int N = 8>
+struct Oct {  // N columns
+  static constexpr int W = N * (int)sizeof(T) / 4;  // 32-bit words
   uint32_t w[W];
 };
 
-// Columns [c, c + n) of a row, n in [0, 8]; the others are zeros.  A row that does not start
-// on 16 bytes (32 for fp32) is read by the 16-byte words that hold its columns, shifted into
+// Columns [c, c + n) of a row, n in [0, N]; the others are zeros.  A row that does not start
+// on 16 bytes (32 for eight of fp32) is read by the 16-byte words that hold its columns, shifted into
 // place (each word that is read holds at least one of them, so none lies outside the row's memory).
-template <typename T>
-ECO_DEV Oct<T> load8(const T* row, int c, int n) {
-  constexpr int W = Oct<T>::W, V = W / 4;  // 32-bit words, 16-byte words
-  Oct<T> o;
+template <typename T, int N = 8>
+ECO_DEV Oct<T, N> load8(const T* row, int c, int n) {
+  constexpr int W = Oct<T, N>::W, V = W / 4;  // 32-bit words, 16-byte words
+  Oct<T, N> o;
   const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
-  if (n == 8 && (a & (16 * V - 1)) == 0) {
+  if (n == N && (a & (16 * V - 1)) == 0) {
     if constexpr (V == 2) {
       // volatile: without it the load counts as a pure function of the address, free to move in
       // front of the conditions that say the address is good
@@ -96,17 +96,17 @@ ECO_DEV void unpack8(const Oct<T>& o, float (&f)[8]) {
   }
 }
 
-// Eight columns of an output row: whole where eight columns of the row start on a boundary of
+// Eight columns of an output row (past L1, which keeps what is read again: a weight): whole where eight columns of the row start on a boundary of
 // their size (its padding takes the rest of the last eight), else n single stores.
 template <typename T>
 ECO_DEV void store8(T* row, int c, int n, bool vec, const float (&f)[8]) {
   if (vec) {
     if constexpr (sizeof(T) == 4) {
-      asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c), "f"(f[0]), "f"(f[1]),
+      asm volatile("st.global.cg.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(row + c), "f"(f[0]), "f"(f[1]),
                    "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
                    : "memory");
     } else {
-      *reinterpret_cast<uint4*>(row + c) = RowIo<T>::pack(f);
+      __stcg(reinterpret_cast<uint4*>(row + c), RowIo<T>::pack(f));
     }
     return;
   }
@@ -143,18 +143,18 @@ ECO_DEV float block_amax(const Oct<T>& o) {
     else return __half2float(__ushort_as_half((unsigned short)m));
   }
 }
-// Gains of N blocks of a half-warp from their maxima, and in lane i (< N) the scale of block i:
+// Gains of N blocks of a half-warp (or warp) from their maxima, and in lane i (< N) the scale of block i:
 // lane i does block i's two divisions, so that N blocks cost the divisions of one.
-template <int N>
+template <int N, int LANES = kLanes>
 ECO_DEV float block_gains(const float (&amax)[N], float (&gain)[N]) {
-  const int lane = threadIdx.x & (kLanes - 1);
+  const int lane = threadIdx.x & (LANES - 1);
   float m = amax[0];
 #pragma unroll
   for (int i = 1; i < N; ++i) m = lane == i ? amax[i] : m;
   const bool zero = m < 0x1p-119f;  // false for NaN
   const float g = zero ? 0.0f : __fdiv_rn(127.0f, m);
 #pragma unroll
-  for (int i = 0; i < N; ++i) gain[i] = N == 1 ? g : __shfl_sync(0xffffffffu, g, i, kLanes);
+  for (int i = 0; i < N; ++i) gain[i] = N == 1 ? g : __shfl_sync(0xffffffffu, g, i, LANES);
   return zero ? 0.0f : (m < INFINITY ? __fdiv_rn(m, 127.0f) : __int_as_float(0x7fc00000));
 }
 // rint(x * gain) of eight values as bytes.  Adding 1.5 * 2^23 rounds to nearest even at the
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads) pack_kernel(Mat x, int rows, int col
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           unpack8(o[u], f);
-          if (n[u] > 0) __stcs(reinterpret_cast<uint2*>(S.q + r[u] * S.ld_q + c), quant8(f, gain[u]));
+          if (n[u] > 0) __stcg(reinterpret_cast<uint2*>(S.q + r[u] * S.ld_q + c), quant8(f, gain[u]));
           if (lane == u && live[u]) S.scale[r[u] * S.ld_s + b] = scale;
         }
       });
@@ -330,9 +330,9 @@ __global__ void __launch_bounds__(kThreads)
           for (int u = 0; u < U; ++u) {
             if (n[u] > 0) {
               unpack8(o[u].a, f);
-              __stcs(reinterpret_cast<uint2*>(SG.q + r[u] * SG.ld_q + c), quant8(f, gain[2 * u]));
+              __stcg(reinterpret_cast<uint2*>(SG.q + r[u] * SG.ld_q + c), quant8(f, gain[2 * u]));
               unpack8(o[u].b, f);
-              __stcs(reinterpret_cast<uint2*>(SU.q + r[u] * SU.ld_q + c), quant8(f, gain[2 * u + 1]));
+              __stcg(reinterpret_cast<uint2*>(SU.q + r[u] * SU.ld_q + c), quant8(f, gain[2 * u + 1]));
             }
             if (lane == 2 * u && live[u]) SG.scale[r[u] * SG.ld_s + b] = scale;
             if (lane == 2 * u + 1 && live[u]) SU.scale[r[u] * SU.ld_s + b] = scale;
@@ -392,22 +392,31 @@ __global__ void __launch_bounds__(kThreads)
 // y = x r w,  r = 1 / sqrt(mean x^2 + eps);  with x' = what the eight bits stand for, u = x' r:
 //   dx = r (w dy - u mean(w dy u)),   dw = sum over rows of dy u.
 //
-// NT threads hold a row, CH groups of eight columns each, so a row is read once; the sum is joined over the
-// threads in a fixed order, with one barrier a row.  A CTA walks down its rows, and each thread
-// copies its own columns of the next rows (Stage::kAhead) into shared memory while it works on one
-// (cp.async: no other thread reads them, so no barrier belongs to the copies): the bytes in
-// flight do not depend on how far the row's barrier has come.  Wider rows are read again for the second pass, and
-// their dw sums live in the CTA's own row of `part`.
-constexpr int kRmsThreads = 512;  // per SM: 128 registers each, and what the stages have room for
+// NT threads hold a row (32 columns each beyond 1024), so a row is read once; the sum is joined
+// over the threads in a fixed order.  A CTA walks down its rows, and each thread copies its own
+// columns of the next rows into shared memory while it works on one (cp.async: no other thread
+// reads them, so no barrier belongs to the copies): the bytes in flight do not depend on how far
+// the row's barrier has come.  The weight stays in shared memory as well: with this much of it
+// in use L1 is too small for a weight (the backward lost a third of its time to L2's latency).
+// Wider rows are read again for the second pass, and their dw sums live in the CTA's own row of
+// `part`.
+constexpr int kRmsThreads = 512;  // of a CTA, one per SM: 128 registers each
 
+// A barrier of NT threads, those of row group `group` (the whole CTA has barrier 0).
 template <int NT>
-ECO_DEV float row_sum(float v, float* sh) {  // sh: this row's buffer (two take turns)
+ECO_DEV void row_barrier(int group) {
+  if constexpr (NT == 32) __syncwarp();
+  else asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(NT) : "memory");
+}
+// Sum over the NT threads of a row; sh: NT / 32 floats of the row group's (two buffers take turns).
+template <int NT>
+ECO_DEV float row_sum(float v, float* sh, int group) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if (NT > 32) {
+  if constexpr (NT > 32) {
     constexpr int W = NT / 32;
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x % NT / 32] = v;
+    row_barrier<NT>(group);
     v = sh[threadIdx.x % W];
 #pragma unroll
     for (int o = W / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -429,262 +438,335 @@ ECO_DEV void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// One thread's columns of a row on their way: CH groups of T (16-byte pieces, a piece of all
-// threads side by side), and for the backward the bytes, scales and the row's rstd.
-template <typename T, int CH, bool BWD>
-struct Stage {
-  static constexpr int V = Oct<T>::W / 4;
-  static constexpr int kBytes = CH * 16 * V + (BWD ? CH * 12 + 4 : 0);  // per thread
-  // Rows on their way besides the one in work: what an SM's stages have room for.
-  static constexpr int kRoom = 200 * 1024 / (kBytes * kRmsThreads) - 1;
-  static constexpr int kAhead = kRoom > 3 ? 3 : kRoom;
-  ECO_DEV static uint4* piece(char* st, int threads, int i, int v) {
-    return reinterpret_cast<uint4*>(st) + (i * V + v) * threads + threadIdx.x;
+// A unit is 16 bytes of x (or dy): G columns, with G of the eight-bit bytes.  Unit j of thread tid is
+// columns (j NT + tid) G: a warp's accesses are contiguous, and a block of 128 columns is 128 / G
+// lanes of one warp.
+template <typename T>
+struct Unit {
+  static constexpr int G = 16 / (int)sizeof(T), kLanes = kBlock / G;
+  ECO_DEV static void unpack(const uint4& r, float (&f)[G]) { RowIo<T>::unpack(r, f); }
+  // max |x| over the block's lanes: a whole warp's in one instruction, or half a warp's
+  ECO_DEV static float amax(const uint4& r) {
+    if constexpr (G == 4) {
+      const uint32_t m = max(max(r.x & 0x7fffffffu, r.y & 0x7fffffffu), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+      return __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+    } else {
+      return block_amax(Oct<T>{{r.x, r.y, r.z, r.w}});
+    }
   }
-  ECO_DEV static uint2* bytes(char* st, int threads, int i) {
-    return reinterpret_cast<uint2*>(st + CH * 16 * V * threads) + i * threads + threadIdx.x;
+  ECO_DEV static uint4 load(const T* row, int c, int n) {  // any alignment, n of the columns
+    const Oct<T, G> o = load8<T, G>(row, c, n);
+    return make_uint4(o.w[0], o.w[1], o.w[2], o.w[3]);
   }
-  ECO_DEV static float* word(char* st, int threads, int i) {  // scales, then rstd
-    return reinterpret_cast<float*>(st + CH * (16 * V + 8) * threads) + i * threads + threadIdx.x;
+  ECO_DEV static void put_bytes(int8_t* q, const float (&f)[G], float gain) {
+    uint32_t b[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) b[i] = __float_as_uint(__fadd_rn(__fmul_rn(f[i], gain), 12582912.0f));
+    const uint32_t lo = pack4(b[0], b[1], b[2], b[3]);
+    if constexpr (G == 4)
+      __stcg(reinterpret_cast<uint32_t*>(q), lo);
+    else
+      __stcg(reinterpret_cast<uint2*>(q), make_uint2(lo, pack4(b[4], b[5], b[6], b[7])));
+  }
+  // byte + 128 in the low mantissa bits of 2^23, less 2^23 + 128: two short operations where a
+  // conversion has a long wait
+  ECO_DEV static void bytes(uint2 q, float (&f)[G]) {
+    const uint32_t w[2] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u};
+#pragma unroll
+    for (int i = 0; i < G; ++i)
+      f[i] = __uint_as_float(__byte_perm(w[i / 4], 0x4B000000u, 0x7440u | (uint32_t)(i & 3))) - 8388736.0f;
   }
 };
+ECO_DEV int left(int cols, int c, int g) { return max(0, min(g, cols - c)); }
 
-// The weight: nothing (ones), fp32 or x's type.  WHOLE: groups of eight columns on 16 bytes.
+// The weight: nothing (ones), fp32 or x's type.
 struct Weight {
   const void* p;
   bool f32;
 };
-template <typename T, bool WHOLE>
-ECO_DEV void load_weight(const Weight& w, int c, int n, float (&f)[8]) {
-  if (!w.p || n == 0) {
+template <typename T, int G>
+ECO_DEV void load_weight(const Weight& w, int c, int n, float (&f)[G]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = 1.0f;
-  } else if constexpr (WHOLE) {
-    if (sizeof(T) == 4 || w.f32) {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(w.p) + c);
-      const float4 a = __ldg(p), b = __ldg(p + 1);
-      f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
-    } else if constexpr (sizeof(T) == 2) {
-      const uint4 t = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(w.p) + c));
-      const Oct<T> o{t.x, t.y, t.z, t.w};
-      unpack8(o, f);
+  for (int k = 0; k < G; ++k) f[k] = 1.0f;
+  if (!w.p || n == 0) return;
+  if (w.f32) {
+    const float* p = static_cast<const float*>(w.p) + c;
+    if (n == G && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+      for (int v = 0; v < G / 4; ++v) {
+        const float4 t = __ldg(reinterpret_cast<const float4*>(p) + v);
+        f[4 * v] = t.x, f[4 * v + 1] = t.y, f[4 * v + 2] = t.z, f[4 * v + 3] = t.w;
+      }
+      return;
     }
-  } else if (w.f32) {
-    unpack8(load8(static_cast<const float*>(w.p), c, n), f);
-  } else {
-    unpack8(load8(static_cast<const T*>(w.p), c, n), f);
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (k < n) f[k] = __ldg(p + k);
+  } else if constexpr (sizeof(T) == 2) {
+    const T* p = static_cast<const T*>(w.p) + c;
+    if (n == G && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      RowIo<T>::unpack(__ldg(reinterpret_cast<const uint4*>(p)), f);
+      return;
+    }
+#pragma unroll
+    for (int k = 0; k < G; ++k)
+      if (k < n) f[k] = to_f32(p[k]);
   }
 }
 
-// WHOLE: rows start on 16 bytes and consist of whole groups of eight columns, and so does the
-// weight; else a row is loaded when it is needed.
-template <typename T, int NT, int CH, bool WHOLE>
-__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, kRmsThreads / (NT == 32 ? kThreads : NT))
+// Shared memory of a CTA: the weight of a row's columns in fp32, then R rows' stages for each of
+// its row groups.  A stage holds what is on its way for one row: U units of all threads side by
+// side; for the backward also their bytes, each block's scale and the row's rstd (copied by the
+// first lane of the block or warp, read by its other lanes).
+template <typename T, int NT, int U, bool BWD>
+struct Stages {
+  static constexpr int G = Unit<T>::G, kScales = kRmsThreads / Unit<T>::kLanes;
+  static constexpr int kWeight = NT * U * G * 4;
+  static constexpr int kUnit = kRmsThreads * (16 + (BWD ? G : 0)) + (BWD ? kScales * 4 : 0);
+  static constexpr int kStage = U * kUnit + (BWD ? kRmsThreads / 32 * 4 : 0);
+  static constexpr int kRoom = (222 * 1024 - kWeight) / kStage;
+  static constexpr int R = kRoom > 4 ? 4 : kRoom;
+  static constexpr int kBytes = kWeight + R * kStage;
+  static_assert(R >= 1 && kUnit % 16 == 0 && kStage % 16 == 0, "a row's stage has to fit");
+  char* p;
+  ECO_DEV float4* weight(int j, int v) const {
+    return reinterpret_cast<float4*>(p) + (j * (G / 4) + v) * NT + threadIdx.x % NT;
+  }
+  ECO_DEV char* unit(int s, int j) const { return p + kWeight + s * kStage + j * kUnit; }
+  ECO_DEV uint4* data(int s, int j) const { return reinterpret_cast<uint4*>(unit(s, j)) + threadIdx.x; }
+  ECO_DEV char* bytes(int s, int j) const { return unit(s, j) + 16 * kRmsThreads + threadIdx.x * G; }
+  ECO_DEV float* scale(int s, int j) const {
+    return reinterpret_cast<float*>(unit(s, j) + (16 + G) * kRmsThreads) + threadIdx.x / Unit<T>::kLanes;
+  }
+  ECO_DEV float* rstd(int s) const { return reinterpret_cast<float*>(unit(s, U)) + threadIdx.x / 32; }
+  ECO_DEV void put_weight(int j, const float (&f)[G]) const {
+#pragma unroll
+    for (int v = 0; v < G / 4; ++v) *weight(j, v) = make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
+  }
+  ECO_DEV void get_weight(int j, float (&f)[G]) const {
+#pragma unroll
+    for (int v = 0; v < G / 4; ++v) {
+      const float4 t = *weight(j, v);
+      f[4 * v] = t.x, f[4 * v + 1] = t.y, f[4 * v + 2] = t.z, f[4 * v + 3] = t.w;
+    }
+  }
+};
+
+// WHOLE: rows start on 16 bytes and consist of whole units, which are copied ahead (R rows of
+// them: a unit's place is filled again as soon as it has been read); else a row is loaded when it
+// is needed.
+template <typename T, int NT, int U, bool WHOLE>
+__global__ void __launch_bounds__(kRmsThreads, 1)
     rms_fwd_kernel(Mat x, int rows, int cols, const Weight w, float eps, Mat y, Saved S, float* rstd) {
-  extern __shared__ __align__(16) char stages[];
-  __shared__ float sh[2][NT / 32];
-  using St = Stage<T, CH, false>;
-  constexpr int THREADS = NT == 32 ? kThreads : NT, RPC = THREADS / NT;
-  constexpr int kStage = St::kBytes * THREADS, kAhead = St::kAhead;
-  const int tid = threadIdx.x % NT, step = (int)gridDim.x * RPC, lane = threadIdx.x & (kLanes - 1);
-  int r = (int)blockIdx.x * RPC + threadIdx.x / NT;
+  constexpr int GROUPS = kRmsThreads / NT;
+  constexpr int G = Unit<T>::G, LB = Unit<T>::kLanes;
+  using St = Stages<T, NT, U, false>;
+  constexpr int R = St::R;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float sh[2][kRmsThreads / 32];
+  const St st{smem};
+  const int tid = threadIdx.x % NT, group = threadIdx.x / NT, step = (int)gridDim.x * GROUPS;
+  const int lane = threadIdx.x & (LB - 1), c = tid * G;
+  int r = (int)blockIdx.x * GROUPS + group;
   const float inv_cols = 1.0f / (float)cols;
-  // groups of eight columns c, c + NT * 8, ...: how many columns each
-  const int c = tid * 8;
-  int n[CH];
-#pragma unroll
-  for (int i = 0; i < CH; ++i) n[i] = left8(cols, c + i * NT * 8);
-  int ahead = r;  // the next row to be copied
-  auto issue = [&](int slot) {
-    if (WHOLE && ahead < rows) {
-      const T* src = static_cast<const T*>(x.p) + (int64_t)ahead * x.ld + c;
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (n[i] > 0) {
-#pragma unroll
-          for (int v = 0; v < St::V; ++v)
-            copy_async<16>(St::piece(stages + slot * kStage, THREADS, i, v), src + i * NT * 8 + v * (16 / (int)sizeof(T)));
-        }
-    }
+  auto n_of = [&](int j) { return WHOLE ? (c + j * NT * G < cols ? G : 0) : left(cols, c + j * NT * G, G); };
+  auto issue = [&](int row, int s, int j) {
+    if (WHOLE && row < rows && c + j * NT * G < cols)
+      copy_async<16>(st.data(s, j), static_cast<const T*>(x.p) + (int64_t)row * x.ld + c + j * NT * G);
     copies_commit();
-    ahead += step;
   };
-  for (int d = 0; d < kAhead; ++d) issue(d);
-  int slot = 0, par = 0;
+#pragma unroll
+  for (int s = 0; s < R; ++s)
+#pragma unroll
+    for (int j = 0; j < U; ++j) issue(r + s * step, s, j);
+  if (group == 0) {
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      float f[G];
+      load_weight<T, G>(w, c + j * NT * G, n_of(j), f);
+      st.put_weight(j, f);
+    }
+  }
+  __syncthreads();
+  int s = 0, par = 0;
   for (; r < rows; r += step) {
-    issue(slot == 0 ? kAhead : slot - 1);
-    Oct<T> o[CH];
-    if constexpr (WHOLE) {
-      copies_wait<kAhead>();
-      char* st = stages + slot * kStage;
+    uint4 raw[U];
+    float ss = 0.0f;
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
+    for (int j = 0; j < U; ++j) {
+      raw[j] = make_uint4(0u, 0u, 0u, 0u);
+      if constexpr (WHOLE) {
+        copies_wait<R * U - 1>();
+        if (n_of(j) > 0) raw[j] = *st.data(s, j);
+        issue(r + R * step, s, j);
+      } else {
+        raw[j] = Unit<T>::load(static_cast<const T*>(x.p) + (int64_t)r * x.ld, c + j * NT * G, n_of(j));
+      }
+      float f[G];
+      Unit<T>::unpack(raw[j], f);
 #pragma unroll
-        for (int v = 0; v < St::V; ++v) {
-          uint4 t = make_uint4(0u, 0u, 0u, 0u);
-          if (n[i] > 0) t = *St::piece(st, THREADS, i, v);
-          o[i].w[4 * v] = t.x, o[i].w[4 * v + 1] = t.y, o[i].w[4 * v + 2] = t.z, o[i].w[4 * v + 3] = t.w;
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-        o[i] = load8(static_cast<const T*>(x.p) + (int64_t)r * x.ld, c + i * NT * 8, n[i]);
+      for (int k = 0; k < G; ++k) ss = fmaf(f[k], f[k], ss);
     }
-    slot = slot == kAhead ? 0 : slot + 1;
-    float ss = 0.0f, f[CH][8];
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      unpack8(o[i], f[i]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(f[i][j], f[i][j], ss);
-    }
+    s = s == R - 1 ? 0 : s + 1;
     if (S.q) {  // in front of the row's barrier: it needs no sum
-      float amax[CH], gain[CH];
+      float amax[U], gain[U];
 #pragma unroll
-      for (int i = 0; i < CH; ++i) amax[i] = block_amax(o[i]);
-      const float scale = block_gains(amax, gain);
+      for (int j = 0; j < U; ++j) amax[j] = Unit<T>::amax(raw[j]);
+      const float scale = block_gains<U, LB>(amax, gain);
       int8_t* q = S.q + (int64_t)r * S.ld_q + c;
       float* sc = S.scale + (int64_t)r * S.ld_s + c / kBlock;
 #pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        if (n[i] > 0) __stcs(reinterpret_cast<uint2*>(q + i * NT * 8), quant8(f[i], gain[i]));
-        if (lane == i && c - 8 * lane + i * NT * 8 < cols) sc[i * (NT * 8 / kBlock)] = scale;
+      for (int j = 0; j < U; ++j) {
+        float f[G];
+        Unit<T>::unpack(raw[j], f);
+        if (n_of(j) > 0) Unit<T>::put_bytes(q + j * NT * G, f, gain[j]);
+        if (lane == j && c - G * lane + j * NT * G < cols) sc[j * (NT * G / kBlock)] = scale;
       }
     }
-    ss = row_sum<NT>(ss, sh[par]);
+    ss = row_sum<NT>(ss, sh[par] + group * (NT / 32), group);
     par ^= 1;
     const float rs = rsqrtf(fmaf(ss, inv_cols, eps));
     if (tid == 0 && rstd) rstd[r] = rs;
     T* out = static_cast<T*>(y.p) + (int64_t)r * y.ld + c;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      float wt[8];
-      load_weight<T, WHOLE>(w, c + i * NT * 8, n[i], wt);
+    for (int j = 0; j < U; ++j) {
+      float f[G], wt[G];
+      Unit<T>::unpack(raw[j], f);
+      st.get_weight(j, wt);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[i][j] = f[i][j] * rs * wt[j];
-      if (n[i] > 0) store8(out, i * NT * 8, n[i], true, f[i]);
+      for (int k = 0; k < G; ++k) f[k] = f[k] * rs * wt[k];
+      if (n_of(j) > 0) __stcg(reinterpret_cast<uint4*>(out + j * NT * G), RowIo<T>::pack(f));
     }
   }
 }
 
-template <typename T, int NT, int CH, bool WHOLE>
-__global__ void __launch_bounds__(NT == 32 ? kThreads : NT, kRmsThreads / (NT == 32 ? kThreads : NT))
+template <typename T, int NT, int U, bool WHOLE>
+__global__ void __launch_bounds__(kRmsThreads, 1)
     rms_bwd_kernel(Mat dy, int rows, int cols, const Weight w, Saved S, const float* __restrict__ rstd, Mat dx,
                    float* part, int64_t ld_part) {
-  extern __shared__ __align__(16) char stages[];
-  __shared__ float sh[2][NT / 32];
-  using St = Stage<T, CH, true>;
-  constexpr int THREADS = NT == 32 ? kThreads : NT, RPC = THREADS / NT;
-  constexpr int kStage = St::kBytes * THREADS, kAhead = St::kAhead;
-  const int tid = threadIdx.x % NT, step = (int)gridDim.x * RPC;
-  int r = (int)blockIdx.x * RPC + threadIdx.x / NT;
+  constexpr int GROUPS = kRmsThreads / NT;
+  constexpr int G = Unit<T>::G, LB = Unit<T>::kLanes;
+  using St = Stages<T, NT, U, true>;
+  constexpr int R = St::R;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float sh[2][kRmsThreads / 32];
+  const St st{smem};
+  const int tid = threadIdx.x % NT, group = threadIdx.x / NT, step = (int)gridDim.x * GROUPS;
+  const int lane = threadIdx.x & (LB - 1), c = tid * G;
+  int r = (int)blockIdx.x * GROUPS + group;
   const float inv_cols = 1.0f / (float)cols;
-  const int c = tid * 8;
-  int n[CH];
-#pragma unroll
-  for (int i = 0; i < CH; ++i) n[i] = left8(cols, c + i * NT * 8);
-  int ahead = r;
-  auto issue = [&](int slot) {
-    if (WHOLE && ahead < rows) {
-      char* st = stages + slot * kStage;
-      const T* src = static_cast<const T*>(dy.p) + (int64_t)ahead * dy.ld + c;
-      const int8_t* q = S.q + (int64_t)ahead * S.ld_q + c;
-      const float* sc = S.scale + (int64_t)ahead * S.ld_s + c / kBlock;
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int at = i * NT * 8;
-        if (n[i] > 0) {
-#pragma unroll
-          for (int v = 0; v < St::V; ++v)
-            copy_async<16>(St::piece(st, THREADS, i, v), src + at + v * (16 / (int)sizeof(T)));
-          copy_async<8>(St::bytes(st, THREADS, i), q + at);
-          copy_async<4>(St::word(st, THREADS, i), sc + at / kBlock);
-        }
+  auto n_of = [&](int j) { return WHOLE ? (c + j * NT * G < cols ? G : 0) : left(cols, c + j * NT * G, G); };
+  auto issue = [&](int row, int s, int j) {
+    const int at = c + j * NT * G;
+    if (WHOLE && row < rows) {
+      if (at < cols) {
+        copy_async<16>(st.data(s, j), static_cast<const T*>(dy.p) + (int64_t)row * dy.ld + at);
+        copy_async<G>(st.bytes(s, j), S.q + (int64_t)row * S.ld_q + at);
+        if (lane == 0) copy_async<4>(st.scale(s, j), S.scale + (int64_t)row * S.ld_s + at / kBlock);
       }
-      copy_async<4>(St::word(st, THREADS, CH), rstd + ahead);
+      if (j == 0 && (threadIdx.x & 31) == 0) copy_async<4>(st.rstd(s), rstd + row);
     }
     copies_commit();
-    ahead += step;
   };
-  for (int d = 0; d < kAhead; ++d) issue(d);
-  float acc[CH][8] = {};
-  int slot = 0, par = 0;
-  for (; r < rows; r += step) {
-    issue(slot == 0 ? kAhead : slot - 1);
-    if constexpr (WHOLE) copies_wait<kAhead>();
-    char* st = stages + slot * kStage;
-    slot = slot == kAhead ? 0 : slot + 1;
-    const float rs = WHOLE ? *St::word(st, THREADS, CH) : rstd[r];
-    // u = byte * scale * rstd: the factor, one per group, goes where it is used once
-    float dot = 0.0f, d[CH][8], k[CH];
-    uint2 bytes[CH];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      Oct<T> o;
-      Eights e{make_uint2(0u, 0u), 0.0f};
-      if constexpr (WHOLE) {
+  for (int s = 0; s < R; ++s)
 #pragma unroll
-        for (int v = 0; v < St::V; ++v) {
-          uint4 t = make_uint4(0u, 0u, 0u, 0u);
-          if (n[i] > 0) t = *St::piece(st, THREADS, i, v);
-          o.w[4 * v] = t.x, o.w[4 * v + 1] = t.y, o.w[4 * v + 2] = t.z, o.w[4 * v + 3] = t.w;
-        }
-        if (n[i] > 0) e = Eights{*St::bytes(st, THREADS, i), *St::word(st, THREADS, i)};
-      } else {
-        o = load8(static_cast<const T*>(dy.p) + (int64_t)r * dy.ld, c + i * NT * 8, n[i]);
-        e = fetch8(S, r, c + i * NT * 8, n[i]);
-      }
-      float wt[8], u[8], part_dot = 0.0f;
-      load_weight<T, WHOLE>(w, c + i * NT * 8, n[i], wt);  // from L1: registers hold the sums
-      unpack8(o, d[i]);
-      dequant8(e.q, u);
-      bytes[i] = e.q;
-      k[i] = e.s * rs;
+    for (int j = 0; j < U; ++j) issue(r + s * step, s, j);
+  if (group == 0) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        acc[i][j] = fmaf(d[i][j] * k[i], u[j], acc[i][j]);
-        d[i][j] *= wt[j];
-        part_dot = fmaf(d[i][j], u[j], part_dot);
-      }
-      dot = fmaf(part_dot, k[i], dot);
+    for (int j = 0; j < U; ++j) {
+      float f[G];
+      load_weight<T, G>(w, c + j * NT * G, n_of(j), f);
+      st.put_weight(j, f);
     }
-    dot = row_sum<NT>(dot, sh[par]) * inv_cols;
+  }
+  __syncthreads();
+  float acc[U][G] = {};
+  int s = 0, par = 0;
+  for (; r < rows; r += step) {
+    // u = byte * scale * rstd: the factor, one per unit, goes where it is used once
+    float dot = 0.0f, d[U][G], k[U], rs = 0.0f;
+    uint2 bytes[U];
+    uint4 raw;
+    auto take = [&](int j) {  // unit j's dy, bytes and factor; its place is free again
+      raw = make_uint4(0u, 0u, 0u, 0u);
+      bytes[j] = make_uint2(0u, 0u);
+      k[j] = 0.0f;
+      if constexpr (WHOLE) {
+        copies_wait<R * U - 1>();
+        __syncwarp();  // the first lanes' copies too
+        if (n_of(j) > 0) {
+          raw = *st.data(s, j);
+          if constexpr (G == 8) bytes[j] = *reinterpret_cast<const uint2*>(st.bytes(s, j));
+          else bytes[j].x = *reinterpret_cast<const uint32_t*>(st.bytes(s, j));
+          k[j] = *st.scale(s, j);
+        }
+        if (j == 0) rs = *st.rstd(s);
+        __syncwarp();  // read by all
+        issue(r + R * step, s, j);
+      } else {
+        const int n = n_of(j), at = c + j * NT * G;
+        raw = Unit<T>::load(static_cast<const T*>(dy.p) + (int64_t)r * dy.ld, at, n);
+        if (n > 0) {
+          const int8_t* q = S.q + (int64_t)r * S.ld_q + at;
+          if constexpr (G == 8) bytes[j] = __ldcs(reinterpret_cast<const uint2*>(q));
+          else bytes[j].x = __ldcs(reinterpret_cast<const uint32_t*>(q));
+          k[j] = __ldg(S.scale + (int64_t)r * S.ld_s + at / kBlock);
+        }
+        if (j == 0) rs = __ldg(rstd + r);
+      }
+    };
+    take(0);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      Unit<T>::unpack(raw, d[j]);
+      if (j + 1 < U) take(j + 1);  // its loads are on their way while unit j is worked on
+      float wt[G], u[G], part_dot = 0.0f;
+      st.get_weight(j, wt);
+      Unit<T>::bytes(bytes[j], u);
+      k[j] *= rs;
+#pragma unroll
+      for (int i = 0; i < G; ++i) {
+        acc[j][i] = fmaf(d[j][i] * k[j], u[i], acc[j][i]);
+        d[j][i] *= wt[i];
+        part_dot = fmaf(d[j][i], u[i], part_dot);
+      }
+      dot = fmaf(part_dot, k[j], dot);
+    }
+    s = s == R - 1 ? 0 : s + 1;
+    dot = row_sum<NT>(dot, sh[par] + group * (NT / 32), group) * inv_cols;
     par ^= 1;
     T* out = static_cast<T*>(dx.p) + (int64_t)r * dx.ld + c;
 #pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const float kd = k[i] * dot;
-      float u[8];
-      asm volatile("" : "+r"(bytes[i].x), "+r"(bytes[i].y));  // converted again: the bytes take a quarter of the room
-      dequant8(bytes[i], u);
+    for (int j = 0; j < U; ++j) {
+      const float kd = k[j] * dot;
+      float u[G];
+      asm volatile("" : "+r"(bytes[j].x), "+r"(bytes[j].y));  // converted again: bytes take a quarter of the room
+      Unit<T>::bytes(bytes[j], u);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) d[i][j] = rs * fmaf(-u[j], kd, d[i][j]);
-      if (n[i] > 0) store8(out, i * NT * 8, n[i], true, d[i]);
+      for (int i = 0; i < G; ++i) d[j][i] = rs * fmaf(-u[i], kd, d[j][i]);
+      if (n_of(j) > 0) __stcg(reinterpret_cast<uint4*>(out + j * NT * G), RowIo<T>::pack(d[j]));
     }
   }
-  if (part) {
+  if (part) {  // the row groups' sums to one row of them, in order
     float* mine = part + (int64_t)blockIdx.x * ld_part;
-    if constexpr (NT == 32) {  // the CTA's eight rows of sums to one, in order
-      constexpr int kSpan = CH * NT * 8;
-      static_assert(RPC * kSpan * 4 <= kStage * (kAhead + 1), "the stages hold the rows of sums");
-      float* joined = reinterpret_cast<float*>(stages);
-      copies_wait<0>();
-      __syncthreads();  // no stage is in use
+    constexpr int kSpan = U * NT * G;
+    static_assert(GROUPS * kSpan * 4 <= St::kBytes, "the shared memory holds the groups' sums");
+    float* joined = reinterpret_cast<float*>(smem);
+    copies_wait<0>();
+    __syncthreads();  // nothing there is in use
 #pragma unroll
-      for (int i = 0; i < CH; ++i)
+    for (int j = 0; j < U; ++j)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) joined[threadIdx.x / NT * kSpan + c + i * NT * 8 + j] = acc[i][j];
-      __syncthreads();
-      for (int at = threadIdx.x; at < cols; at += THREADS) {
-        float v = joined[at];
+      for (int v = 0; v < G / 4; ++v)
+        reinterpret_cast<float4*>(joined + group * kSpan + c + j * NT * G)[v] =
+            make_float4(acc[j][4 * v], acc[j][4 * v + 1], acc[j][4 * v + 2], acc[j][4 * v + 3]);
+    __syncthreads();
+    for (int at = threadIdx.x; at < cols; at += kRmsThreads) {
+      float v = joined[at];
 #pragma unroll
-        for (int w8 = 1; w8 < RPC; ++w8) v += joined[w8 * kSpan + at];
-        mine[at] = v;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-        if (n[i] > 0) store8(mine, c + i * NT * 8, 8, true, acc[i]);
+      for (int g = 1; g < GROUPS; ++g) v += joined[g * kSpan + at];
+      mine[at] = v;
     }
   }
 }
@@ -708,7 +790,7 @@ __global__ void __launch_bounds__(kWide)
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
     }
-    ss = row_sum<kWide>(ss, sh[k & 1]);
+    ss = row_sum<kWide>(ss, sh[k & 1], 0);
     const float rs = rsqrtf(ss / (float)cols + eps);
     if (threadIdx.x == 0 && rstd) rstd[r] = rs;
     for (int cc = 0; cc < cols; cc += kWide * 8) {  // every lane, for the shuffles
@@ -721,10 +803,10 @@ __global__ void __launch_bounds__(kWide)
         const float amax[1] = {block_amax(o)};
         float gain[1];
         const float scale = block_gains(amax, gain);
-        if (n > 0) __stcs(reinterpret_cast<uint2*>(S.q + r * S.ld_q + c), quant8(f, gain[0]));
+        if (n > 0) __stcg(reinterpret_cast<uint2*>(S.q + r * S.ld_q + c), quant8(f, gain[0]));
         if (lane == 0 && c0 < cols) S.scale[r * S.ld_s + c0 / kBlock] = scale;
       }
-      load_weight<T, false>(w, c, n, wt);
+      load_weight<T, 8>(w, c, n, wt);
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = f[j] * rs * wt[j];
       if (n > 0) store8(static_cast<T*>(y.p) + r * y.ld, c, n, true, f);
@@ -750,7 +832,7 @@ __global__ void __launch_bounds__(kWide)
       Eights e = fetch8(S, r, c, n);
       e.s *= rs;
       values8(e, u);
-      load_weight<T, false>(w, c, n, wt);
+      load_weight<T, 8>(w, c, n, wt);
       if (mine) {  // a thread owns its columns of the CTA's sums: plain loads and stores, no atomics
         float4* at = reinterpret_cast<float4*>(mine + c);
         float4 s0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), s1 = s0;
@@ -761,7 +843,7 @@ __global__ void __launch_bounds__(kWide)
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot = fmaf(d[j] * wt[j], u[j], dot);
     }
-    dot = row_sum<kWide>(dot, sh[k & 1]) / (float)cols;
+    dot = row_sum<kWide>(dot, sh[k & 1], 0) / (float)cols;
     for (int c = threadIdx.x * 8; c < cols; c += kWide * 8) {
       const int n = left8(cols, c);
       float d[8], u[8], wt[8];
@@ -769,7 +851,7 @@ __global__ void __launch_bounds__(kWide)
       Eights e = fetch8(S, r, c, n);
       e.s *= rs;
       values8(e, u);
-      load_weight<T, false>(w, c, n, wt);
+      load_weight<T, 8>(w, c, n, wt);
 #pragma unroll
       for (int j = 0; j < 8; ++j) d[j] = rs * fmaf(-u[j], dot, d[j] * wt[j]);
       store8(static_cast<T*>(dx.p) + r * dx.ld, c, n, true, d);
@@ -879,18 +961,17 @@ void by_width(int64_t cols, F f) {
   else if (cols <= 16384) f(integral_constant<int, 512>{}, integral_constant<int, 4>{});
   else f(integral_constant<int, 0>{}, integral_constant<int, 0>{});
 }
-// Rows of whole groups of eight columns on 16 bytes, and a weight on 16 bytes.
-bool whole_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const void* w) {
-  return rows_on_16(p, ld, rows, type) && cols % 8 == 0 && eco_aligned16(w);
+// Rows of whole units on 16 bytes.
+bool whole_rows(const void* p, int64_t ld, int64_t rows, int64_t cols, int type) {
+  return rows_on_16(p, ld, rows, type) && cols * es_of(type) % 16 == 0;
 }
-// CTAs of the norm's kernels: what is resident.
+// CTAs of the norm's kernels: what is resident (two of the two-pass kernels per SM).
 int64_t rms_ctas(int64_t rows, int64_t cols) {
   int64_t n = 0;
   by_width(cols, [&](auto nt, auto) {
     constexpr int NT = decltype(nt)::value;
-    constexpr int threads = NT == 0 ? kWide : NT == 32 ? kThreads : NT, rpc = NT == 32 ? kThreads / 32 : 1;
-    const int per_sm = NT == 0 ? 1024 / kWide : kRmsThreads / threads;
-    n = std::min<int64_t>((rows + rpc - 1) / rpc, (int64_t)eco_num_sms() * per_sm);
+    const int64_t groups = NT == 0 ? 1 : kRmsThreads / (NT ? NT : 1);
+    n = std::min<int64_t>((rows + groups - 1) / groups, (int64_t)eco_num_sms() * (NT == 0 ? 2 : 1));
   });
   return n;
 }
@@ -1020,13 +1101,13 @@ extern "C" int eco_rms_norm(const void* x, int64_t ld, int type, int64_t rows, i
         rms_fwd_wide_kernel<T><<<grid, kWide, 0, eco_stream(stream)>>>(xi, (int)rows, (int)cols, wt, (float)eps, yo,
                                                                        saved_of(saved), rstd);
       } else {
-        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, CH, false>::kBytes * threads * (Stage<T, CH, false>::kAhead + 1);
-        if (!whole_rows(x, ld, rows, cols, type, w))
-          rms_fwd_kernel<T, NT, CH, false><<<grid, threads, 0, eco_stream(stream)>>>(xi, (int)rows, (int)cols, wt, (float)eps,
-                                                                                 yo, saved_of(saved), rstd);
-        else if ((ok = allow_smem(rms_fwd_kernel<T, NT, CH, true>, smem)))
-          rms_fwd_kernel<T, NT, CH, true><<<grid, threads, smem, eco_stream(stream)>>>(xi, (int)rows, (int)cols, wt,
-                                                                                   (float)eps, yo, saved_of(saved), rstd);
+        constexpr int U = CH * 8 / Unit<T>::G, smem = Stages<T, NT, U, false>::kBytes;
+        const auto kernel = whole_rows(x, ld, rows, cols, type) ? rms_fwd_kernel<T, NT, U, true>
+                                                                : rms_fwd_kernel<T, NT, U, false>;
+        ok = allow_smem(kernel, smem);
+        if (ok)
+          kernel<<<grid, kRmsThreads, smem, eco_stream(stream)>>>(xi, (int)rows, (int)cols, wt, (float)eps, yo,
+                                                              saved_of(saved), rstd);
       }
     });
   });
@@ -1072,13 +1153,12 @@ extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t
         rms_bwd_wide_kernel<T><<<grid, kWide, 0, s>>>(d, (int)rows, (int)cols, wt, saved_of(saved), rstd, o, part,
                                                            ld_part);
       } else {
-        constexpr int threads = NT == 32 ? kThreads : NT, smem = Stage<T, CH, true>::kBytes * threads * (Stage<T, CH, true>::kAhead + 1);
-        const bool whole = whole_rows(dy, ld_dy, rows, cols, type, w);
-        const auto kernel = whole ? rms_bwd_kernel<T, NT, CH, true> : rms_bwd_kernel<T, NT, CH, false>;
-        const int bytes = whole || NT == 32 ? smem : 0;
-        ok = allow_smem(kernel, bytes);
+        constexpr int U = CH * 8 / Unit<T>::G, smem = Stages<T, NT, U, true>::kBytes;
+        const auto kernel = whole_rows(dy, ld_dy, rows, cols, type) ? rms_bwd_kernel<T, NT, U, true>
+                                                                    : rms_bwd_kernel<T, NT, U, false>;
+        ok = allow_smem(kernel, smem);
         if (ok)
-          kernel<<<grid, threads, bytes, s>>>(d, (int)rows, (int)cols, wt, saved_of(saved), rstd, o, part, ld_part);
+          kernel<<<grid, kRmsThreads, smem, s>>>(d, (int)rows, (int)cols, wt, saved_of(saved), rstd, o, part, ld_part);
       }
     });
   });
