@@ -1150,43 +1150,50 @@ extern "C" int eco_policy_grad(const eco_logits_t* logits, const int64_t* tokens
   return eco_launch_check("eco_policy_grad");
 }
 
-extern "C" int eco_policy_tokens(const double* logp64, const int64_t* tokens, const uint8_t* mask, int64_t rows,
-                                 int64_t cols, const float* old_logp, const float* adv, const float* ref_logp,
-                                 double low, double high, double kl_coef, double denom, float* coef, float* out,
-                                 eco_stream_t stream) {
-  ECO_REQUIRE(rows >= 0 && cols > 0 && out, ECO_ERR_ARG, "eco_policy_tokens: bad arguments");
+extern "C" int eco_policy_forward(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
+                                  const float* old_logp, const float* adv, const float* ref_logp, double low,
+                                  double high, double kl_coef, double denom, float* logp, double* logp64,
+                                  float* row_stats, float* coef, float* out, eco_stream_t stream) {
+  if (int rc = check_logits(logits, tokens, "eco_policy_forward")) return rc;
+  ECO_REQUIRE(out, ECO_ERR_ARG, "eco_policy_forward: null output");
+  const Rows R = rows_of(*logits, tokens, mask, nullptr, 0);
   cudaStream_t s = eco_stream(stream);
-  if (rows == 0) {
-    if (cudaMemsetAsync(out, 0, 3 * sizeof(float), s) != cudaSuccess) return eco_launch_check("eco_policy_tokens");
+  if (R.rows == 0) {
+    if (cudaMemsetAsync(out, 0, 3 * sizeof(float), s) != cudaSuccess) return eco_launch_check("eco_policy_forward");
     return ECO_OK;
   }
   Policy P;
-  if (int rc = policy_of(P, old_logp, adv, ref_logp, low, high, kl_coef, denom, "eco_policy_tokens")) return rc;
-  ECO_REQUIRE(logp64 && tokens && coef, ECO_ERR_ARG, "eco_policy_tokens: null pointers");
-  const eco_logits_t L{nullptr, ECO_F32, 0, 1, rows, 0, 0, cols, 1.0};
-  const Rows R = rows_of(L, tokens, mask, nullptr, 0);
+  if (int rc = policy_of(P, old_logp, adv, ref_logp, low, high, kl_coef, denom, "eco_policy_forward")) return rc;
+  ECO_REQUIRE(logp64 && row_stats && coef, ECO_ERR_ARG, "eco_policy_forward: null output");
+  if (int rc = eco_token_logp(logits, tokens, mask, nullptr, 0, logp, logp64, row_stats, nullptr, stream)) return rc;
   policy_tokens_kernel<<<1, 1024, 0, s>>>(R, P, logp64, coef, out);
-  return eco_launch_check("eco_policy_tokens");
+  return eco_launch_check("eco_policy_forward");
 }
 
-extern "C" int eco_preference_pairs(const double* logp64, const int64_t* tokens, const uint8_t* mask, int64_t rows,
-                                    int64_t cols, const float* ref_logp, const int32_t* cu_seqlens, int64_t seq_len,
-                                    int64_t pairs, int kind, double beta, double label_smoothing, int average,
-                                    double denom, float* coef, float* log_ratio, float* margin, double* pair_loss,
-                                    float* out, eco_stream_t stream) {
-  ECO_REQUIRE(rows >= 0 && cols > 0 && pairs > 0 && pairs < (1 << 30) && seq_len >= 0 && log_ratio && margin &&
-                  pair_loss && out && (rows == 0 || (logp64 && tokens && ref_logp && coef)),
-              ECO_ERR_ARG, "eco_preference_pairs: bad arguments");
-  ECO_REQUIRE(cu_seqlens || rows / 2 / pairs >= seq_len, ECO_ERR_ARG, "eco_preference_pairs: more sequences than rows");
+extern "C" int eco_preference(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
+                              const float* ref_logp, const int32_t* cu_seqlens, int64_t seq_len, int64_t pairs,
+                              int kind, double beta, double label_smoothing, int average, double denom, double gain,
+                              double* wide, float* row_stats, float* coef, float* log_ratio, float* margin,
+                              float* loss, const eco_grad_t* grad, eco_stream_t stream) {
+  if (int rc = check_logits(logits, tokens, "eco_preference")) return rc;
+  const Rows R = rows_of(*logits, tokens, mask, cu_seqlens, 2 * pairs);
+  ECO_REQUIRE(pairs > 0 && pairs < (1 << 30) && seq_len >= 0 && wide && log_ratio && margin && loss &&
+                  (R.rows == 0 || (ref_logp && row_stats && coef)),
+              ECO_ERR_ARG, "eco_preference: bad arguments");
+  ECO_REQUIRE(cu_seqlens || R.rows / 2 / pairs >= seq_len, ECO_ERR_ARG, "eco_preference: more sequences than rows");
   ECO_REQUIRE(kind >= ECO_PREFERENCE_SIGMOID && kind <= ECO_PREFERENCE_IPO, ECO_ERR_ARG,
-              "eco_preference_pairs: unknown kind %d", kind);
+              "eco_preference: unknown kind %d", kind);
   ECO_REQUIRE(std::isfinite(beta) && beta > 0.0 && label_smoothing >= 0.0 && label_smoothing <= 1.0 && denom > 0.0,
-              ECO_ERR_ARG, "eco_preference_pairs: bad beta, smoothing or denominator");
-  const eco_logits_t L{nullptr, ECO_F32, 0, 1, rows, 0, 0, cols, 1.0};
-  const Rows R = rows_of(L, tokens, mask, cu_seqlens, 2 * pairs);
+              ECO_ERR_ARG, "eco_preference: bad beta, smoothing or denominator");
+  if (grad && R.rows > 0)
+    if (int rc = check_grad(*logits, grad, "eco_preference")) return rc;
   const Pairs P{ref_logp, seq_len, pairs, beta, label_smoothing, denom, kind, average != 0};
   cudaStream_t s = eco_stream(stream);
-  pair_kernel<<<(unsigned)pairs, 256, 0, s>>>(R, P, logp64, coef, log_ratio, margin, pair_loss);
-  pair_finish_kernel<<<1, 256, 0, s>>>(pair_loss, pairs, denom, out);
-  return eco_launch_check("eco_preference_pairs");
+  if (R.rows > 0)
+    if (int rc = eco_token_logp(logits, tokens, mask, cu_seqlens, 2 * pairs, nullptr, wide, row_stats, coef, stream))
+      return rc;
+  pair_kernel<<<(unsigned)pairs, 256, 0, s>>>(R, P, wide, coef, log_ratio, margin, wide + R.rows);
+  pair_finish_kernel<<<1, 256, 0, s>>>(wide + R.rows, pairs, denom, loss);
+  if (int rc = eco_launch_check("eco_preference")) return rc;
+  return grad ? eco_token_grad(logits, tokens, row_stats, coef, nullptr, gain, grad, stream) : ECO_OK;
 }

@@ -136,9 +136,9 @@ _SIGS = {
     "eco_token_logp": (c_i32, [_LP, c_p, c_p, c_p, c_i64, c_p, c_p, c_p, c_p, c_p]),
     "eco_token_grad": (c_i32, [_LP, c_p, c_p, c_p, c_p, c_d, _GP, c_p]),
     "eco_policy_grad": (c_i32, [_LP, c_p, c_p, c_p, c_p, c_p, c_d, c_d, c_d, c_d, c_d, c_p, c_p, c_p, _GP, c_p]),
-    "eco_policy_tokens": (c_i32, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_p, c_p, c_d, c_d, c_d, c_d, c_p, c_p, c_p]),
-    "eco_preference_pairs": (c_i32, [c_p, c_p, c_p, c_i64, c_i64, c_p, c_p, c_i64, c_i64, c_i32, c_d, c_d, c_i32,
-                                     c_d, c_p, c_p, c_p, c_p, c_p, c_p]),
+    "eco_policy_forward": (c_i32, [_LP, c_p, c_p, c_p, c_p, c_p, c_d, c_d, c_d, c_d, c_p, c_p, c_p, c_p, c_p, c_p]),
+    "eco_preference": (c_i32, [_LP, c_p, c_p, c_p, c_p, c_i64, c_i64, c_i32, c_d, c_d, c_i32, c_d, c_d, c_p, c_p, c_p,
+                               c_p, c_p, c_p, _GP, c_p]),
     "eco_ckpt_pack": (c_i32, [c_p, c_i32, c_i64, c_i64, c_i64, _SP, c_p]),
     "eco_ckpt_restore": (c_i32, [_SP, c_i32, c_i64, c_i64, c_p, c_i64, c_p]),
     "eco_gated_act": (c_i32, [c_p, c_i64, c_p, c_i64, c_i32, c_i32, c_i64, c_i64, c_p, c_i64, _SP, _SP, c_p]),
@@ -181,8 +181,14 @@ def last_error() -> str:
     return load().eco_last_error().decode(errors="replace")
 
 
+_FNS: dict = {}  # name -> the loaded entry point
+
+
 def call(name: str, *args) -> None:
-    rc = getattr(load(), name)(*args)
+    fn = _FNS.get(name)
+    if fn is None:
+        fn = _FNS[name] = getattr(load(), name)
+    rc = fn(*args)
     if rc != ECO_OK:
         raise RuntimeError(f"{name} failed ({rc}): {last_error()}")
 

@@ -34,30 +34,31 @@ _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
 def _matrix(t: torch.Tensor, name: str) -> torch.Tensor:
     """``t`` as ``[rows, cols]`` with unit column stride (a view where its strides allow one)."""
-    if t.dtype not in _FLOATS or t.dim() < 1:
+    shape = t.shape
+    if t.dtype not in _FLOATS or len(shape) < 1:
         raise AssertionError(f"{name} must be an fp32, bf16 or fp16 tensor of at least one dimension")
-    if t.shape[-1] == 0:
+    if shape[-1] == 0:
         raise AssertionError(f"{name} has empty rows")
-    m = t.reshape(-1, t.shape[-1])
-    return m if (m.stride(1) == 1 or m.shape[1] == 1) and m.stride(0) < 1 << 31 else m.contiguous()
+    m = t if len(shape) == 2 else t.reshape(-1, shape[-1])
+    ld, unit = m.stride()
+    return m if (unit == 1 or m.shape[1] == 1) and ld < 1 << 31 else m.contiguous()
 
 
-def _empty_rows(rows: int, cols: int, dtype, dev) -> torch.Tensor:
+def _empty_rows(like: torch.Tensor, rows: int, cols: int, dtype=None) -> torch.Tensor:
     """``[rows, cols]`` whose rows start on a multiple of eight elements."""
     if cols % 8 == 0:
-        return torch.empty((rows, cols), dtype=dtype, device=dev)
-    return torch.empty((rows, (cols + 7) // 8 * 8), dtype=dtype, device=dev)[:, :cols]
+        return like.new_empty((rows, cols), dtype=dtype)
+    return like.new_empty((rows, (cols + 7) // 8 * 8), dtype=dtype)[:, :cols]
 
 
-class _Eight:
+def _shaped(m: torch.Tensor, shape) -> torch.Tensor:
+    return m if m.shape == shape else m.view(shape)
+
+
+def _eight(like: torch.Tensor, rows: int, cols: int):
     """int8 rows and fp32 block scales of a ``[rows, cols]`` matrix."""
-
-    __slots__ = ("q", "scale", "spec")
-
-    def __init__(self, rows, cols, dev):
-        self.q = torch.empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8, device=dev)
-        self.scale = torch.empty((rows, (cols + BLOCK - 1) // BLOCK), dtype=torch.float32, device=dev)
-        self.spec = _spec(self.q, self.scale)
+    return (like.new_empty((rows, (cols + 15) // 16 * 16), dtype=torch.int8),
+            like.new_empty((rows, (cols + BLOCK - 1) // BLOCK), dtype=torch.float32))
 
 
 def _spec(q, scale):
@@ -83,10 +84,10 @@ def checkpoint_i8(x: torch.Tensor) -> Checkpoint8:
     m = _matrix(x, "x")
     rows, cols = m.shape
     with nat.on_device(dev):
-        e = _Eight(rows, cols, dev)
-        nat.call("eco_ckpt_pack", m.data_ptr(), nat.TYPES[m.dtype], rows, cols, m.stride(0), ctypes.byref(e.spec),
-                 nat.stream())
-    return Checkpoint8(e.q, e.scale, x.shape, x.dtype)
+        q, scale = _eight(m, rows, cols)
+        nat.call("eco_ckpt_pack", m.data_ptr(), nat.TYPES[m.dtype], rows, cols, m.stride(0),
+                 ctypes.byref(_spec(q, scale)), nat.stream())
+    return Checkpoint8(q, scale, x.shape, x.dtype)
 
 
 def restore_i8(c: Checkpoint8, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -97,10 +98,10 @@ def restore_i8(c: Checkpoint8, dtype: torch.dtype | None = None) -> torch.Tensor
     dev = nat.require_cuda(c.q, c.scale)
     rows, cols = c.q.shape[0], c.shape[-1]
     with nat.on_device(dev):
-        x = _empty_rows(rows, cols, dtype, dev)
+        x = _empty_rows(c.q, rows, cols, dtype)
         nat.call("eco_ckpt_restore", ctypes.byref(_spec(c.q, c.scale)), nat.TYPES[dtype], rows, cols, x.data_ptr(),
                  x.stride(0), nat.stream())
-    return x.view(c.shape)
+    return _shaped(x, c.shape)
 
 
 def _is_weight(t: torch.Tensor) -> bool:
@@ -145,38 +146,41 @@ class _RMSNorm(torch.autograd.Function):
         if not (eps >= 0.0 and math.isfinite(eps)):
             raise ValueError("eps must not be negative")
         wants = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        kind, w_kind = nat.TYPES[m.dtype], 0 if weight is None else nat.TYPES[weight.dtype]
+        q = scale = rstd = saved = None
         with nat.on_device(dev):
-            y = _empty_rows(rows, cols, x.dtype, dev)
-            e = _Eight(rows, cols, dev) if wants else None
-            rstd = torch.empty(rows, dtype=torch.float32, device=dev) if wants else None
-            nat.call("eco_rms_norm", m.data_ptr(), m.stride(0), nat.TYPES[m.dtype], rows, cols, nat.ptr(weight),
-                     0 if weight is None else nat.TYPES[weight.dtype], eps, y.data_ptr(), y.stride(0),
-                     ctypes.byref(e.spec) if wants else None, nat.ptr(rstd), nat.stream())
+            y = _empty_rows(m, rows, cols)
+            if wants:
+                q, scale = _eight(m, rows, cols)
+                rstd = m.new_empty(rows, dtype=torch.float32)
+                saved = ctypes.byref(_spec(q, scale))
+            nat.call("eco_rms_norm", m.data_ptr(), m.stride(0), kind, rows, cols, nat.ptr(weight), w_kind, eps,
+                     y.data_ptr(), y.stride(0), saved, nat.ptr(rstd), nat.stream())
         if wants:
             # q and the weight are open to saved-tensor hooks; scales and roots stay as they are
-            ctx.save_for_backward(e.q, weight)
-            ctx.own = (e.scale, rstd, x.shape)
-        return y.view(x.shape)
+            ctx.save_for_backward(q, weight)
+            ctx.own = (scale, rstd, x.shape, kind, w_kind)
+        return _shaped(y, x.shape)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         q, weight = ctx.saved_tensors
-        scale, rstd, shape = ctx.own
+        scale, rstd, shape, kind, w_kind = ctx.own
         m = _matrix(dy, "dy")
         rows, cols = m.shape
         with nat.on_device(m.device):
-            dx = _empty_rows(rows, cols, m.dtype, m.device)
+            dx = _empty_rows(m, rows, cols)
             dw = scratch = None
+            room = 0
             if weight is not None and ctx.needs_input_grad[1]:
                 dw = torch.empty_like(weight)
-                scratch = torch.empty(nat.load().eco_rms_norm_bwd_scratch(rows, cols), dtype=torch.float32,
-                                      device=m.device)
-            nat.call("eco_rms_norm_bwd", m.data_ptr(), m.stride(0), nat.TYPES[m.dtype], rows, cols, nat.ptr(weight),
-                     0 if weight is None else nat.TYPES[weight.dtype], ctypes.byref(_spec(q, scale)),
-                     rstd.data_ptr(), dx.data_ptr(), dx.stride(0), nat.ptr(dw), nat.ptr(scratch),
-                     0 if scratch is None else scratch.numel(), nat.stream())
-        return dx.view(shape), dw, None
+                room = nat.load().eco_rms_norm_bwd_scratch(rows, cols)
+                scratch = m.new_empty(room, dtype=torch.float32)
+            nat.call("eco_rms_norm_bwd", m.data_ptr(), m.stride(0), kind, rows, cols, nat.ptr(weight), w_kind,
+                     ctypes.byref(_spec(q, scale)), rstd.data_ptr(), dx.data_ptr(), dx.stride(0), nat.ptr(dw),
+                     nat.ptr(scratch), room, nat.stream())
+        return _shaped(dx, shape), dw, None
 
 
 def rms_norm_i8(x: torch.Tensor, weight: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
@@ -215,23 +219,27 @@ class _GatedAct(torch.autograd.Function):
         if up is None:
             if g.shape[1] % 2:
                 raise AssertionError("without up, gate holds both halves: an even number of columns")
-            u, cols = g[:, g.shape[1] // 2:], g.shape[1] // 2
+            cols = g.shape[1] // 2
+            up_at, up_ld = g.data_ptr() + cols * g.element_size(), g.stride(0)
         else:
             if up.shape != gate.shape or up.dtype != gate.dtype:
                 raise AssertionError("gate and up must have one shape and type")
             u, cols = _matrix(up, "up"), g.shape[1]
+            up_at, up_ld = u.data_ptr(), u.stride(0)
         rows, kind = g.shape[0], nat.TYPES[g.dtype]
         wants = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
         with nat.on_device(dev):
-            y = _empty_rows(rows, cols, g.dtype, dev)
-            eg, eu = (_Eight(rows, cols, dev), _Eight(rows, cols, dev)) if wants else (None, None)
-            nat.call("eco_gated_act", g.data_ptr(), g.stride(0), u.data_ptr(), u.stride(0), kind, _ACTS[act], rows,
-                     cols, y.data_ptr(), y.stride(0), ctypes.byref(eg.spec) if wants else None,
-                     ctypes.byref(eu.spec) if wants else None, nat.stream())
+            y = _empty_rows(g, rows, cols)
+            eg = eu = (None, None)
+            if wants:
+                eg, eu = _eight(g, rows, cols), _eight(g, rows, cols)
+            nat.call("eco_gated_act", g.data_ptr(), g.stride(0), up_at, up_ld, kind, _ACTS[act], rows, cols,
+                     y.data_ptr(), y.stride(0), ctypes.byref(_spec(*eg)) if wants else None,
+                     ctypes.byref(_spec(*eu)) if wants else None, nat.stream())
         if wants:
-            ctx.save_for_backward(eg.q, eu.q)
-            ctx.own = (eg.scale, eu.scale, act, up is None, gate.shape)
-        return y.view(*gate.shape[:-1], cols)
+            ctx.save_for_backward(eg[0], eu[0])
+            ctx.own = (eg[1], eu[1], act, up is None, gate.shape)
+        return _shaped(y, (*gate.shape[:-1], cols))
 
     @staticmethod
     @torch.autograd.function.once_differentiable
@@ -242,14 +250,15 @@ class _GatedAct(torch.autograd.Function):
         rows, cols = m.shape
         with nat.on_device(m.device):
             if packed:
-                dg = _empty_rows(rows, 2 * cols, m.dtype, m.device)
-                du = dg[:, cols:]
+                dg, du = _empty_rows(m, rows, 2 * cols), None
+                du_at, du_ld = dg.data_ptr() + cols * dg.element_size(), dg.stride(0)
             else:
-                dg, du = (_empty_rows(rows, cols, m.dtype, m.device) for _ in range(2))
+                dg, du = _empty_rows(m, rows, cols), _empty_rows(m, rows, cols)
+                du_at, du_ld = du.data_ptr(), du.stride(0)
             nat.call("eco_gated_act_bwd", m.data_ptr(), m.stride(0), nat.TYPES[m.dtype], _ACTS[act], rows, cols,
                      ctypes.byref(_spec(gq, gs)), ctypes.byref(_spec(uq, us)), dg.data_ptr(), dg.stride(0),
-                     du.data_ptr(), du.stride(0), nat.stream())
-        return dg.view(shape), None if packed else du.view(shape), None
+                     du_at, du_ld, nat.stream())
+        return _shaped(dg, shape), None if packed else _shaped(du, shape), None
 
 
 def gated_act_i8(gate: torch.Tensor, up: torch.Tensor | None = None, act: str = "silu") -> torch.Tensor:

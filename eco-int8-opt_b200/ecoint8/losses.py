@@ -71,26 +71,25 @@ class _Rows:
 
     def __init__(self, logits, tokens, mask, temperature, s_out):
         self.dev = nat.require_cuda(logits, tokens, mask)
-        if logits.dtype not in nat.TYPES or logits.dim() not in (2, 3):
+        dtype, shape = logits.dtype, logits.shape
+        if dtype not in nat.TYPES or len(shape) not in (2, 3):
             raise AssertionError("logits must be fp32, bf16, fp16 or int8, [rows, vocab] or [batch, length, vocab]")
-        self.lead = lead = logits.shape[:-1]
+        self.lead = lead = shape[:-1]
         if tokens.dtype != torch.int64 or tokens.shape != lead:
             raise AssertionError(f"tokens must be int64 {list(lead)}, one per row of logits")
         if mask is not None and (mask.dtype not in (torch.bool, torch.uint8) or mask.shape != lead):
             raise AssertionError(f"mask must be bool {list(lead)}")
-        if logits.shape[-1] == 0:
+        if shape[-1] == 0:
             raise AssertionError("an empty vocabulary")
         temperature = float(temperature)
         if not (temperature > 0.0 and math.isfinite(temperature)):
             raise ValueError("temperature must be positive")
-        i8 = logits.dtype == torch.int8
-        if i8 != (s_out is not None):
+        if (dtype is torch.int8) != (s_out is not None):
             raise ValueError("int8 logits need their scale s_out, and only they have one")
-        scale = float(s_out) if i8 else 1.0
+        scale = 1.0 if s_out is None else float(s_out)
         if not (scale > 0.0 and math.isfinite(scale)):
             raise ValueError("s_out must be positive")
-        x = logits if logits.stride(-1) == 1 or logits.shape[-1] == 1 else logits.contiguous()
-        self.x = x
+        self.x = x = logits if logits.stride(-1) == 1 or shape[-1] == 1 else logits.contiguous()
         self.gain = 1.0 / temperature
         self.rows = tokens.numel()
         self.spec = _spec(x, scale / temperature)
@@ -101,8 +100,9 @@ class _Rows:
         """A per-token fp32 tensor in the rows' order (broadcast to the tokens' shape)."""
         if t is None:
             return None
-        nat.require_cuda(self.x, t)
-        if t.dtype != torch.float32:
+        if t.device != self.dev:
+            nat.require_cuda(self.x, t)
+        if t.dtype is not torch.float32:
             raise AssertionError(f"{name} must be fp32")
         if t.shape != self.lead:
             try:
@@ -121,40 +121,44 @@ class _Rows:
         s1 = cols + (want1 - cols) % per
         s0 = n1 * s1 + (want0 - n1 * s1) % per if n0 > 1 else n1 * s1
         if skew == 0 and s1 == cols and s0 == n1 * s1:
-            g = torch.empty(x.shape, dtype=dtype, device=x.device)
+            g = x.new_empty(x.shape, dtype=dtype)
         else:
             shape, strides = ((n1, cols), (s1, 1)) if x.dim() == 2 else ((n0, n1, cols), (s0, s1, 1))
-            g = torch.empty(skew + n0 * s0, dtype=dtype, device=x.device).as_strided(shape, strides, skew)
+            g = x.new_empty(skew + n0 * s0, dtype=dtype).as_strided(shape, strides, skew)
         return g, nat.Grad(g.data_ptr(), s0, s1)
 
-    def token_logp(self, logp=None, lp64=None, stats=None, coef=None, cu=None):
-        nat.call("eco_token_logp", ctypes.byref(self.spec), self.tokens.data_ptr(), nat.ptr(self.mask), nat.ptr(cu),
-                 0 if cu is None else cu.numel() - 1, nat.ptr(logp), nat.ptr(lp64), nat.ptr(stats), nat.ptr(coef),
-                 nat.stream())
-
-    def token_grad(self, stats, coef, scale=None):
+    def token_grad(self, stats: int, coef: int, scale=None):
+        """The gradient from row statistics and coefficients (device addresses)."""
         with nat.on_device(self.dev):
             g, spec = self.new_grad()
-            nat.call("eco_token_grad", ctypes.byref(self.spec), self.tokens.data_ptr(), stats.data_ptr(),
-                     coef.data_ptr(), nat.ptr(scale), self.gain, ctypes.byref(spec), nat.stream())
+            nat.call("eco_token_grad", ctypes.byref(self.spec), self.tokens.data_ptr(), stats, coef, nat.ptr(scale),
+                     self.gain, ctypes.byref(spec), nat.stream())
         return g
 
+    def workspace(self, pairs: int = 0):
+        """``(buffer, fp64 log-probabilities and pairs, row statistics, coefficients)``: one allocation
+        and the addresses of its three parts (statistics are two fp32 numbers per row)."""
+        n = self.rows
+        buf = self.tokens.new_empty(2 * n + pairs + (n + 1) // 2, dtype=torch.float64)
+        at = buf.data_ptr()
+        return buf, at, at + 8 * (n + pairs), at + 8 * (2 * n + pairs)
+
     def new(self, *shape, dtype=torch.float32):
-        return torch.empty(shape, dtype=dtype, device=self.dev)
+        return self.tokens.new_empty(shape, dtype=dtype)
 
 
-def _keep_rows(ctx, rows, stats, coef=None):
+def _keep_rows(ctx, rows, buf, stats, coef=None):
     # The logits and tokens go through autograd's saved tensors (checked for changes in place,
     # and open to hooks that move or pack them); the row statistics and coefficients are the
-    # kernels' own and stay as they are.
+    # kernels' own and stay where they are.
     ctx.save_for_backward(rows.x, rows.tokens)
-    ctx.own = (rows.gain, rows.spec.mul, stats, coef)
+    ctx.own = (rows.gain, rows.spec.mul, buf, stats, coef)
 
 
 def _saved_rows(ctx):
-    """``(rows, stats, coef)``: the forward's rows over the tensors that autograd hands back."""
+    """``(rows, statistics, coefficients)``: the forward's rows over the tensors that autograd hands back."""
     x, tokens = ctx.saved_tensors
-    gain, mul, stats, coef = ctx.own
+    gain, mul, _, stats, coef = ctx.own
     rows = _Rows.__new__(_Rows)
     rows.x = x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
     rows.tokens, rows.mask, rows.gain, rows.dev = tokens.contiguous(), None, gain, x.device
@@ -173,16 +177,18 @@ class _TokenLogprobs(torch.autograd.Function):
         with nat.on_device(rows.dev):
             logp = rows.new(*rows.lead)
             stats = rows.new(rows.rows, 2) if ctx.needs_input_grad[0] else None
-            rows.token_logp(logp=logp, stats=stats)
+            nat.call("eco_token_logp", ctypes.byref(rows.spec), rows.tokens.data_ptr(), nat.ptr(rows.mask), None, 0,
+                     logp.data_ptr(), None, nat.ptr(stats), None, nat.stream())
         if stats is not None:
-            _keep_rows(ctx, rows, stats)
+            _keep_rows(ctx, rows, stats, stats.data_ptr())
         return logp
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dlogp):
         rows, stats, _ = _saved_rows(ctx)
-        return rows.token_grad(stats, dlogp.contiguous()), None, None, None, None
+        dlogp = dlogp.contiguous()
+        return rows.token_grad(stats, dlogp.data_ptr()), None, None, None, None
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, mask: torch.Tensor | None = None,
@@ -245,12 +251,11 @@ class _PolicyLoss(torch.autograd.Function):
         rows = _Rows(logits, tokens, mask, temperature, s_out)
         keep, args = _policy_args(rows, old_logp, advantages, ref_logp, *how)
         with nat.on_device(rows.dev):
-            logp, out, coef = rows.new(*rows.lead), rows.new(3), rows.new(rows.rows)
-            lp64, stats = rows.new(rows.rows, dtype=torch.float64), rows.new(rows.rows, 2)
-            rows.token_logp(logp=logp, lp64=lp64, stats=stats)
-            nat.call("eco_policy_tokens", lp64.data_ptr(), rows.tokens.data_ptr(), nat.ptr(rows.mask), rows.rows,
-                     rows.x.shape[-1], *args, coef.data_ptr(), out.data_ptr(), nat.stream())
-        _keep_rows(ctx, rows, stats, coef)
+            logp, out = rows.new(*rows.lead), rows.new(3)
+            buf, lp64, stats, coef = rows.workspace()
+            nat.call("eco_policy_forward", ctypes.byref(rows.spec), rows.tokens.data_ptr(), nat.ptr(rows.mask), *args,
+                     logp.data_ptr(), lp64, stats, coef, out.data_ptr(), nat.stream())
+        _keep_rows(ctx, rows, buf, stats, coef)
         loss, kl, clipped = out.unbind()
         ctx.mark_non_differentiable(logp, kl, clipped)
         ctx.set_materialize_grads(False)
@@ -279,7 +284,8 @@ def policy_loss(logits: torch.Tensor, tokens: torch.Tensor, old_logp: torch.Tens
 # ------------------------------------------------------------------ preference loss
 
 
-def _preference_forward(rows, ref_logp, beta, kind, label_smoothing, average, cu_seqlens, denom):
+def _preference(rows, with_grad, ref_logp, beta, kind, label_smoothing, average, cu_seqlens, denom):
+    """``(workspace, its parts, loss, log ratios, margins, gradient or None)`` in one call."""
     ref = rows.per_row(ref_logp, "ref_logp")
     if ref is None:
         raise AssertionError("ref_logp must be given")
@@ -304,17 +310,17 @@ def _preference_forward(rows, ref_logp, beta, kind, label_smoothing, average, cu
     denom = float(pairs) if denom is None else float(denom)
     if not (denom > 0.0 and math.isfinite(denom)):
         raise ValueError("denom must be positive")
-    n = rows.rows
-    wide = rows.new(n + pairs, dtype=torch.float64)  # log-probabilities, then each pair's loss
-    lp64, pair_loss = wide[:n], wide[n:]
-    stats, coef, out = rows.new(n, 2), rows.new(n), rows.new(3 * pairs + 1)
-    log_ratio, margin, loss = out[:2 * pairs], out[2 * pairs:3 * pairs], out[3 * pairs]
-    rows.token_logp(lp64=lp64, stats=stats, coef=coef, cu=cu_seqlens)
-    nat.call("eco_preference_pairs", lp64.data_ptr(), rows.tokens.data_ptr(), nat.ptr(rows.mask), n,
-             rows.x.shape[-1], ref.data_ptr(), nat.ptr(cu_seqlens), seq_len, pairs, _KINDS[kind], beta,
-             label_smoothing, int(bool(average)), denom, coef.data_ptr(), log_ratio.data_ptr(), margin.data_ptr(),
-             pair_loss.data_ptr(), loss.data_ptr(), nat.stream())
-    return stats, coef, loss, log_ratio, margin
+    with nat.on_device(rows.dev):
+        buf, wide, stats, coef = rows.workspace(pairs)
+        g, spec = rows.new_grad() if with_grad else (None, None)
+        out = rows.new(3 * pairs + 1)
+        at = out.data_ptr()
+        nat.call("eco_preference", ctypes.byref(rows.spec), rows.tokens.data_ptr(), nat.ptr(rows.mask), ref.data_ptr(),
+                 nat.ptr(cu_seqlens), seq_len, pairs, _KINDS[kind], beta, label_smoothing, int(bool(average)), denom,
+                 rows.gain, wide, stats, coef, at, at + 8 * pairs, at + 12 * pairs,
+                 ctypes.byref(spec) if with_grad else None, nat.stream())
+    log_ratio, margin, loss = out.split_with_sizes((2 * pairs, pairs, 1))
+    return (buf, stats, coef), loss.view(()), log_ratio, margin, g
 
 
 def preference_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: torch.Tensor, *, beta: float = 0.1,
@@ -340,19 +346,17 @@ def preference_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: t
     pairs by ``denom``, by default their number.  A sequence's gradient needs all its rows, so
     the logits are read twice."""
     rows = _Rows(logits, tokens, mask, temperature, s_out)
-    with nat.on_device(rows.dev):
-        stats, coef, loss, log_ratio, margin = _preference_forward(rows, ref_logp, beta, kind, label_smoothing,
-                                                                   average, cu_seqlens, denom)
-        return PreferenceLoss(loss, rows.token_grad(stats, coef), log_ratio, margin)
+    _, loss, log_ratio, margin, g = _preference(rows, True, ref_logp, beta, kind, label_smoothing, average, cu_seqlens,
+                                                denom)
+    return PreferenceLoss(loss, g, log_ratio, margin)
 
 
 class _PreferenceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, mask, temperature, s_out, *how):
         rows = _Rows(logits, tokens, mask, temperature, s_out)
-        with nat.on_device(rows.dev):
-            stats, coef, loss, log_ratio, margin = _preference_forward(rows, *how)
-        _keep_rows(ctx, rows, stats, coef)
+        work, loss, log_ratio, margin, _ = _preference(rows, False, *how)
+        _keep_rows(ctx, rows, *work)
         ctx.mark_non_differentiable(log_ratio, margin)
         ctx.set_materialize_grads(False)
         return loss, log_ratio, margin

@@ -485,29 +485,31 @@ ECO_API int eco_token_grad(const eco_logits_t* logits, const int64_t* tokens, co
  *   k = exp(ref - lp) - (ref - lp) - 1  (0 without ref_logp)
  * out[0..2] = sum l / denom, sum k / denom, share of rows whose clipped term is the larger.
  * eco_policy_grad does all of it from the logits: logp [rows], terms float [3 rows + 64]
- * (workspace), the gradient times gain.  eco_policy_tokens starts from fp64
- * log-probabilities and leaves each row's d loss / d lp in coef (for eco_token_grad). */
+ * (workspace), the gradient times gain.  eco_policy_forward leaves what a later eco_token_grad
+ * needs: row_stats [rows, 2] and each row's d loss / d lp in coef [rows]; logp64 [rows] is
+ * workspace. */
 ECO_API int eco_policy_grad(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
                             const float* old_logp, const float* adv, const float* ref_logp, double low,
                             double high, double kl_coef, double denom, double gain, float* logp, float* terms,
                             float* out, const eco_grad_t* grad, eco_stream_t stream);
-ECO_API int eco_policy_tokens(const double* logp64, const int64_t* tokens, const uint8_t* mask, int64_t rows,
-                              int64_t cols, const float* old_logp, const float* adv, const float* ref_logp,
-                              double low, double high, double kl_coef, double denom, float* coef, float* out,
-                              eco_stream_t stream);
+ECO_API int eco_policy_forward(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
+                               const float* old_logp, const float* adv, const float* ref_logp, double low,
+                               double high, double kl_coef, double denom, float* logp, double* logp64,
+                               float* row_stats, float* coef, float* out, eco_stream_t stream);
 
 /* Preference loss over `pairs` pairs of sequences, the preferred ones first: sequence q has
  * rows [q seq_len, (q + 1) seq_len), or [cu_seqlens[q], cu_seqlens[q + 1]) where cu_seqlens
  * (int32 [2 pairs + 1]) is given.  D_q = sum over its counting rows of lp - ref (average: over
  * their number); h = beta (D_p - D_{p + pairs}).  sigmoid: -(1 - e) log s(h) - e log s(-h);
- * hinge: max(0, 1 - h); ipo: (h / beta - 1 / (2 beta))^2; out[0] = their sum / denom.
- * log_ratio [2 pairs] = D, margin [pairs] = h, pair_loss [pairs] (workspace); coef: each
- * counting row's d loss / d lp (other rows are left as they are). */
-ECO_API int eco_preference_pairs(const double* logp64, const int64_t* tokens, const uint8_t* mask, int64_t rows,
-                                 int64_t cols, const float* ref_logp, const int32_t* cu_seqlens, int64_t seq_len,
-                                 int64_t pairs, int kind, double beta, double label_smoothing, int average,
-                                 double denom, float* coef, float* log_ratio, float* margin, double* pair_loss,
-                                 float* out, eco_stream_t stream);
+ * hinge: max(0, 1 - h); ipo: (h / beta - 1 / (2 beta))^2.
+ * log_ratio [2 pairs] = D, margin [pairs] = h, loss: the losses' sum / denom.  row_stats [rows, 2]
+ * and coef [rows] (each row's d loss / d lp) are what eco_token_grad needs; with grad (nullable)
+ * it is launched too, times gain.  wide [rows + pairs] is workspace. */
+ECO_API int eco_preference(const eco_logits_t* logits, const int64_t* tokens, const uint8_t* mask,
+                           const float* ref_logp, const int32_t* cu_seqlens, int64_t seq_len, int64_t pairs,
+                           int kind, double beta, double label_smoothing, int average, double denom,
+                           double gain, double* wide, float* row_stats, float* coef, float* log_ratio,
+                           float* margin, float* loss, const eco_grad_t* grad, eco_stream_t stream);
 
 /* ---------------------------------------- activations kept in eight bits ----------
  * A row is kept in blocks of ECO_CKPT_BLOCK columns: scale = amax / 127, q = rint(x * (127 /

@@ -143,14 +143,17 @@ def test_token_objectives_refuse_bad_arguments():
     _refused(policy(1.2, 0.8, 0.0), -1, "clip range")
     _refused(policy(0.8, 1.2, math.inf), -1, "clip range")
     _refused(policy(0.8, 1.2, 0.0, old=None), -1, "null")
-    _refused(lib.eco_policy_tokens(None, 8192, None, 4, 64, 8192, 8192, None, 0.8, 1.2, 0.0, 0.0, 8192, 8192, None), -1,
-             "null")
-    pairs = lambda **h: lib.eco_preference_pairs(  # noqa: E731
-        8192, 8192, None, h.get("rows", 8), 64, 8192, None, h.get("s", 4), h.get("pairs", 1), h.get("kind", 0),
-        h.get("beta", 0.1), h.get("smooth", 0.0), 0, h.get("denom", 1.0), 8192, 8192, 8192, 8192, 8192, None)
+    _refused(lib.eco_policy_forward(_logits_spec(), 8192, None, 8192, 8192, None, 0.8, 1.2, 0.0, 0.0, None, None, 8192,
+                                    8192, 8192, None), -1, "null")
+    pairs = lambda **h: lib.eco_preference(  # noqa: E731
+        _logits_spec(n1=8), 8192, None, h.get("ref", 8192), None, h.get("s", 4), h.get("pairs", 1), h.get("kind", 0),
+        h.get("beta", 0.1), h.get("smooth", 0.0), 0, h.get("denom", 1.0), 1.0, 8192, 8192, 8192, 8192, 8192, 8192,
+        h.get("grad"), None)
     _refused(pairs(s=5), -1, "more sequences")
     _refused(pairs(pairs=0), -1, "bad arguments")
+    _refused(pairs(ref=None), -1, "bad arguments")
     _refused(pairs(kind=3), -1, "kind")
+    _refused(pairs(grad=grad(8194, 0, 64)), -2, "modulo 8 elements")
     for h in (dict(beta=0.0), dict(beta=math.nan), dict(smooth=1.5), dict(denom=0.0)):
         _refused(pairs(**h), -1, "beta")
 
