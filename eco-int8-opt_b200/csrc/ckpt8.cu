@@ -183,56 +183,93 @@ struct Saved {  // q [rows, ld_q] int8 (ld_q a multiple of 16), scale [rows, ld_
 
 ECO_DEV int left8(int cols, int c) { return max(0, min(8, cols - c)); }
 
-// Where a half-warp works: blocks of one row side by side, rows below each other.  2^l blocks of
-// a row in a CTA (up to 16) and 16 / 2^l rows.  Loops over (row, block) in groups of U rows,
+// Where a half-warp works: 2^l blocks of a row side by side in a CTA (up to 16), 16 / 2^l rows
+// below each other; a thread keeps its eight columns and walks down the rows in groups of U,
 // whose loads are all issued before the first is used (a thread has one or two 16-byte loads per
-// row: alone they would not cover the memory's latency).  Both halves of a warp stay in step
-// (the shuffles need all 32 lanes): lanes past the last row or column get n = 0 columns, blocks
-// past the last row or block `live` = false.
-// load(r, c, n) -> L;  use(L[U], r[U], n[U], live[U], b, c).
+// row: alone they would not cover the memory's latency).  Both halves of a warp stay in step (the
+// shuffles need all 32 lanes).  Groups of which every row exists are told apart once per group
+// (`full`), for the CTA as a whole.
+//   load(r) -> L for a row that exists;   use(full, L[U], first row, step)
+// Lanes whose n is 0 have no columns; blocks with `live` false lie past the last.
+struct Place {
+  int lane, c, n, b, row, per;
+  bool live;
+  ECO_DEV Place(int cols, int l) {
+    const int half = threadIdx.x / kLanes;
+    lane = threadIdx.x & (kLanes - 1);
+    b = ((int)blockIdx.x << l) + (half & ((1 << l) - 1));
+    c = b * kBlock + lane * 8;
+    live = b * kBlock < cols;
+    n = left8(cols, c);
+    row = half >> l;
+    per = kHalves >> l;
+  }
+};
 template <int U, typename L, typename Load, typename Use>
-ECO_DEV void for_blocks(int rows, int cols, int l, Load load, Use use) {
-  const int half = threadIdx.x / kLanes, lane = threadIdx.x & (kLanes - 1);
-  const int blocks = (cols + kBlock - 1) / kBlock, per = kHalves >> l;
-  const int row_step = (int)gridDim.y * per, b_step = (int)gridDim.x << l;
-  for (int64_t rr = (int64_t)blockIdx.y * per; rr < rows; rr += (int64_t)U * row_step)
-    for (int bb = (int)blockIdx.x << l; bb < blocks; bb += b_step) {
-      const int b = bb + (half & ((1 << l) - 1)), c = b * kBlock + lane * 8;
-      const int64_t r0 = rr + (half >> l);
-      L in[U];
-      int64_t r[U];
-      int n[U];
-      bool live[U];
-      const int most = b < blocks ? left8(cols, c) : 0;
+ECO_DEV void for_rows(int rows, const Place& at, Load load, Use use) {
+  const int step = (int)gridDim.y * at.per;
+  for (int rr = (int)blockIdx.y * at.per; rr < rows; rr += U * step) {
+    const int r = rr + at.row;
+    L in[U];
+    if (rr + (U - 1) * step + at.per <= rows) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) in[u] = load(r + u * step);
+      use(std::true_type{}, in, r, step);
+    } else {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        r[u] = r0 + (int64_t)u * row_step;
-        live[u] = r[u] < rows && b < blocks;
-        n[u] = live[u] ? most : 0;
-        if (!live[u]) r[u] = 0;
-        in[u] = load(r[u], c, n[u]);
+        in[u] = L{};
+        if (r + u * step < rows) in[u] = load(r + u * step);
       }
-      use(in, r, n, live, b, c);
+      use(std::false_type{}, in, r, step);
     }
+  }
+}
+// Eight columns of a row: WHOLE rows consist of whole groups that start on a boundary of their size.
+template <typename T, bool WHOLE>
+ECO_DEV Oct<T> load_cols(const Mat& x, int r, const Place& at) {
+  const T* row = static_cast<const T*>(x.p) + (int64_t)r * x.ld;
+  if constexpr (!WHOLE) return load8(row, at.c, at.n);
+  Oct<T> o{};
+  if (at.n > 0) {
+    if constexpr (sizeof(T) == 4) {
+      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                   : "=r"(o.w[0]), "=r"(o.w[1]), "=r"(o.w[2]), "=r"(o.w[3]), "=r"(o.w[4]), "=r"(o.w[5]), "=r"(o.w[6]),
+                     "=r"(o.w[7])
+                   : "l"(row + at.c));
+    } else {
+      const uint4 t = __ldg(reinterpret_cast<const uint4*>(row + at.c));
+      o.w[0] = t.x, o.w[1] = t.y, o.w[2] = t.z, o.w[3] = t.w;
+    }
+  }
+  return o;
+}
+// Puts the eight columns of N numbers (rows, or gate and up of them) away: their maxima, the
+// gains of all N blocks at once, the bytes; lane i keeps block i's scale.
+template <typename T>
+ECO_DEV void put_bytes(const Oct<T>& o, float gain, int8_t* q) {
+  float f[8];
+  unpack8(o, f);
+  __stcg(reinterpret_cast<uint2*>(q), quant8(f, gain));
 }
 
 // ------------------------------------------------ put away, bring back
-template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) pack_kernel(Mat x, int rows, int cols, Saved S, int bpr_log2) {
-  for_blocks<U, Oct<T>>(
-      rows, cols, bpr_log2,
-      [&](int64_t r, int c, int n) { return load8(static_cast<const T*>(x.p) + r * x.ld, c, n); },
-      [&](const Oct<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
-        float f[8], amax[U], gain[U];
+template <typename T, int U, bool WHOLE>
+__global__ void __launch_bounds__(kThreads) pack_kernel(Mat x, int rows, int cols, Saved S, int l) {
+  const Place at(cols, l);
+  for_rows<U, Oct<T>>(
+      rows, at, [&](int r) { return load_cols<T, WHOLE>(x, r, at); },
+      [&](auto full, const Oct<T>(&o)[U], int r0, int step) {
+        float amax[U], gain[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) amax[u] = block_amax(o[u]);
         const float scale = block_gains(amax, gain);
-        const int lane = threadIdx.x & (kLanes - 1);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          unpack8(o[u], f);
-          if (n[u] > 0) __stcg(reinterpret_cast<uint2*>(S.q + r[u] * S.ld_q + c), quant8(f, gain[u]));
-          if (lane == u && live[u]) S.scale[r[u] * S.ld_s + b] = scale;
+          const int r = r0 + u * step;
+          if (!full && r >= rows) break;
+          if (at.n > 0) put_bytes(o[u], gain[u], S.q + (int64_t)r * S.ld_q + at.c);
+          if (at.lane == u && at.live) S.scale[(int64_t)r * S.ld_s + at.b] = scale;
         }
       });
 }
@@ -256,15 +293,18 @@ ECO_DEV void values8(const Eights& e, float (&f)[8]) {
 }
 
 template <typename T, int U>
-__global__ void __launch_bounds__(kThreads) restore_kernel(Saved S, int rows, int cols, Mat x, int bpr_log2) {
-  for_blocks<U, Eights>(
-      rows, cols, bpr_log2, [&](int64_t r, int c, int n) { return fetch8(S, r, c, n); },
-      [&](const Eights(&e)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
+__global__ void __launch_bounds__(kThreads) restore_kernel(Saved S, int rows, int cols, Mat x, int l) {
+  const Place at(cols, l);
+  for_rows<U, Eights>(
+      rows, at, [&](int r) { return fetch8(S, r, at.c, at.n); },
+      [&](auto full, const Eights(&e)[U], int r0, int step) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * step;
+          if (at.n == 0 || (!full && r >= rows)) break;
           float f[8];
           values8(e[u], f);
-          if (n[u] > 0) store8(static_cast<T*>(x.p) + r[u] * x.ld, c, n[u], true, f);
+          store8(static_cast<T*>(x.p) + (int64_t)r * x.ld, at.c, at.n, true, f);
         }
       });
 }
@@ -307,45 +347,41 @@ struct OctPair {
   Oct<T> a, b;
 };
 
-template <typename T, bool GELU, int U>
+template <typename T, bool GELU, int U, bool WHOLE>
 __global__ void __launch_bounds__(kThreads)
-    gated_fwd_kernel(Mat gate, Mat up, int rows, int cols, Mat y, Saved SG, Saved SU, int bpr_log2) {
-  for_blocks<U, OctPair<T>>(
-      rows, cols, bpr_log2,
-      [&](int64_t r, int c, int n) {
-        return OctPair<T>{load8(static_cast<const T*>(gate.p) + r * gate.ld, c, n),
-                          load8(static_cast<const T*>(up.p) + r * up.ld, c, n)};
-      },
-      [&](const OctPair<T>(&o)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
-        const int lane = threadIdx.x & (kLanes - 1);
+    gated_fwd_kernel(Mat gate, Mat up, int rows, int cols, Mat y, Saved SG, Saved SU, int l) {
+  const Place at(cols, l);
+  for_rows<U, OctPair<T>>(
+      rows, at,
+      [&](int r) { return OctPair<T>{load_cols<T, WHOLE>(gate, r, at), load_cols<T, WHOLE>(up, r, at)}; },
+      [&](auto full, const OctPair<T>(&o)[U], int r0, int step) {
+        float amax[2 * U], gain[2 * U], scale = 0.0f;
         if (SG.q) {
-          float f[8], amax[2 * U], gain[2 * U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             amax[2 * u] = block_amax(o[u].a);
             amax[2 * u + 1] = block_amax(o[u].b);
           }
-          const float scale = block_gains(amax, gain);
-#pragma unroll
-          for (int u = 0; u < U; ++u) {
-            if (n[u] > 0) {
-              unpack8(o[u].a, f);
-              __stcg(reinterpret_cast<uint2*>(SG.q + r[u] * SG.ld_q + c), quant8(f, gain[2 * u]));
-              unpack8(o[u].b, f);
-              __stcg(reinterpret_cast<uint2*>(SU.q + r[u] * SU.ld_q + c), quant8(f, gain[2 * u + 1]));
-            }
-            if (lane == 2 * u && live[u]) SG.scale[r[u] * SG.ld_s + b] = scale;
-            if (lane == 2 * u + 1 && live[u]) SU.scale[r[u] * SU.ld_s + b] = scale;
-          }
+          scale = block_gains(amax, gain);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * step;
+          if (!full && r >= rows) break;
+          if (SG.q) {
+            if (at.n > 0) {
+              put_bytes(o[u].a, gain[2 * u], SG.q + (int64_t)r * SG.ld_q + at.c);
+              put_bytes(o[u].b, gain[2 * u + 1], SU.q + (int64_t)r * SU.ld_q + at.c);
+            }
+            if (at.lane == 2 * u && at.live) SG.scale[(int64_t)r * SG.ld_s + at.b] = scale;
+            if (at.lane == 2 * u + 1 && at.live) SU.scale[(int64_t)r * SU.ld_s + at.b] = scale;
+          }
           float g[8], v[8];
           unpack8(o[u].a, g);
           unpack8(o[u].b, v);
 #pragma unroll
           for (int i = 0; i < 8; ++i) g[i] = g[i] * act_of<GELU>(g[i]).over * v[i];
-          if (n[u] > 0) store8(static_cast<T*>(y.p) + r[u] * y.ld, c, n[u], true, g);
+          if (at.n > 0) store8(static_cast<T*>(y.p) + (int64_t)r * y.ld, at.c, at.n, true, g);
         }
       });
 }
@@ -356,19 +392,21 @@ struct GatedIn {
   Eights g, u;
 };
 
-template <typename T, bool GELU, int U>
+template <typename T, bool GELU, int U, bool WHOLE>
 __global__ void __launch_bounds__(kThreads)
-    gated_bwd_kernel(Mat dy, int rows, int cols, Saved SG, Saved SU, Mat dgate, Mat dup, bool vec_g,
-                     bool vec_u, int bpr_log2) {
-  for_blocks<U, GatedIn<T>>(
-      rows, cols, bpr_log2,
-      [&](int64_t r, int c, int n) {
-        return GatedIn<T>{load8(static_cast<const T*>(dy.p) + r * dy.ld, c, n), fetch8(SG, r, c, n),
-                          fetch8(SU, r, c, n)};
+    gated_bwd_kernel(Mat dy, int rows, int cols, Saved SG, Saved SU, Mat dgate, Mat dup, bool vec_g, bool vec_u,
+                     int l) {
+  const Place at(cols, l);
+  for_rows<U, GatedIn<T>>(
+      rows, at,
+      [&](int r) {
+        return GatedIn<T>{load_cols<T, WHOLE>(dy, r, at), fetch8(SG, r, at.c, at.n), fetch8(SU, r, at.c, at.n)};
       },
-      [&](const GatedIn<T>(&in)[U], const int64_t(&r)[U], const int(&n)[U], const bool(&live)[U], int b, int c) {
+      [&](auto full, const GatedIn<T>(&in)[U], int r0, int step) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+          const int r = r0 + u * step;
+          if (at.n == 0 || (!full && r >= rows)) break;
           float g[8], v[8], d[8];
           values8(in[u].g, g);
           values8(in[u].u, v);
@@ -380,10 +418,8 @@ __global__ void __launch_bounds__(kThreads)
             v[i] = d[i] * g[i] * s.over;
             g[i] = dg;
           }
-          if (n[u] > 0) {
-            store8(static_cast<T*>(dgate.p) + r[u] * dgate.ld, c, n[u], vec_g && n[u] == 8, g);
-            store8(static_cast<T*>(dup.p) + r[u] * dup.ld, c, n[u], vec_u && n[u] == 8, v);
-          }
+          store8(static_cast<T*>(dgate.p) + (int64_t)r * dgate.ld, at.c, at.n, WHOLE || (vec_g && at.n == 8), g);
+          store8(static_cast<T*>(dup.p) + (int64_t)r * dup.ld, at.c, at.n, WHOLE || (vec_u && at.n == 8), v);
         }
       });
 }
@@ -894,13 +930,13 @@ int bpr_log2_of(int64_t cols) {
   while (l < 4 && (1 << l) < blocks) ++l;
   return l;
 }
-// As many CTAs as are resident (eight of 256 threads per SM), each walking down its rows.
-dim3 block_grid(int64_t rows, int64_t cols, int bpr_log2, int unroll) {
-  const int64_t blocks = (cols + kBlock - 1) / kBlock, rpc = (int64_t)(kHalves >> bpr_log2) * unroll;
-  const int64_t gx = std::min<int64_t>((blocks + (1 << bpr_log2) - 1) >> bpr_log2, 65535);
+// A column of CTAs for every 2^l blocks; down the rows, as many as are resident (eight of 256
+// threads per SM), each walking on.
+dim3 block_grid(int64_t rows, int64_t cols, int l, int unroll) {
+  const int64_t blocks = (cols + kBlock - 1) / kBlock, per = (int64_t)(kHalves >> l) * unroll;
+  const int64_t gx = (blocks + (1 << l) - 1) >> l;
   const int64_t most = std::max<int64_t>(1, (int64_t)eco_num_sms() * 8 / gx);
-  const int64_t gy = std::min<int64_t>((rows + rpc - 1) / rpc, std::min<int64_t>(most, 65535));
-  return dim3((unsigned)gx, (unsigned)gy);
+  return dim3((unsigned)gx, (unsigned)std::min<int64_t>((rows + per - 1) / per, std::min<int64_t>(most, 65535)));
 }
 
 int check_saved(const eco_saved_i8_t* S, int64_t rows, int64_t cols, const char* who) {
@@ -921,6 +957,10 @@ bool rows_on_16(const void* p, int64_t ld, int64_t rows, int type) {
 // Eight columns of every row start on a boundary of their size: 32 bytes for fp32, else 16.
 bool rows_on_8(const void* p, int64_t ld, int64_t rows, int type) {
   return reinterpret_cast<uintptr_t>(p) % (uintptr_t)(8 * es_of(type)) == 0 && (rows <= 1 || ld % 8 == 0);
+}
+// Rows of whole groups of eight columns that start on a boundary of their size.
+bool whole8(const void* p, int64_t ld, int64_t rows, int64_t cols, int type) {
+  return rows_on_8(p, ld, rows, type) && cols % 8 == 0;
 }
 int check_in(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const char* who) {
   ECO_REQUIRE(p && (rows <= 1 || (ld >= 0 && ld <= INT32_MAX)) && reinterpret_cast<uintptr_t>(p) % (uintptr_t)es_of(type) == 0, ECO_ERR_ARG,
@@ -995,7 +1035,8 @@ extern "C" int eco_ckpt_pack(const void* x, int type, int64_t rows, int64_t cols
   by_float(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int U = sizeof(T) == 4 ? 2 : 4;
-    pack_kernel<T, U><<<block_grid(rows, cols, l, U), kThreads, 0, eco_stream(stream)>>>(
+    const auto kernel = whole8(x, ld, rows, cols, type) ? pack_kernel<T, U, true> : pack_kernel<T, U, false>;
+    kernel<<<block_grid(rows, cols, l, U), kThreads, 0, eco_stream(stream)>>>(
         mat(x, ld), (int)rows, (int)cols, saved_of(saved), l);
   });
   return eco_launch_check("eco_ckpt_pack");
@@ -1035,13 +1076,12 @@ extern "C" int eco_gated_act(const void* gate, int64_t ld_gate, const void* up, 
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int U = sizeof(T) == 4 ? 1 : 2;
     const dim3 grid = block_grid(rows, cols, l, U);
-    const Mat g = mat(gate, ld_gate), u = mat(up, ld_up), o = mat(y, ld_y);
-    if (act == ECO_ACT_GELU)
-      gated_fwd_kernel<T, true, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, (int)rows, (int)cols, o, saved_of(saved_gate),
-                                                                           saved_of(saved_up), l);
-    else
-      gated_fwd_kernel<T, false, U><<<grid, kThreads, 0, eco_stream(stream)>>>(g, u, (int)rows, (int)cols, o, saved_of(saved_gate),
-                                                                            saved_of(saved_up), l);
+    const bool whole = whole8(gate, ld_gate, rows, cols, type) && whole8(up, ld_up, rows, cols, type);
+    const auto kernel = act == ECO_ACT_GELU
+                            ? (whole ? gated_fwd_kernel<T, true, U, true> : gated_fwd_kernel<T, true, U, false>)
+                            : (whole ? gated_fwd_kernel<T, false, U, true> : gated_fwd_kernel<T, false, U, false>);
+    kernel<<<grid, kThreads, 0, eco_stream(stream)>>>(mat(gate, ld_gate), mat(up, ld_up), (int)rows, (int)cols,
+                                                      mat(y, ld_y), saved_of(saved_gate), saved_of(saved_up), l);
   });
   return eco_launch_check("eco_gated_act");
 }
@@ -1066,13 +1106,13 @@ extern "C" int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int ac
     using T = std::remove_pointer_t<decltype(t)>;
     constexpr int U = sizeof(T) == 4 ? 1 : 2;
     const dim3 grid = block_grid(rows, cols, l, U);
-    const Mat d = mat(dy, ld_dy), g = mat(dgate, ld_dgate), u = mat(dup, ld_dup);
-    if (act == ECO_ACT_GELU)
-      gated_bwd_kernel<T, true, U><<<grid, kThreads, 0, eco_stream(stream)>>>(
-          d, (int)rows, (int)cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
-    else
-      gated_bwd_kernel<T, false, U><<<grid, kThreads, 0, eco_stream(stream)>>>(
-          d, (int)rows, (int)cols, saved_of(saved_gate), saved_of(saved_up), g, u, vg, vu, l);
+    const bool whole = vg && vu && whole8(dy, ld_dy, rows, cols, type);
+    const auto kernel = act == ECO_ACT_GELU
+                            ? (whole ? gated_bwd_kernel<T, true, U, true> : gated_bwd_kernel<T, true, U, false>)
+                            : (whole ? gated_bwd_kernel<T, false, U, true> : gated_bwd_kernel<T, false, U, false>);
+    kernel<<<grid, kThreads, 0, eco_stream(stream)>>>(mat(dy, ld_dy), (int)rows, (int)cols, saved_of(saved_gate),
+                                                      saved_of(saved_up), mat(dgate, ld_dgate), mat(dup, ld_dup), vg, vu,
+                                                      l);
   });
   return eco_launch_check("eco_gated_act_bwd");
 }
