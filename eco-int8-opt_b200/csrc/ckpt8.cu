@@ -692,11 +692,17 @@ __global__ void __launch_bounds__(kRmsThreads, 1)
   int r = (int)blockIdx.x * GROUPS + group;
   const float inv_cols = 1.0f / (float)cols;
   auto n_of = [&](int j) { return WHOLE ? (c + j * NT * G < cols ? G : 0) : left(cols, c + j * NT * G, G); };
-  auto issue = [&](int row, int s, int j) {
+  // What a unit's place holds of row `row`: its dy, read once; its bytes and scale, read in both
+  // passes over the row (registers have no room to keep them).
+  auto issue_dy = [&](int row, int s, int j) {
+    if (WHOLE && row < rows && c + j * NT * G < cols)
+      copy_async<16>(st.data(s, j), static_cast<const T*>(dy.p) + (int64_t)row * dy.ld + c + j * NT * G);
+    copies_commit();
+  };
+  auto issue_bytes = [&](int row, int s, int j) {
     const int at = c + j * NT * G;
     if (WHOLE && row < rows) {
       if (at < cols) {
-        copy_async<16>(st.data(s, j), static_cast<const T*>(dy.p) + (int64_t)row * dy.ld + at);
         copy_async<G>(st.bytes(s, j), S.q + (int64_t)row * S.ld_q + at);
         if (lane == 0) copy_async<4>(st.scale(s, j), S.scale + (int64_t)row * S.ld_s + at / kBlock);
       }
@@ -705,9 +711,12 @@ __global__ void __launch_bounds__(kRmsThreads, 1)
     copies_commit();
   };
 #pragma unroll
-  for (int s = 0; s < R; ++s)
+  for (int s = 0; s < R; ++s) {
 #pragma unroll
-    for (int j = 0; j < U; ++j) issue(r + s * step, s, j);
+    for (int j = 0; j < U; ++j) issue_dy(r + s * step, s, j);
+#pragma unroll
+    for (int j = 0; j < U; ++j) issue_bytes(r + s * step, s, j);
+  }
   if (group == 0) {
 #pragma unroll
     for (int j = 0; j < U; ++j) {
@@ -720,69 +729,78 @@ __global__ void __launch_bounds__(kRmsThreads, 1)
   float acc[U][G] = {};
   int s = 0, par = 0;
   for (; r < rows; r += step) {
-    // u = byte * scale * rstd: the factor, one per unit, goes where it is used once
-    float dot = 0.0f, d[U][G], k[U], rs = 0.0f;
-    uint2 bytes[U];
-    uint4 raw;
-    auto take = [&](int j) {  // unit j's dy, bytes and factor; its place is free again
-      raw = make_uint4(0u, 0u, 0u, 0u);
-      bytes[j] = make_uint2(0u, 0u);
-      k[j] = 0.0f;
+    auto take_dy = [&](int j) {
+      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
       if constexpr (WHOLE) {
-        copies_wait<R * U - 1>();
-        __syncwarp();  // the first lanes' copies too
-        if (n_of(j) > 0) {
-          raw = *st.data(s, j);
-          if constexpr (G == 8) bytes[j] = *reinterpret_cast<const uint2*>(st.bytes(s, j));
-          else bytes[j].x = *reinterpret_cast<const uint32_t*>(st.bytes(s, j));
-          k[j] = *st.scale(s, j);
-        }
-        if (j == 0) rs = *st.rstd(s);
-        __syncwarp();  // read by all
-        issue(r + R * step, s, j);
+        // behind this unit's bytes: the rest of their row's, R - 1 rows of U + U, and this row's dy
+        copies_wait<2 * U * R - U - 1>();
+        if (n_of(j) > 0) raw = *st.data(s, j);
+        issue_dy(r + R * step, s, j);
       } else {
-        const int n = n_of(j), at = c + j * NT * G;
-        raw = Unit<T>::load(static_cast<const T*>(dy.p) + (int64_t)r * dy.ld, at, n);
-        if (n > 0) {
-          const int8_t* q = S.q + (int64_t)r * S.ld_q + at;
-          if constexpr (G == 8) bytes[j] = __ldcs(reinterpret_cast<const uint2*>(q));
-          else bytes[j].x = __ldcs(reinterpret_cast<const uint32_t*>(q));
-          k[j] = __ldg(S.scale + (int64_t)r * S.ld_s + at / kBlock);
-        }
-        if (j == 0) rs = __ldg(rstd + r);
+        raw = Unit<T>::load(static_cast<const T*>(dy.p) + (int64_t)r * dy.ld, c + j * NT * G, n_of(j));
+      }
+      return raw;
+    };
+    auto take_bytes = [&](int j, uint2& q, float& scale) {
+      q = make_uint2(0u, 0u);
+      scale = 0.0f;
+      if (n_of(j) == 0) return;
+      if constexpr (WHOLE) {
+        if constexpr (G == 8) q = *reinterpret_cast<const uint2*>(st.bytes(s, j));
+        else q.x = *reinterpret_cast<const uint32_t*>(st.bytes(s, j));
+        scale = *st.scale(s, j);
+      } else {
+        const int at = c + j * NT * G;
+        const int8_t* p = S.q + (int64_t)r * S.ld_q + at;
+        if constexpr (G == 8) q = __ldg(reinterpret_cast<const uint2*>(p));
+        else q.x = __ldg(reinterpret_cast<const uint32_t*>(p));
+        scale = __ldg(S.scale + (int64_t)r * S.ld_s + at / kBlock);
       }
     };
-    take(0);
+    // u = byte * scale * rstd: the factor, one per unit, goes where it is used once
+    float dot = 0.0f, d[U][G];
+    uint4 raw = take_dy(0);
+    __syncwarp();  // the first lanes' copies too (scales, rstd)
+    const float rs = WHOLE ? *st.rstd(s) : __ldg(rstd + r);
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       Unit<T>::unpack(raw, d[j]);
-      if (j + 1 < U) take(j + 1);  // its loads are on their way while unit j is worked on
-      float wt[G], u[G], part_dot = 0.0f;
+      uint2 q;
+      float k, wt[G], u[G], part_dot = 0.0f;
+      take_bytes(j, q, k);
       st.get_weight(j, wt);
-      Unit<T>::bytes(bytes[j], u);
-      k[j] *= rs;
+      if (j + 1 < U) {
+        raw = take_dy(j + 1);  // on its way while unit j is worked on
+        __syncwarp();
+      }
+      Unit<T>::bytes(q, u);
+      k *= rs;
 #pragma unroll
       for (int i = 0; i < G; ++i) {
-        acc[j][i] = fmaf(d[j][i] * k[j], u[i], acc[j][i]);
+        acc[j][i] = fmaf(d[j][i] * k, u[i], acc[j][i]);
         d[j][i] *= wt[i];
         part_dot = fmaf(d[j][i], u[i], part_dot);
       }
-      dot = fmaf(part_dot, k[j], dot);
+      dot = fmaf(part_dot, k, dot);
     }
-    s = s == R - 1 ? 0 : s + 1;
     dot = row_sum<NT>(dot, sh[par] + group * (NT / 32), group) * inv_cols;
     par ^= 1;
     T* out = static_cast<T*>(dx.p) + (int64_t)r * dx.ld + c;
+    const float rd = rs * dot;
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      const float kd = k[j] * dot;
-      float u[G];
-      asm volatile("" : "+r"(bytes[j].x), "+r"(bytes[j].y));  // converted again: bytes take a quarter of the room
-      Unit<T>::bytes(bytes[j], u);
+      uint2 q;
+      float k, u[G];
+      take_bytes(j, q, k);
+      Unit<T>::bytes(q, u);
+      __syncwarp();  // read by all: the place is free again
+      issue_bytes(r + R * step, s, j);
+      k *= rd;
 #pragma unroll
-      for (int i = 0; i < G; ++i) d[j][i] = rs * fmaf(-u[i], kd, d[j][i]);
+      for (int i = 0; i < G; ++i) d[j][i] = rs * fmaf(-u[i], k, d[j][i]);
       if (n_of(j) > 0) __stcg(reinterpret_cast<uint4*>(out + j * NT * G), RowIo<T>::pack(d[j]));
     }
+    s = s == R - 1 ? 0 : s + 1;
   }
   if (part) {  // the row groups' sums to one row of them, in order
     float* mine = part + (int64_t)blockIdx.x * ld_part;
