@@ -463,40 +463,49 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
     look(xc.r);
     return w;
   };
-  // The row's vectors [first, whole) lie within it; one before and one behind may hold others'
-  // elements and are worked on by the thread that has them, one element at a time.
-  auto sum = [&](int slot, Row w) {
+  // The row's vectors [first, whole) lie within it.  The elements before and behind them (fewer
+  // than 2 E <= 32) go one to a lane of warp 0, which loads them from the row itself: worked on
+  // in their vectors, they would cost a lane E terms while the others wait.
+  auto edge_index = [&](int skew) {
+    const int end = skew + cols, head = skew > 0 ? min(E - skew, cols) : 0, tail = skew > 0 && end < E ? 0 : end % E;
+    return tid < head ? tid : tid < head + tail ? cols - tail + tid - head : -1;
+  };
+  auto edge_of = [&](const T* x, Row w) {
+    if (w.y < 0 || (w.skew | cols % E) == 0) return -INFINITY;
+    const int i = edge_index(w.skew);
+    return i >= 0 ? to_f32(x[i]) : -INFINITY;
+  };
+  auto sum = [&](int slot, Row w, float edge) {
     MaxSum a{-INFINITY, 0.0f};
     if (w.y < 0) return a;
     const uint4* at = mine + slot * (kPieces * NT);
     const int first = w.skew > 0, end = w.skew + cols, whole = end / E - tid;
+    const int pieces = (end / E + NT - 1) / NT;
+    auto group = [&](int q, auto n) {
+      constexpr int N = decltype(n)::value;
+      uint4 raw[N];
+      bool in[N];
+#pragma unroll
+      for (int p = 0; p < N; ++p) {
+        in[p] = (q + p) * NT < whole && (q + p) * NT + tid >= first;
+        raw[p] = at[(q + p) * NT];
+      }
+      take_vectors<T, false, N>(a, raw, in, R.c);
+    };
 #pragma unroll
     for (int q = 0; q < kPieces; q += 4) {
-      if (q * NT < whole) {
-        uint4 raw[4];
-        bool in[4];
-#pragma unroll
-        for (int p = 0; p < 4; ++p) {
-          in[p] = (q + p) * NT < whole && (q + p) * NT + tid >= first;
-          raw[p] = at[(q + p) * NT];
-        }
-        take_vectors<T, false, 4>(a, raw, in, R.c);
-      }
+      // A vector of int8 is 16 terms a lane, so that a group of four with two in it is worth
+      // shortening (100000 rows of 1000: 141 -> 98 us); one of four or eight terms is not.
+      if (E == 16 && pieces - q == 1)
+        group(q, std::integral_constant<int, 1>());
+      else if (E == 16 && pieces - q == 2)
+        group(q, std::integral_constant<int, 2>());
+      else if (pieces > q)
+        group(q, std::integral_constant<int, 4>());
     }
-    if (w.skew > 0 || end % E) {
-      const int last = end / E;
-#pragma unroll 1
-      for (int k = 0; k < 2; ++k) {
-        const int v = k ? last : 0;
-        if (k ? (end % E == 0 || (last == 0 && w.skew > 0)) : w.skew == 0) continue;
-        if (v % NT != tid) continue;
-        float f[E];
-        RowIo<T>::unpack(at[v / NT * NT], f);
-#pragma unroll
-        for (int i = 0; i < E; ++i)
-          if (v * E + i < w.skew || v * E + i >= end) f[i] = -INFINITY;
-        take<E>(a, f, R.c);
-      }
+    if ((w.skew | cols % E) != 0 && tid < 32) {
+      const float f[1] = {edge};
+      take<1>(a, f, R.c);
     }
     return a;
   };
@@ -532,10 +541,11 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
   Cursor rc(R, blockIdx.x, step, R.s0, R.s1);                             // its logits, for the token's own
   Row w0 = issue(0), w1 = issue(1), w2 = issue(2), w3{-1, 0};
   float raw0 = raw_token(static_cast<const T*>(R.x) + rc.off, w0.y), raw1 = 0.0f;
+  float edge0 = edge_of(static_cast<const T*>(R.x) + rc.off, w0), edge1 = 0.0f;
   Given v0 = given(rc.r, w0.y), v1{0.0f, 0.0f, 0.0f};
   if (gc.r < rows) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kRows - 1) : "memory");
-    const MaxSum a = lanes_join<32>(sum(0, w0), R.c);
+    const MaxSum a = lanes_join<32>(sum(0, w0, edge0), R.c);
     if (!GRAD) w3 = issue(0);
     if ((tid & 31) == 0) warp_part[0][tid >> 5] = a;
     if (W > 1) __syncthreads(); else __syncwarp();
@@ -547,9 +557,10 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
     rc.next();
     if (rc.r < rows) {
       raw1 = raw_token(static_cast<const T*>(R.x) + rc.off, w1.y);
+      edge1 = edge_of(static_cast<const T*>(R.x) + rc.off, w1);
       v1 = given(rc.r, w1.y);
       asm volatile("cp.async.wait_group %0;" ::"n"(GRAD ? kRows - 2 : kRows - 1) : "memory");
-      const MaxSum a = lanes_join<32>(sum(slot1, w1), R.c);
+      const MaxSum a = lanes_join<32>(sum(slot1, w1, edge1), R.c);
       if ((tid & 31) == 0) warp_part[par ^ 1][tid >> 5] = a;
     }
     if (W > 1) __syncthreads(); else __syncwarp();  // row i's scalars, row i + 1's warps
@@ -573,26 +584,14 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
         for (int p = 0; p < kPieces; ++p)
           if (p * NT < whole && p * NT + tid >= first) store_slope<T, true>(gv, p * NT, at[p * NT], c);
       }
-      if (skew > 0 || end % E) {
-        const int last = end / E;
-#pragma unroll 1
-        for (int k = 0; k < 2; ++k) {
-          const int v = k ? last : 0;
-          if (k ? (end % E == 0 || (last == 0 && skew > 0)) : skew == 0) continue;
-          if (v % NT != tid) continue;
-          const T* xs = reinterpret_cast<const T*>(at + v / NT * NT);
-#pragma unroll 1
-          for (int i = 0; i < E; ++i)
-            if (v * E + i >= skew && v * E + i < end)
-              g[v * E + i - skew] = from_f32<GT>(zero ? 0.0f : slope_at(to_f32(xs[i]), c, false));
-        }
+      if ((skew | cols % E) != 0) {
+        const int i = edge_index(skew);
+        if (i >= 0) g[i] = from_f32<GT>(zero ? 0.0f : slope_at(edge0, c, i == w0.y));
       }
-      if (!zero) {  // the token's element, by the thread that has written its vector
-        const int v = (w0.y + skew) / E;
-        if (v % NT == tid) {
-          const float xy = to_f32(reinterpret_cast<const T*>(at + v / NT * NT)[(w0.y + skew) % E]);
-          g[w0.y] = from_f32<GT>(slope_at(xy, c, true));
-        }
+      const int yv = (w0.y + skew) / E;  // the token's element, by the thread that has written its vector
+      if (!zero && yv >= first && yv < end / E && yv % NT == tid) {
+        const float xy = to_f32(reinterpret_cast<const T*>(at + yv / NT * NT)[(w0.y + skew) % E]);
+        g[w0.y] = from_f32<GT>(slope_at(xy, c, true));
       }
       w3 = issue(slot);
     } else {
@@ -602,6 +601,7 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
     gc.next();
     w0 = w1, w1 = w2, w2 = w3, w3 = w4;
     raw0 = raw1;
+    edge0 = edge1;
     v0 = v1;
   }
 }
@@ -966,7 +966,8 @@ int check_logits(const eco_logits_t* L, const int64_t* tokens, const char* who) 
   ECO_REQUIRE(L->s0 >= 0 && L->s1 >= 0, ECO_ERR_ARG, "%s: negative strides", who);
   ECO_REQUIRE(reinterpret_cast<uintptr_t>(L->x) % (uintptr_t)esize(L->type) == 0, ECO_ERR_MISALIGNED,
               "%s: logits are not aligned to their type", who);
-  ECO_REQUIRE(L->n1 == 0 || L->n0 <= INT32_MAX / L->n1, ECO_ERR_ARG, "%s: 2^31 rows or more", who);
+  // 2^30, so that a row's number and a step of the grid more stay below 2^31
+  ECO_REQUIRE(L->n1 == 0 || L->n0 <= ((int64_t)1 << 30) / L->n1, ECO_ERR_ARG, "%s: more than 2^30 rows", who);
   ECO_REQUIRE(L->cols <= (int64_t)1 << 28, ECO_ERR_ARG, "%s: more than 2^28 columns", who);
   return ECO_OK;
 }

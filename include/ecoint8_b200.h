@@ -445,8 +445,8 @@ ECO_API int64_t eco_fp32_eco_scratch_len(const eco_fp32_layer_t* layers, int n_l
  * numbered n1 * i0 + i1, and tokens, mask and every per-row array have n0 * n1 values in
  * that order.  x = raw * mul (1 / temperature; int8 logits: also their scale).  A row counts
  * when its mask byte is nonzero (mask nullable) and its token lies in [0, cols); other rows
- * are not read, have log-probability 0 and zeros as gradient.  Fewer than 2^31 rows, at most
- * 2^28 columns. */
+ * are not read, have log-probability 0 and zeros as gradient.  At most 2^30 rows and 2^28
+ * columns. */
 enum { ECO_F32 = 0, ECO_BF16 = 1, ECO_F16 = 2, ECO_I8 = 3 };
 enum { ECO_PREFERENCE_SIGMOID = 0, ECO_PREFERENCE_HINGE = 1, ECO_PREFERENCE_IPO = 2 };
 

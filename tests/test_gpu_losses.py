@@ -260,6 +260,37 @@ def test_policy_loss(form, name, lead, cols, shifted):
     _check_policy(r, grad, x, raw, x64, tokens, mask, old, adv, ref, t, kl, lo, hi)
 
 
+# More rows than are in work at a time, several times over, for each width that is treated in
+# its own way (by 16-byte vectors per row: up to 256, 512, 1024, 2048, and two sizes beyond).
+MANY = [("fp32", (12007,), 37), ("bf16", (3, 4001), 1001), ("int8", (12007,), 503), ("fp16", (6007,), 3001),
+        ("fp32", (2, 3001), 2000), ("int8", (6007,), 8001), ("bf16", (3001,), 8192), ("int8", (2501,), 12345),
+        ("fp16", (2, 751), 12001), ("fp32", (1501,), 8001), ("int8", (1201,), 32000), ("bf16", (2, 451), 17003),
+        ("fp32", (901,), 9001), ("int8", (901,), 40001), ("bf16", (501,), 150001), ("fp32", (2, 251), 75003)]
+
+
+@pytest.mark.parametrize("name,lead,cols", MANY)
+def test_rows_of_every_width_many_times_over(name, lead, cols):
+    from ecoint8.losses import policy_loss_grad, token_logprobs
+
+    t, kl, lo, hi = 0.9, 0.05, 0.2, 0.28
+    x, tokens, mask, gen = _case(TYPES[name], lead, cols, cols, shifted=len(lead) == 2)
+    tokens.view(-1)[::11] = -100
+    tokens.view(-1)[5::101] = cols
+    raw, x64 = _fp64(x, t)
+    old, adv, ref = _policy_inputs(x64, tokens, gen)
+    lp = orc.token_logprobs(x64, tokens, orc.counting(tokens, cols))
+    for edge in (1 - lo, 1 + hi):  # ratios at a border of the clip may fall on either side: kept away from it
+        old = torch.where((torch.exp(lp - old.double()) - edge).abs() < 1e-3, old + 0.01, old)
+    s_out = S_OUT if name == "int8" else None
+    got = token_logprobs(x, tokens, mask=mask, temperature=t, s_out=s_out)
+    keep = orc.counting(tokens, cols, mask)
+    want = torch.where(keep, lp, 0.0)
+    assert ((got.double() - want).abs() <= _err(x64) + want.abs() * 2.0 ** -24).all()
+    r = policy_loss_grad(x, tokens, old, adv, ref_logp=ref, mask=mask, clip_low=lo, clip_high=hi, kl_coef=kl,
+                         temperature=t, s_out=s_out)
+    _check_policy(r, r.grad, x, raw, x64, tokens, mask, old, adv, ref, t, kl, lo, hi)
+
+
 def test_policy_without_reference_with_a_given_denominator_and_upstream_gradient():
     from ecoint8.losses import policy_loss, policy_loss_grad
 

@@ -124,7 +124,8 @@ def test_token_objectives_refuse_bad_arguments():
     nat, lib = _lib()
     bad = [(dict(cols=0), -1, "shape"), (dict(n1=-1), -1, "shape"), (dict(type=9), -1, "type"),
            (dict(mul=0.0), -1, "factor"), (dict(mul=math.nan), -1, "factor"), (dict(x=4097), -2, "aligned"),
-           (dict(x=None), -1, "null"), (dict(s1=-64), -1, "strides"), (dict(n0=1 << 20, n1=1 << 12), -1, "2^31"),
+           (dict(x=None), -1, "null"), (dict(s1=-64), -1, "strides"), (dict(n0=1 << 20, n1=1 << 12), -1, "2^30 rows"),
+           (dict(n1=(1 << 30) + 1), -1, "2^30 rows"),
            (dict(cols=(1 << 28) + 1), -1, "2^28")]
     for how, code, text in bad:
         _refused(lib.eco_token_logp(_logits_spec(**how), 8192, None, None, 0, 8192, None, None, None, None), code, text)
