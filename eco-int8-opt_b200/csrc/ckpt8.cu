@@ -9,8 +9,17 @@
 // would leave the fp32 range near there); a block that holds an infinity or NaN stands for
 // NaN throughout, so that what was not finite does not come back as something finite.
 //
-// Every kernel here gives a block to 16 lanes, eight columns each: the maximum is four
-// shuffles, the eight bytes one 8-byte store, and the bytes moved are the bound.
+// A block belongs to 16 lanes of eight columns each (fp32 in the norm: a warp of four each), so
+// that its maximum is a few shuffles and its bytes go out in one store per lane.  The bytes
+// moved bound every kernel here; at 16384 x 8192, in us and as a share of the bandwidth of a
+// copy (6.5 TB/s):
+//
+//           put away    bring back   gated f / b (8192 a side)   norm f / b
+//   bf16    71 (0.88)   72 (0.86)    193 / 195 (0.86 / 0.85)     120 / 127 (0.86 / 0.81)
+//   fp32    105 (0.98)  120 (0.86)   314 / 334 (0.92 / 0.86)     216 / 197 (0.86 / 0.94)
+//
+// (the norm's backward without dw; gelu in place of silu: 232 / 207 in bf16, where its arithmetic is as
+// long as the copy).
 #include <algorithm>
 #include <cmath>
 
@@ -33,8 +42,9 @@ struct Oct {  // N columns
 };
 
 // Columns [c, c + n) of a row, n in [0, N]; the others are zeros.  A row that does not start
-// on 16 bytes (32 for eight of fp32) is read by the 16-byte words that hold its columns, shifted into
-// place (each word that is read holds at least one of them, so none lies outside the row's memory).
+// on 16 bytes (32 for eight of fp32) is read by the 16-byte words that hold its columns, shifted
+// into place (each word that is read holds at least one of them, so none lies outside the row's
+// memory).
 template <typename T, int N = 8>
 ECO_DEV Oct<T, N> load8(const T* row, int c, int n) {
   constexpr int W = Oct<T, N>::W, V = W / 4;  // 32-bit words, 16-byte words
@@ -45,8 +55,9 @@ ECO_DEV Oct<T, N> load8(const T* row, int c, int n) {
       // volatile: without it the load counts as a pure function of the address, free to move in
       // front of the conditions that say the address is good
       asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-          : "=r"(o.w[0]), "=r"(o.w[1]), "=r"(o.w[2]), "=r"(o.w[3]), "=r"(o.w[4]), "=r"(o.w[5]), "=r"(o.w[6]), "=r"(o.w[7])
-          : "l"(row + c));
+                   : "=r"(o.w[0]), "=r"(o.w[1]), "=r"(o.w[2]), "=r"(o.w[3]), "=r"(o.w[4]), "=r"(o.w[5]), "=r"(o.w[6]),
+                     "=r"(o.w[7])
+                   : "l"(row + c));
     } else {
       const uint4 t = __ldg(reinterpret_cast<const uint4*>(row + c));
       o.w[0] = t.x, o.w[1] = t.y, o.w[2] = t.z, o.w[3] = t.w;
@@ -96,8 +107,9 @@ ECO_DEV void unpack8(const Oct<T>& o, float (&f)[8]) {
   }
 }
 
-// Eight columns of an output row (past L1, which keeps what is read again: a weight): whole where eight columns of the row start on a boundary of
-// their size (its padding takes the rest of the last eight), else n single stores.
+// Eight columns of an output row, past L1 (which keeps what is read again: a weight): whole where
+// eight columns of the row start on a boundary of their size (its padding takes the rest of the
+// last eight), else n single stores.
 template <typename T>
 ECO_DEV void store8(T* row, int c, int n, bool vec, const float (&f)[8]) {
   if (vec) {
@@ -143,8 +155,8 @@ ECO_DEV float block_amax(const Oct<T>& o) {
     else return __half2float(__ushort_as_half((unsigned short)m));
   }
 }
-// Gains of N blocks of a half-warp (or warp) from their maxima, and in lane i (< N) the scale of block i:
-// lane i does block i's two divisions, so that N blocks cost the divisions of one.
+// Gains of N blocks of a half-warp (or warp) from their maxima, and in lane i (< N) the scale of
+// block i: lane i does block i's two divisions, so that N blocks cost the divisions of one.
 template <int N, int LANES = kLanes>
 ECO_DEV float block_gains(const float (&amax)[N], float (&gain)[N]) {
   const int lane = threadIdx.x & (LANES - 1);
@@ -244,8 +256,6 @@ ECO_DEV Oct<T> load_cols(const Mat& x, int r, const Place& at) {
   }
   return o;
 }
-// Puts the eight columns of N numbers (rows, or gate and up of them) away: their maxima, the
-// gains of all N blocks at once, the bytes; lane i keeps block i's scale.
 template <typename T>
 ECO_DEV void put_bytes(const Oct<T>& o, float gain, int8_t* q) {
   float f[8];
@@ -958,7 +968,8 @@ dim3 block_grid(int64_t rows, int64_t cols, int l, int unroll) {
 }
 
 int check_saved(const eco_saved_i8_t* S, int64_t rows, int64_t cols, const char* who) {
-  ECO_REQUIRE(S && S->q && S->scale && S->ld_q >= cols && S->ld_q <= INT32_MAX && S->ld_q % 16 == 0 && eco_aligned16(S->q) &&
+  ECO_REQUIRE(S && S->q && S->scale && S->ld_q >= cols && S->ld_q <= INT32_MAX && S->ld_q % 16 == 0 &&
+                  eco_aligned16(S->q) && reinterpret_cast<uintptr_t>(S->scale) % 4 == 0 &&
                   S->ld_scale >= (cols + kBlock - 1) / kBlock && S->ld_scale <= INT32_MAX,
               ECO_ERR_ARG, "%s: bad eight-bit buffers", who);
   return ECO_OK;
@@ -981,8 +992,9 @@ bool whole8(const void* p, int64_t ld, int64_t rows, int64_t cols, int type) {
   return rows_on_8(p, ld, rows, type) && cols % 8 == 0;
 }
 int check_in(const void* p, int64_t ld, int64_t rows, int64_t cols, int type, const char* who) {
-  ECO_REQUIRE(p && (rows <= 1 || (ld >= 0 && ld <= INT32_MAX)) && reinterpret_cast<uintptr_t>(p) % (uintptr_t)es_of(type) == 0, ECO_ERR_ARG,
-              "%s: bad input", who);
+  ECO_REQUIRE(p && (rows <= 1 || (ld >= 0 && ld <= INT32_MAX)) &&
+                  reinterpret_cast<uintptr_t>(p) % (uintptr_t)es_of(type) == 0,
+              ECO_ERR_ARG, "%s: bad input", who);
   return ECO_OK;
 }
 // Outputs have rows of whole groups of eight columns that start on a boundary of their size.
@@ -1113,8 +1125,10 @@ extern "C" int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int ac
   if (int rc = check_in(dy, ld_dy, rows, cols, type, "eco_gated_act_bwd")) return rc;
   if (int rc = check_saved(saved_gate, rows, cols, "eco_gated_act_bwd")) return rc;
   if (int rc = check_saved(saved_up, rows, cols, "eco_gated_act_bwd")) return rc;
-  ECO_REQUIRE(dgate && dup && (rows <= 1 || (ld_dgate >= cols && ld_dup >= cols && ld_dgate <= INT32_MAX && ld_dup <= INT32_MAX)), ECO_ERR_ARG,
-              "eco_gated_act_bwd: bad outputs");
+  ECO_REQUIRE(dgate && dup &&
+                  (rows <= 1 ||
+                   (ld_dgate >= cols && ld_dup >= cols && ld_dgate <= INT32_MAX && ld_dup <= INT32_MAX)),
+              ECO_ERR_ARG, "eco_gated_act_bwd: bad outputs");
   // A half of one packed output has no padding of its own: the last columns, fewer than eight,
   // are stored one by one, and so is a half whose rows do not start on eight elements.
   const bool vg = rows_on_8(dgate, ld_dgate, rows, type);
@@ -1194,7 +1208,7 @@ extern "C" int eco_rms_norm_bwd(const void* dy, int64_t ld_dy, int type, int64_t
   if (int rc = check_in(dy, ld_dy, rows, cols, type, "eco_rms_norm_bwd")) return rc;
   if (int rc = check_saved(saved, rows, cols, "eco_rms_norm_bwd")) return rc;
   if (int rc = check_out(dx, ld_dx, rows, cols, type, "eco_rms_norm_bwd")) return rc;
-  ECO_REQUIRE(rstd, ECO_ERR_ARG, "eco_rms_norm_bwd: null rstd");
+  ECO_REQUIRE(rstd && reinterpret_cast<uintptr_t>(rstd) % 4 == 0, ECO_ERR_ARG, "eco_rms_norm_bwd: bad rstd");
   const int64_t ctas = rms_ctas(rows, cols), ld_part = (cols + 7) / 8 * 8;
   ECO_REQUIRE(!dw || (scratch && eco_aligned16(scratch) && scratch_len >= ctas * ld_part), ECO_ERR_ARG,
               "eco_rms_norm_bwd: scratch too small (eco_rms_norm_bwd_scratch)");

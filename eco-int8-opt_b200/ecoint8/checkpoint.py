@@ -114,11 +114,12 @@ def saved_i8(min_numel: int = 1 << 16):
     """Inside this context, autograd keeps the floating CUDA activations it saves in eight bits.
 
     Parameters and other leaves that ask for gradients (and views of them), tensors of other
-    types and tensors of fewer than ``min_numel`` values are kept as they are.  A tensor that
+    types or layouts and those of fewer than ``min_numel`` values are kept as they are.  A tensor that
     is not kept by its caller is freed; its backward formula reads what the eight bits stand for."""
 
     def pack(t):
-        if not t.is_cuda or t.dtype not in _FLOATS or t.dim() < 1 or t.numel() < max(1, min_numel) or _is_weight(t):
+        if not t.is_cuda or t.layout is not torch.strided or t.dtype not in _FLOATS or t.dim() < 1 or \
+                t.numel() < max(1, min_numel) or _is_weight(t):
             return t
         return checkpoint_i8(t.detach())
 

@@ -69,6 +69,17 @@ def test_strides_alignment_and_shapes(name):
         assert torch.equal(got.reshape(flat.shape), orc.stands_for(flat).float().to(x.dtype))
 
 
+# More rows than are in work at a time, by the number of blocks that stand side by side in a CTA.
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("rows,cols", [(150001, 120), (90001, 256), (50003, 384), (20001, 1001), (10007, 2048)])
+def test_eight_bits_of_many_rows(name, rows, cols):
+    from ecoint8.checkpoint import checkpoint_i8, restore_i8
+
+    x, _ = _x(rows, cols, TYPES[name], cols)
+    assert torch.equal(restore_i8(checkpoint_i8(x), torch.float32).double(), orc.stands_for(x).float().double())
+    assert torch.equal(restore_i8(checkpoint_i8(x)), orc.stands_for(x).float().to(x.dtype))
+
+
 def test_zeros_tiny_huge_and_not_finite_blocks():
     from ecoint8.checkpoint import checkpoint_i8, restore_i8
 
@@ -105,6 +116,16 @@ def test_rms_norm(name, cols):
                                                   ("bf16", "fp32", 400, 17000)])
 def test_rms_norm_weights_and_many_rows(name, wname, rows, cols):
     _rms_case(TYPES[name], rows, cols, TYPES[wname] if wname else None, rows)
+
+
+# Every number of threads per row, with more rows than fit the stages of all CTAs at a time.
+@pytest.mark.parametrize("name,rows,cols", [("bf16", 12001, 256), ("fp32", 12001, 256), ("fp16", 10001, 512),
+                                            ("fp32", 10001, 388), ("bf16", 9001, 1000), ("fp32", 9001, 1024),
+                                            ("bf16", 6001, 2048), ("fp32", 6001, 1500), ("fp16", 4001, 4096),
+                                            ("fp32", 3001, 4096), ("bf16", 2001, 8192), ("fp32", 2001, 8000),
+                                            ("bf16", 1101, 16384), ("fp32", 1101, 16384), ("fp16", 3001, 4095)])
+def test_rms_norm_of_every_width_many_times_over(name, rows, cols):
+    _rms_case(TYPES[name], rows, cols, TYPES[name], rows + cols)
 
 
 def _rms_case(dtype, rows, cols, wtype, seed):
@@ -209,7 +230,9 @@ def test_rms_norm_of_zero_rows_and_differences():
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("rows,cols,packed", [(1, 1, True), (3, 5, True), (4, 128, True), (9, 1337, True),
-                                              (2, 2000, False), (40, 129, False), (300, 3, False), (5, 8192, True)])
+                                              (2, 2000, False), (40, 129, False), (300, 3, False), (5, 8192, True),
+                                              (60001, 128, True), (30001, 200, False), (9001, 1001, True),
+                                              (5003, 2048, False)])
 def test_gated_activation(act, name, rows, cols, packed):
     from ecoint8.checkpoint import gated_act_i8
 
@@ -393,6 +416,17 @@ def test_losses_and_layers_under_saved_i8_keep_their_own_state():
     # a logit is off by half a step of its block: its probability by that much relatively, and a little more
     step = x.abs().double().view(600, 2, 128).amax(2).repeat_interleave(128, 1) / 254
     assert ((g.double() - want).abs() <= p * step * 1.1 + 2.0 ** -20).all()
+
+
+def test_sparse_tensors_pass_through_saved_i8():
+    from ecoint8.checkpoint import saved_i8
+
+    a = torch.eye(40).cuda().to_sparse()
+    x = torch.ones(40, 30).cuda().requires_grad_()
+    with saved_i8(min_numel=1):
+        y = torch.sparse.mm(a, x)
+    (g,) = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(g, torch.ones_like(g))
 
 
 def test_feed_forward_block_trains():

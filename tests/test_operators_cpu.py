@@ -166,7 +166,7 @@ def test_eight_bit_activations_refuse_bad_arguments():
     _refused(lib.eco_ckpt_pack(8192, 0, 4, 0, 64, ok, None), -1, "shape")
     _refused(lib.eco_ckpt_pack(8193, 0, 4, 64, 64, ok, None), -1, "input")
     for saved in ((None, 8192, 64, 1), (8192, 8192, 63, 1), (8192, 8192, 48, 1), (8200, 8192, 64, 1),
-                  (8192, 8192, 64, 0)):
+                  (8192, 8192, 64, 0), (8192, 8194, 64, 1)):
         _refused(lib.eco_ckpt_pack(8192, 0, 4, 64, 64, ctypes.byref(nat.SavedI8(*saved)), None), -1, "eight-bit")
     _refused(lib.eco_ckpt_restore(ok, 1, 4, 63, 8192, 63, None), -1, "too short")
     _refused(lib.eco_ckpt_restore(ok, 1, 4, 64, 8200, 64, None), -2, "eight elements")
