@@ -41,55 +41,63 @@ struct Oct {  // N columns
   uint32_t w[W];
 };
 
-// Columns [c, c + n) of a row, n in [0, N]; the others are zeros.  A row that does not start
-// on 16 bytes (32 for eight of fp32) is read by the 16-byte words that hold its columns, shifted
-// into place (each word that is read holds at least one of them, so none lies outside the row's
-// memory).
+// Where `on`, 16 bytes; else zeros.  No branch, so that several rows' loads go out together;
+// volatile: a load that counts as a pure function of its address may move in front of the
+// conditions that say the address is good.
+ECO_DEV uint4 load_if(const uint4* p, bool on) {
+  uint4 t;
+  asm volatile(
+      "{ .reg .pred on; setp.ne.u32 on, %5, 0;\n"
+      "mov.b32 %0, 0; mov.b32 %1, 0; mov.b32 %2, 0; mov.b32 %3, 0;\n"
+      "@on ld.global.nc.v4.b32 {%0, %1, %2, %3}, [%4]; }"
+      : "=&r"(t.x), "=&r"(t.y), "=&r"(t.z), "=&r"(t.w)
+      : "l"(p), "r"((uint32_t)on));
+  return t;
+}
+
+// Columns [c, c + n) of a row of any alignment, n in [0, N]; the others are zeros.  The 16-byte
+// words that hold the columns are read and shifted into place (each word that is read holds at
+// least one of them, so none lies outside the row's memory).
 template <typename T, int N = 8>
 ECO_DEV Oct<T, N> load8(const T* row, int c, int n) {
   constexpr int W = Oct<T, N>::W, V = W / 4;  // 32-bit words, 16-byte words
   Oct<T, N> o;
   const uintptr_t a = reinterpret_cast<uintptr_t>(row + c);
-  if (n == N && (a & (16 * V - 1)) == 0) {
-    if constexpr (V == 2) {
-      // volatile: without it the load counts as a pure function of the address, free to move in
-      // front of the conditions that say the address is good
-      asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                   : "=r"(o.w[0]), "=r"(o.w[1]), "=r"(o.w[2]), "=r"(o.w[3]), "=r"(o.w[4]), "=r"(o.w[5]), "=r"(o.w[6]),
-                     "=r"(o.w[7])
-                   : "l"(row + c));
-    } else {
-      const uint4 t = __ldg(reinterpret_cast<const uint4*>(row + c));
-      o.w[0] = t.x, o.w[1] = t.y, o.w[2] = t.z, o.w[3] = t.w;
-    }
-    return o;
-  }
   const uint4* p = reinterpret_cast<const uint4*>(a & ~uintptr_t(15));
   const uint32_t skew = (uint32_t)a & 15;
   const int end = n > 0 ? (int)skew + n * (int)sizeof(T) : 0;  // bytes that are needed, from p on
   uint32_t w[W + 4];
 #pragma unroll
   for (int v = 0; v <= V; ++v) {
-    uint4 t = make_uint4(0u, 0u, 0u, 0u);
-    if (16 * v < end) t = __ldg(p + v);
+    const uint4 t = load_if(p + v, 16 * v < end);
     w[4 * v] = t.x, w[4 * v + 1] = t.y, w[4 * v + 2] = t.z, w[4 * v + 3] = t.w;
   }
-  if (skew & 8) {
 #pragma unroll
-    for (int i = 0; i < W + 2; ++i) w[i] = w[i + 2];
-  }
-  if (skew & 4) {
+  for (int i = 0; i < W + 2; ++i) w[i] = skew & 8 ? w[i + 2] : w[i];
 #pragma unroll
-    for (int i = 0; i < W + 1; ++i) w[i] = w[i + 1];
-  }
-  const uint32_t bits = (skew & 3) * 8;
+  for (int i = 0; i < W + 1; ++i) w[i] = skew & 4 ? w[i + 1] : w[i];
 #pragma unroll
   for (int i = 0; i < W; ++i) {  // columns past the n-th are the row's neighbours: zeros here
-    o.w[i] = __funnelshift_r(w[i], w[i + 1], bits);
-    if constexpr (sizeof(T) == 4)
-      o.w[i] = i < n ? o.w[i] : 0u;
-    else
+    if constexpr (sizeof(T) == 4) {
+      o.w[i] = i < n ? w[i] : 0u;
+    } else {
+      o.w[i] = __funnelshift_r(w[i], w[i + 1], (skew & 3) * 8);
       o.w[i] = 2 * i + 1 < n ? o.w[i] : (2 * i < n ? o.w[i] & 0xffffu : 0u);
+    }
+  }
+  return o;
+}
+
+// The same, in one load where the eight columns lie on a boundary: for kernels that do not know
+// of their rows.
+template <typename T>
+ECO_DEV Oct<T> load8_either(const T* row, int c, int n) {
+  if (n < 8 || (reinterpret_cast<uintptr_t>(row + c) & 15) != 0) return load8(row, c, n);
+  Oct<T> o;
+#pragma unroll
+  for (int v = 0; v < Oct<T>::W / 4; ++v) {
+    const uint4 t = load_if(reinterpret_cast<const uint4*>(row + c) + v, true);
+    o.w[4 * v] = t.x, o.w[4 * v + 1] = t.y, o.w[4 * v + 2] = t.z, o.w[4 * v + 3] = t.w;
   }
   return o;
 }
@@ -850,7 +858,7 @@ __global__ void __launch_bounds__(kWide)
     float ss = 0.0f;
     for (int c = threadIdx.x * 8; c < cols; c += kWide * 8) {
       float f[8];
-      unpack8(load8(row, c, left8(cols, c)), f);
+      unpack8(load8_either(row, c, left8(cols, c)), f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
     }
@@ -861,7 +869,7 @@ __global__ void __launch_bounds__(kWide)
       const int c = cc + threadIdx.x * 8, c0 = c - 8 * lane;
       const int n = left8(cols, c);
       float f[8], wt[8];
-      const Oct<T> o = load8(row, c, n);
+      const Oct<T> o = load8_either(row, c, n);
       unpack8(o, f);
       if (S.q) {
         const float amax[1] = {block_amax(o)};
@@ -892,7 +900,7 @@ __global__ void __launch_bounds__(kWide)
     for (int c = threadIdx.x * 8; c < cols; c += kWide * 8) {
       const int n = left8(cols, c);
       float d[8], u[8], wt[8];
-      unpack8(load8(row, c, n), d);
+      unpack8(load8_either(row, c, n), d);
       Eights e = fetch8(S, r, c, n);
       e.s *= rs;
       values8(e, u);
@@ -911,7 +919,7 @@ __global__ void __launch_bounds__(kWide)
     for (int c = threadIdx.x * 8; c < cols; c += kWide * 8) {
       const int n = left8(cols, c);
       float d[8], u[8], wt[8];
-      unpack8(load8(row, c, n), d);
+      unpack8(load8_either(row, c, n), d);
       Eights e = fetch8(S, r, c, n);
       e.s *= rs;
       values8(e, u);
@@ -952,10 +960,12 @@ __global__ void __launch_bounds__(1024) rms_dw_kernel(const float* __restrict__ 
 }
 
 // ------------------------------------------------ host side
+// 2^l blocks side by side in a CTA: as many as leave no more than an eighth of the places empty
+// (33 blocks: four side by side, nine columns of CTAs; sixteen would leave 15 of 48 places idle).
 int bpr_log2_of(int64_t cols) {
   const int64_t blocks = (cols + kBlock - 1) / kBlock;
-  int l = 0;
-  while (l < 4 && (1 << l) < blocks) ++l;
+  int l = 4;
+  while (l > 0 && ((-blocks & ((1 << l) - 1)) * 8 > blocks + 6)) --l;
   return l;
 }
 // A column of CTAs for every 2^l blocks; down the rows, as many as are resident (eight of 256
