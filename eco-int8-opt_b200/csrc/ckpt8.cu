@@ -909,8 +909,10 @@ __global__ void __launch_bounds__(kWide)
         float4* at = reinterpret_cast<float4*>(mine + c);
         float4 s0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), s1 = s0;
         if (k) s0 = at[0], s1 = at[1];
-        at[0] = make_float4(fmaf(d[0], u[0], s0.x), fmaf(d[1], u[1], s0.y), fmaf(d[2], u[2], s0.z), fmaf(d[3], u[3], s0.w));
-        at[1] = make_float4(fmaf(d[4], u[4], s1.x), fmaf(d[5], u[5], s1.y), fmaf(d[6], u[6], s1.z), fmaf(d[7], u[7], s1.w));
+        at[0] = make_float4(fmaf(d[0], u[0], s0.x), fmaf(d[1], u[1], s0.y), fmaf(d[2], u[2], s0.z),
+                            fmaf(d[3], u[3], s0.w));
+        at[1] = make_float4(fmaf(d[4], u[4], s1.x), fmaf(d[5], u[5], s1.y), fmaf(d[6], u[6], s1.z),
+                            fmaf(d[7], u[7], s1.w));
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) dot = fmaf(d[j] * wt[j], u[j], dot);
@@ -1153,8 +1155,8 @@ extern "C" int eco_gated_act_bwd(const void* dy, int64_t ld_dy, int type, int ac
                             ? (whole ? gated_bwd_kernel<T, true, U, true> : gated_bwd_kernel<T, true, U, false>)
                             : (whole ? gated_bwd_kernel<T, false, U, true> : gated_bwd_kernel<T, false, U, false>);
     kernel<<<grid, kThreads, 0, eco_stream(stream)>>>(mat(dy, ld_dy), (int)rows, (int)cols, saved_of(saved_gate),
-                                                      saved_of(saved_up), mat(dgate, ld_dgate), mat(dup, ld_dup), vg, vu,
-                                                      l);
+                                                      saved_of(saved_up), mat(dgate, ld_dgate), mat(dup, ld_dup), vg,
+                                                      vu, l);
   });
   return eco_launch_check("eco_gated_act_bwd");
 }

@@ -458,7 +458,8 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
 #pragma unroll
       for (int p = 0; p < kPieces; ++p)
         if (p * NT < left)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + p * NT * 16), "l"(src + p * NT) : "memory");
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + p * NT * 16), "l"(src + p * NT)
+                       : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     xc.next();
@@ -643,11 +644,14 @@ __global__ void __launch_bounds__(kWide, 3)
   }
 }
 
-// The whole policy loss.  The first kPlaces vectors per thread of a row stay in shared memory, the rest is read again
-// for the gradient, from L2: the launch lets no more rows be in work than L2 holds the rests of.
-// As soon as a place has been used for the last time, the next row's vector is copied there
-// (cp.async by the thread that will use it), so memory is read while the end of a row is
-// summed, joined and written.
+// The whole policy loss.  The first kPlaces vectors per thread of a row stay in shared memory, the
+// rest is read again for the gradient, from L2: the launch lets no more rows be in work than L2
+// holds the rests of.  As soon as a place has been used for the last time, the next row's vector
+// is copied there (cp.async by the thread that will use it), so memory is read while the end of a
+// row is summed, joined and written.
+// One read and one write of bf16 8192 x 131072: 850 us, 0.77 of the bandwidth of a copy (fp32 4096
+// rows: 805, 0.81).  DRAM is busy for 0.85 of it (what L2 loses of the rests comes on top) and the
+// issue slots for 0.56 of it; two CTAs per SM take turns at reading and writing.
 constexpr int kPlaces = 12;
 constexpr int kBatch = 4;  // vectors read again at a time
 
@@ -692,10 +696,14 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
     }
     return w;
   };
+  // These are read once: they leave L2 to the rests, of which a third was lost to them (fp32 4096
+  // rows of 131072: 866 -> 804 us).
+  uint64_t once;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(once));
   auto copy = [&](const Row& w, int p) {
     if (p * NT + tid < w.vecs)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine_s + p * NT * 16),
-                   "l"(reinterpret_cast<const uint4*>(w.x + w.head) + p * NT + tid)
+      asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(mine_s + p * NT * 16),
+                   "l"(reinterpret_cast<const uint4*>(w.x + w.head) + p * NT + tid), "l"(once)
                    : "memory");
   };
   look(xc.r);
@@ -1004,7 +1012,8 @@ bool launch_held(const Rows& R, const Policy& P, const int* counts, float gain, 
                  cudaStream_t s) {
   const auto kernel = held_rows_kernel<T, NT, GRAD>;
   constexpr int smem = kRows * kPieces * NT * 16;
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if (smem > 40 * 1024 &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return false;
   const int64_t grid = std::min<int64_t>(R.rows, (int64_t)eco_num_sms() * (kHeld / NT));
   kernel<<<(unsigned)grid, NT, smem, s>>>(R, P, counts, gain, O, G);
