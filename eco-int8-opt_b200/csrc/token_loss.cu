@@ -809,67 +809,65 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
   }
 }
 
-// Fixed-order sum over a CTA of 1024 threads.
-ECO_DEV double cta_sum(double v, double* sh) {
+// N sums over a CTA in a fixed order, to every thread; sh: 32 N doubles.  The warps' sums are
+// joined by shuffles as well: one after the other they took longer than all the rest for few rows.
+template <int N>
+ECO_DEV void cta_sums(double (&v)[N], double* sh) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x / 32;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+  if (lane == 0)
+#pragma unroll
+    for (int i = 0; i < N; ++i) sh[i * 32 + warp] = v[i];
   __syncthreads();
-  v = 0.0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) v += sh[w];
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = lane < warps ? sh[i * 32 + lane] : 0.0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
   __syncthreads();
-  return v;
 }
 
 // loss, kl and clip fraction from the rows' terms (one CTA, fixed order, sums in double).
 __global__ void __launch_bounds__(1024) policy_finish_kernel(const __grid_constant__ Rows R, const Terms terms,
                                                               double denom, const int* counts, float* out) {
-  __shared__ double sh[32];
+  __shared__ double sh[3 * 32];
   __shared__ int counts_sh[32];
   const double n = policy_denom(R, denom, counts, counts_sh);
-  double a = 0.0, b = 0.0, d = 0.0;
+  double v[3] = {};
   for (int64_t r = threadIdx.x; r < R.rows; r += blockDim.x) {
-    a += terms.loss[r];
-    b += terms.kl[r];
-    d += terms.clip[r];
+    v[0] += terms.loss[r];
+    v[1] += terms.kl[r];
+    v[2] += terms.clip[r];
   }
-  a = cta_sum(a, sh);
-  b = cta_sum(b, sh);
-  d = cta_sum(d, sh);
-  if (threadIdx.x == 0) {
-    out[0] = (float)(a / n);
-    out[1] = (float)(b / n);
-    out[2] = (float)(d / n);
-  }
+  cta_sums(v, sh);
+  if (threadIdx.x < 3) out[threadIdx.x] = (float)((threadIdx.x == 0 ? v[0] : threadIdx.x == 1 ? v[1] : v[2]) / n);
 }
 
 // The policy loss from log-probabilities: terms and coefficients (one CTA).
 __global__ void __launch_bounds__(1024) policy_tokens_kernel(const __grid_constant__ Rows R,
                                                               const __grid_constant__ Policy P, const double* lp64,
                                                               float* coef, float* out) {
-  __shared__ double sh[32];
+  __shared__ double sh[3 * 32];
   __shared__ int counts_sh[32];
   const double n = policy_denom(R, P.denom, nullptr, counts_sh), inv = 1.0 / n;
-  double a = 0.0, b = 0.0, d = 0.0;
+  double v[3] = {};
   for (int64_t r = threadIdx.x; r < R.rows; r += blockDim.x) {
     float k = 0.0f;
     if (R.counts(r)) {
       const Token t = policy_token(P, given_of(P, r), lp64[r]);
-      a += t.loss;
-      b += t.kl;
-      d += t.clipped ? 1.0 : 0.0;
+      v[0] += t.loss;
+      v[1] += t.kl;
+      v[2] += t.clipped ? 1.0 : 0.0;
       k = over(t.coef, inv, 1.0f);
     }
     coef[r] = k;
   }
-  a = cta_sum(a, sh);
-  b = cta_sum(b, sh);
-  d = cta_sum(d, sh);
-  if (threadIdx.x == 0) {
-    out[0] = (float)(a / n);
-    out[1] = (float)(b / n);
-    out[2] = (float)(d / n);
-  }
+  cta_sums(v, sh);
+  if (threadIdx.x < 3) out[threadIdx.x] = (float)((threadIdx.x == 0 ? v[0] : threadIdx.x == 1 ? v[1] : v[2]) / n);
 }
 
 // ------------------------------------------------ the preference loss
@@ -887,27 +885,29 @@ struct Pairs {
 __global__ void __launch_bounds__(256) pair_kernel(const __grid_constant__ Rows R, const __grid_constant__ Pairs P,
                                                     const double* lp64, float* coef, float* log_ratio, float* margin,
                                                     double* pair_loss) {
-  __shared__ double sh[32];
+  __shared__ double sh[4 * 32];
   const int64_t p = blockIdx.x;
   int64_t lo[2], hi[2];
-  double ratio[2], per[2];
+  double ratio[2], per[2], v[4] = {};  // sums and numbers of rows
+#pragma unroll
   for (int s = 0; s < 2; ++s) {
     const int64_t q = p + s * P.pairs;
     int64_t b = R.cu ? (int64_t)R.cu[q] : q * P.seq_len, e = R.cu ? (int64_t)R.cu[q + 1] : (q + 1) * P.seq_len;
     b = b < 0 ? 0 : (b > R.rows ? R.rows : b);
     e = e < b ? b : (e > R.rows ? R.rows : e);
-    double v = 0.0, n = 0.0;
     for (int64_t r = b + threadIdx.x; r < e; r += blockDim.x)
       if (R.counts(r)) {
-        v += lp64[r] - (double)P.ref[r];
-        n += 1.0;
+        v[s] += lp64[r] - (double)P.ref[r];
+        v[2 + s] += 1.0;
       }
-    v = cta_sum(v, sh);
-    n = cta_sum(n, sh);
     lo[s] = b;
     hi[s] = e;
-    per[s] = P.average && n > 0.0 ? 1.0 / n : 1.0;
-    ratio[s] = v * per[s];
+  }
+  cta_sums(v, sh);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    per[s] = P.average && v[2 + s] > 0.0 ? 1.0 / v[2 + s] : 1.0;
+    ratio[s] = v[s] * per[s];
   }
   const double delta = ratio[0] - ratio[1], h = P.beta * delta;
   double loss, slope;  // slope: d loss / d delta
@@ -929,6 +929,7 @@ __global__ void __launch_bounds__(256) pair_kernel(const __grid_constant__ Rows 
     margin[p] = (float)h;
     pair_loss[p] = loss;
   }
+#pragma unroll
   for (int s = 0; s < 2; ++s) {
     const float k = (float)((s ? -slope : slope) * per[s] / P.denom);
     for (int64_t r = lo[s] + threadIdx.x; r < hi[s]; r += blockDim.x)
@@ -939,10 +940,10 @@ __global__ void __launch_bounds__(256) pair_kernel(const __grid_constant__ Rows 
 __global__ void __launch_bounds__(256) pair_finish_kernel(const double* pair_loss, int64_t pairs, double denom,
                                                            float* out) {
   __shared__ double sh[32];
-  double a = 0.0;
-  for (int64_t p = threadIdx.x; p < pairs; p += blockDim.x) a += pair_loss[p];
-  a = cta_sum(a, sh);
-  if (threadIdx.x == 0) out[0] = (float)(a / denom);
+  double a[1] = {};
+  for (int64_t p = threadIdx.x; p < pairs; p += blockDim.x) a[0] += pair_loss[p];
+  cta_sums(a, sh);
+  if (threadIdx.x == 0) out[0] = (float)(a[0] / denom);
 }
 
 // ------------------------------------------------ host side
@@ -966,13 +967,16 @@ Rows rows_of(const eco_logits_t& L, const int64_t* tokens, const uint8_t* mask, 
   return R;
 }
 
+// Threads of a kernel of one CTA over n rows.
+unsigned one_cta(int64_t n) { return (unsigned)std::min<int64_t>(1024, (n + 31) / 32 * 32); }
+
 int esize(int type) { return type == ECO_F32 ? 4 : type == ECO_I8 ? 1 : 2; }
 
 int check_logits(const eco_logits_t* L, const int64_t* tokens, const char* who) {
   ECO_REQUIRE(L && L->n0 >= 0 && L->n1 >= 0 && L->cols > 0, ECO_ERR_ARG, "%s: bad shape", who);
   ECO_REQUIRE(L->type >= ECO_F32 && L->type <= ECO_I8, ECO_ERR_ARG, "%s: unknown logits type %d", who, L->type);
   ECO_REQUIRE(L->n0 == 0 || L->n1 == 0 || (L->x && tokens), ECO_ERR_ARG, "%s: null logits or tokens", who);
-  ECO_REQUIRE(std::isfinite(L->mul) && L->mul > 0.0, ECO_ERR_ARG, "%s: the logits' factor must be positive", who);
+  ECO_REQUIRE(L->mul >= 1e-30 && L->mul <= 1e30, ECO_ERR_ARG, "%s: the logits' factor must lie in [1e-30, 1e30]", who);
   ECO_REQUIRE(L->s0 >= 0 && L->s1 >= 0, ECO_ERR_ARG, "%s: negative strides", who);
   ECO_REQUIRE(reinterpret_cast<uintptr_t>(L->x) % (uintptr_t)esize(L->type) == 0, ECO_ERR_MISALIGNED,
               "%s: logits are not aligned to their type", who);
@@ -1158,7 +1162,7 @@ extern "C" int eco_policy_grad(const eco_logits_t* logits, const int64_t* tokens
     return 0;
   });
   if (!ok) return eco_fail(ECO_ERR_LAUNCH, "eco_policy_grad: %s", cudaGetErrorString(cudaGetLastError()));
-  policy_finish_kernel<<<1, 1024, 0, s>>>(R, t, denom, counts, out);
+  policy_finish_kernel<<<1, one_cta(R.rows), 0, s>>>(R, t, denom, counts, out);
   return eco_launch_check("eco_policy_grad");
 }
 
@@ -1178,7 +1182,7 @@ extern "C" int eco_policy_forward(const eco_logits_t* logits, const int64_t* tok
   if (int rc = policy_of(P, old_logp, adv, ref_logp, low, high, kl_coef, denom, "eco_policy_forward")) return rc;
   ECO_REQUIRE(logp64 && row_stats && coef, ECO_ERR_ARG, "eco_policy_forward: null output");
   if (int rc = eco_token_logp(logits, tokens, mask, nullptr, 0, logp, logp64, row_stats, nullptr, stream)) return rc;
-  policy_tokens_kernel<<<1, 1024, 0, s>>>(R, P, logp64, coef, out);
+  policy_tokens_kernel<<<1, one_cta(R.rows), 0, s>>>(R, P, logp64, coef, out);
   return eco_launch_check("eco_policy_forward");
 }
 
@@ -1205,7 +1209,7 @@ extern "C" int eco_preference(const eco_logits_t* logits, const int64_t* tokens,
     if (int rc = eco_token_logp(logits, tokens, mask, cu_seqlens, 2 * pairs, nullptr, wide, row_stats, coef, stream))
       return rc;
   pair_kernel<<<(unsigned)pairs, 256, 0, s>>>(R, P, wide, coef, log_ratio, margin, wide + R.rows);
-  pair_finish_kernel<<<1, 256, 0, s>>>(wide + R.rows, pairs, denom, loss);
+  pair_finish_kernel<<<1, std::min(256u, one_cta(pairs)), 0, s>>>(wide + R.rows, pairs, denom, loss);
   if (int rc = eco_launch_check("eco_preference")) return rc;
   return grad ? eco_token_grad(logits, tokens, row_stats, coef, nullptr, gain, grad, stream) : ECO_OK;
 }

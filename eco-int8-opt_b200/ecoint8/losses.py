@@ -82,13 +82,13 @@ class _Rows:
         if shape[-1] == 0:
             raise AssertionError("an empty vocabulary")
         temperature = float(temperature)
-        if not (temperature > 0.0 and math.isfinite(temperature)):
-            raise ValueError("temperature must be positive")
+        if not 1e-15 <= temperature <= 1e15:
+            raise ValueError("temperature must be positive (and within [1e-15, 1e15])")
         if (dtype is torch.int8) != (s_out is not None):
             raise ValueError("int8 logits need their scale s_out, and only they have one")
         scale = 1.0 if s_out is None else float(s_out)
-        if not (scale > 0.0 and math.isfinite(scale)):
-            raise ValueError("s_out must be positive")
+        if not 1e-15 <= scale <= 1e15:
+            raise ValueError("s_out must be positive (and within [1e-15, 1e15])")
         self.x = x = logits if logits.stride(-1) == 1 or shape[-1] == 1 else logits.contiguous()
         self.gain = 1.0 / temperature
         self.rows = tokens.numel()
@@ -332,7 +332,7 @@ def preference_loss_grad(logits: torch.Tensor, tokens: torch.Tensor, ref_logp: t
 
     ``logits`` ``[2 pairs, length, vocab]``: the preferred sequences, then the rejected ones in
     the same order; or packed ``[rows, vocab]`` with ``cu_seqlens`` int32 ``[2 pairs + 1]`` on the
-    device (rows outside ``[cu_seqlens[0], cu_seqlens[-1])`` do not count; offsets beyond the rows
+    device, not decreasing (rows outside ``[cu_seqlens[0], cu_seqlens[-1])`` do not count; offsets beyond the rows
     are cut there).  ``ref_logp``: the reference's log-probability of each token
     (``token_logprobs``).  With ``D`` a sequence's sum over its counting rows of ``logp - ref_logp``
     (``average``: over their number; 0 for a sequence without any) and ``h = beta (D_preferred -

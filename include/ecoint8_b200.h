@@ -443,10 +443,10 @@ ECO_API int64_t eco_fp32_eco_scratch_len(const eco_fp32_layer_t* layers, int n_l
  * No counterpart in the reference, whose one objective is cross entropy (above).  Logits
  * [n0, n1, cols] with row strides s0, s1 (elements) and unit column stride; their rows are
  * numbered n1 * i0 + i1, and tokens, mask and every per-row array have n0 * n1 values in
- * that order.  x = raw * mul (1 / temperature; int8 logits: also their scale).  A row counts
- * when its mask byte is nonzero (mask nullable) and its token lies in [0, cols); other rows
- * are not read, have log-probability 0 and zeros as gradient.  At most 2^30 rows and 2^28
- * columns. */
+ * that order.  x = raw * mul (1 / temperature; int8 logits: also their scale), mul in [1e-30,
+ * 1e30].  A row counts when its mask byte is nonzero (mask nullable) and its token lies in
+ * [0, cols); other rows are not read, have log-probability 0 and zeros as gradient.  At most
+ * 2^30 rows and 2^28 columns. */
 enum { ECO_F32 = 0, ECO_BF16 = 1, ECO_F16 = 2, ECO_I8 = 3 };
 enum { ECO_PREFERENCE_SIGMOID = 0, ECO_PREFERENCE_HINGE = 1, ECO_PREFERENCE_IPO = 2 };
 
@@ -499,7 +499,7 @@ ECO_API int eco_policy_forward(const eco_logits_t* logits, const int64_t* tokens
 
 /* Preference loss over `pairs` pairs of sequences, the preferred ones first: sequence q has
  * rows [q seq_len, (q + 1) seq_len), or [cu_seqlens[q], cu_seqlens[q + 1]) where cu_seqlens
- * (int32 [2 pairs + 1]) is given.  D_q = sum over its counting rows of lp - ref (average: over
+ * (int32 [2 pairs + 1], not decreasing) is given.  D_q = sum over its counting rows of lp - ref (average: over
  * their number); h = beta (D_p - D_{p + pairs}).  sigmoid: -(1 - e) log s(h) - e log s(-h);
  * hinge: max(0, 1 - h); ipo: (h / beta - 1 / (2 beta))^2.
  * log_ratio [2 pairs] = D, margin [pairs] = h, loss: the losses' sum / denom.  row_stats [rows, 2]

@@ -519,6 +519,20 @@ def test_refusals():
         token_logprobs(x.cpu(), tokens.cpu())
 
 
+def test_factors_that_would_leave_the_range_of_fp32_are_refused():
+    from ecoint8.losses import token_logprobs
+
+    x, tokens, _, _ = _case(torch.float32, (6,), 50, 1)
+    for bad in (dict(temperature=1e-40), dict(temperature=1e40), dict(temperature=float("nan"))):
+        with pytest.raises(ValueError):
+            token_logprobs(x, tokens, **bad)
+    with pytest.raises(ValueError):
+        token_logprobs(x.to(torch.int8), tokens, s_out=1e30)
+    # at the border every row is still its maximum and nothing else
+    got = token_logprobs(x, x.argmax(1), temperature=1e-15)
+    assert (got == 0).all()
+
+
 # --------------------------------------------------------------------- as they are used
 
 
