@@ -357,7 +357,7 @@ ECO_DEV void put(const Terms& t, int64_t r, float loss, float kl, float clip) {
 }
 
 // ------------------------------------------------ rows held on the chip
-// Rows of up to kPieces vectors per thread stay in shared memory between the pass that sums
+// Rows of up to PIECES vectors per thread stay in shared memory between the pass that sums
 // them and the pass that writes their gradient.  A CTA walks down its rows; each thread copies
 // the vectors it will work on itself (cp.async, kRows rows' worth of places), so no barrier
 // belongs to the copies: while a row's sums are joined and its gradient is written, the next
@@ -368,9 +368,11 @@ ECO_DEV void put(const Terms& t, int64_t r, float loss, float kl, float clip) {
 // Vectors are counted from the 16-byte boundary at or before the row's start: the first and
 // last may hold neighbours' elements, which are read (they share 16 bytes with the row) and
 // left out.
-constexpr int kPieces = 8;  // vectors per thread and row
-constexpr int kRows = 3;    // rows in the ring
-constexpr int kHeld = 512;  // threads per SM that the ring has room for
+constexpr int kPieces = 8;                // vectors per thread and row, at most
+constexpr int kRows = 3;                  // rows in the ring
+constexpr int kHeldVecs = 256 * kPieces;  // of the widest rows
+// CTAs per SM that the ring (3 x 4096 vectors, 192 KB) has room for.
+constexpr int held_ctas(int nt, int pieces) { return 4096 / (nt * pieces); }
 
 struct RowOut {  // what a row leaves besides its gradient; all nullable
   float* logp;
@@ -414,13 +416,13 @@ struct Cursor {
   }
 };
 
-template <typename T, int NT, bool GRAD>
-__global__ void __launch_bounds__(NT, kHeld / NT)
+template <typename T, int NT, int PIECES, bool GRAD>
+__global__ void __launch_bounds__(NT, held_ctas(NT, PIECES))
     held_rows_kernel(const __grid_constant__ Rows R, const __grid_constant__ Policy P, const int* counts, float gain,
                      const __grid_constant__ RowOut O, const __grid_constant__ Grad G) {
   using GT = typename RowIo<T>::G;
   constexpr int E = RowIo<T>::E, W = NT / 32;
-  extern __shared__ __align__(16) uint4 ring[];  // [kRows][kPieces][NT]
+  extern __shared__ __align__(16) uint4 ring[];  // [kRows][PIECES][NT]
   __shared__ MaxSum warp_part[2][W];
   __shared__ Slope row_sh[2];
   __shared__ int counts_sh[W];
@@ -454,9 +456,9 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
       w.skew = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
       const uint4* src = reinterpret_cast<const uint4*>(x - w.skew) + tid;
       const int left = (w.skew + cols + E - 1) / E - tid;  // vectors from mine on
-      const uint32_t d = mine_s + slot * (kPieces * NT * 16);
+      const uint32_t d = mine_s + slot * (PIECES * NT * 16);
 #pragma unroll
-      for (int p = 0; p < kPieces; ++p)
+      for (int p = 0; p < PIECES; ++p)
         if (p * NT < left)
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + p * NT * 16), "l"(src + p * NT)
                        : "memory");
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
   auto sum = [&](int slot, Row w, float edge) {
     MaxSum a{-INFINITY, 0.0f};
     if (w.y < 0) return a;
-    const uint4* at = mine + slot * (kPieces * NT);
+    const uint4* at = mine + slot * (PIECES * NT);
     const int first = w.skew > 0, end = w.skew + cols, whole = end / E - tid;
     const int pieces = (end / E + NT - 1) / NT;
     auto group = [&](int q, auto n) {
@@ -496,7 +498,7 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
       take_vectors<T, false, N>(a, raw, in, R.c);
     };
 #pragma unroll
-    for (int q = 0; q < kPieces; q += 4) {
+    for (int q = 0; q < PIECES; q += 4) {
       // A vector of int8 is 16 terms a lane, so that a group of four with two in it is worth
       // shortening (100000 rows of 1000: 141 -> 98 us); one of four or eight terms is not.
       if (E == 16 && pieces - q == 1)
@@ -574,17 +576,17 @@ __global__ void __launch_bounds__(NT, kHeld / NT)
       // a row that does not count was not looked at: its gradient starts as its logits do
       const int skew = (int)((reinterpret_cast<uintptr_t>(g) / sizeof(GT)) & (E - 1));
       const bool zero = w0.y < 0 || c.coef == 0.0f;
-      const uint4* at = mine + slot * (kPieces * NT);
+      const uint4* at = mine + slot * (PIECES * NT);
       const int first = skew > 0, end = skew + cols, whole = end / E - tid;
       GT* gv = g - skew + tid * E;
       if (zero) {
         const float f[E] = {};
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p)
+        for (int p = 0; p < PIECES; ++p)
           if (p * NT < whole && p * NT + tid >= first) RowIo<T>::store(gv, p * NT, f);
       } else {
 #pragma unroll
-        for (int p = 0; p < kPieces; ++p)
+        for (int p = 0; p < PIECES; ++p)
           if (p * NT < whole && p * NT + tid >= first) store_slope<T, true>(gv, p * NT, at[p * NT], c);
       }
       if ((skew | cols % E) != 0) {
@@ -1011,22 +1013,25 @@ int by_type(int type, F f) {
   }
 }
 
-template <typename T, int NT, bool GRAD>
+template <typename T, int NT, int PIECES, bool GRAD>
 bool launch_held(const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O, const Grad& G,
                  cudaStream_t s) {
-  const auto kernel = held_rows_kernel<T, NT, GRAD>;
-  constexpr int smem = kRows * kPieces * NT * 16;
+  const auto kernel = held_rows_kernel<T, NT, PIECES, GRAD>;
+  constexpr int smem = kRows * PIECES * NT * 16;
   if (smem > 40 * 1024 &&
       cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return false;
-  const int64_t grid = std::min<int64_t>(R.rows, (int64_t)eco_num_sms() * (kHeld / NT));
+  const int64_t grid = std::min<int64_t>(R.rows, (int64_t)eco_num_sms() * held_ctas(NT, PIECES));
   kernel<<<(unsigned)grid, NT, smem, s>>>(R, P, counts, gain, O, G);
   return true;
 }
 
 // Threads per CTA by the vectors of a row (at whatever alignment it starts): as few as hold it,
-// so that a row's fixed work is shared by as many of its elements as possible.
-constexpr int64_t kHeldVecs = 256 * kPieces;
+// eight vectors each, so that a row's fixed work is shared by as many of its elements as
+// possible.  Rows that a warp holds in four each let twice as many warps be in work, which hides
+// that fixed work better (bf16 200000 x 1000: 355 -> 322 us; int8 100000 x 1000: 224 -> 190);
+// four each with twice the threads for wider rows lost to the barriers among them (bf16 32768 x
+// 8192: 278 -> 298).
 template <typename T>
 int64_t row_vecs(const Rows& R) {
   constexpr int64_t E = RowIo<T>::E;
@@ -1036,10 +1041,11 @@ int64_t row_vecs(const Rows& R) {
 template <typename T, bool GRAD>
 bool by_vecs(int64_t vecs, const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O,
              const Grad& G, cudaStream_t s) {
-  if (vecs <= 32 * kPieces) return launch_held<T, 32, GRAD>(R, P, counts, gain, O, G, s);
-  if (vecs <= 64 * kPieces) return launch_held<T, 64, GRAD>(R, P, counts, gain, O, G, s);
-  if (vecs <= 128 * kPieces) return launch_held<T, 128, GRAD>(R, P, counts, gain, O, G, s);
-  return launch_held<T, 256, GRAD>(R, P, counts, gain, O, G, s);
+  if (vecs <= 32 * 4) return launch_held<T, 32, 4, GRAD>(R, P, counts, gain, O, G, s);
+  if (vecs <= 32 * kPieces) return launch_held<T, 32, kPieces, GRAD>(R, P, counts, gain, O, G, s);
+  if (vecs <= 64 * kPieces) return launch_held<T, 64, kPieces, GRAD>(R, P, counts, gain, O, G, s);
+  if (vecs <= 128 * kPieces) return launch_held<T, 128, kPieces, GRAD>(R, P, counts, gain, O, G, s);
+  return launch_held<T, 256, kPieces, GRAD>(R, P, counts, gain, O, G, s);
 }
 
 template <typename T, int NT>
