@@ -497,13 +497,15 @@ __global__ void __launch_bounds__(NT, held_ctas(NT, PIECES))
       }
       take_vectors<T, false, N>(a, raw, in, R.c);
     };
+    constexpr bool kShort = E == 16 || PIECES == 4;
 #pragma unroll
     for (int q = 0; q < PIECES; q += 4) {
-      // A vector of int8 is 16 terms a lane, so that a group of four with two in it is worth
-      // shortening (100000 rows of 1000: 141 -> 98 us); one of four or eight terms is not.
-      if (E == 16 && pieces - q == 1)
+      // A group of four with one or two vectors in it is worth shortening where it is much of the
+      // row's work: int8, 16 terms a vector (100000 rows of 1000: 141 -> 98 us), and rows of a
+      // single group (bf16 400000 x 300: 296 -> 251); else it cost the full groups 3%.
+      if (kShort && pieces - q == 1)
         group(q, std::integral_constant<int, 1>());
-      else if (E == 16 && pieces - q == 2)
+      else if (kShort && pieces - q == 2)
         group(q, std::integral_constant<int, 2>());
       else if (pieces > q)
         group(q, std::integral_constant<int, 4>());
