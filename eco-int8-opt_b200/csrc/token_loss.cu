@@ -356,24 +356,7 @@ ECO_DEV void put(const Terms& t, int64_t r, float loss, float kl, float clip) {
   t.clip[r] = clip;
 }
 
-// ------------------------------------------------ rows held on the chip
-// Rows of up to PIECES vectors per thread stay in shared memory between the pass that sums
-// them and the pass that writes their gradient.  A CTA walks down its rows; each thread copies
-// the vectors it will work on itself (cp.async, kRows rows' worth of places), so no barrier
-// belongs to the copies: while a row's sums are joined and its gradient is written, the next
-// two rows are on their way.  Row i + 1 is summed before row i's gradient is written, so that
-// the scalar work of row i (logarithm, loss terms: one thread) runs behind it; one CTA barrier a
-// row.  A forward alone needs no place for a row once it is summed, and has three on their way.
-//
-// Vectors are counted from the 16-byte boundary at or before the row's start: the first and
-// last may hold neighbours' elements, which are read (they share 16 bytes with the row) and
-// left out.
-constexpr int kPieces = 8;                // vectors per thread and row, at most
-constexpr int kRows = 3;                  // rows in the ring
-constexpr int kHeldVecs = 256 * kPieces;  // of the widest rows
-// CTAs per SM that the ring (3 x 4096 vectors, 192 KB) has room for.
-constexpr int held_ctas(int nt, int pieces) { return 4096 / (nt * pieces); }
-
+// ------------------------------------------------ what a row leaves, and where rows lie
 struct RowOut {  // what a row leaves besides its gradient; all nullable
   float* logp;
   double* lp64;
@@ -416,20 +399,127 @@ struct Cursor {
   }
 };
 
-template <typename T, int NT, int PIECES, bool GRAD>
-__global__ void __launch_bounds__(NT, held_ctas(NT, PIECES))
+// ------------------------------------------------ rows on NT threads
+// Rows side by side in a CTA of 128 threads, or one row per CTA; as many CTAs per SM as registers
+// allow, which is what hides a row's fixed work (the joins; one thread's logarithm and loss
+// terms) and its loads' latency: nothing is copied ahead.  The gradient reads the row again, out
+// of L1 or L2, where the rows in work (148 SMs x 1024 threads x 16 vectors: 39 MB) stay.
+// Sixteen vectors per thread: with four or eight the fixed work is a larger share (bf16 65536 x
+// 4096, us by 4 / 8 / 16: forward 131 / 109 / 92, policy loss 313 / 276 / 248; a ring of copies
+// in shared memory, which leaves room for 16 warps only: 140 and 306).
+constexpr int rows_beside(int nt) { return nt == 32 ? 4 : 1; }
+constexpr int rows_ctas(int nt, bool grad) { return (grad ? 1024 : 1536) / (nt * rows_beside(nt)); }
+template <typename T, int NT, bool GRAD>
+__global__ void __launch_bounds__(NT * rows_beside(NT), rows_ctas(NT, GRAD))
+    row_kernel(const __grid_constant__ Rows R, const __grid_constant__ Policy P, const int* counts, float gain,
+               const __grid_constant__ RowOut O, const __grid_constant__ Grad G) {
+  using GT = typename RowIo<T>::G;
+  constexpr int E = RowIo<T>::E, W = NT / 32, BESIDE = rows_beside(NT);
+  __shared__ MaxSum sh[W];
+  __shared__ Slope row_sh[BESIDE];
+  __shared__ int counts_sh[W * BESIDE];
+  const int tid = threadIdx.x % NT, beside = threadIdx.x / NT, cols = (int)R.cols, rows = (int)R.rows;
+  const double inv_denom = GRAD ? 1.0 / policy_denom(R, P.denom, counts, counts_sh) : 1.0;
+  Cursor xc(R, (int)blockIdx.x * BESIDE + beside, (int)gridDim.x * BESIDE, R.s0, R.s1);
+  Cursor gc(R, (int)blockIdx.x * BESIDE + beside, (int)gridDim.x * BESIDE, GRAD ? G.s0 : R.s0, GRAD ? G.s1 : R.s1);
+  for (; xc.r < rows; xc.next(), gc.next()) {
+    const T* x = static_cast<const T*>(R.x) + xc.off;
+    const int y = R.counts(xc.r) ? (int)R.tokens[xc.r] : -1;
+    const RowSplit sp = RowIo<T>::split(x, cols);
+    const int vecs = (int)sp.vecs, edges = sp.head + sp.tail;
+    const uint4* body = reinterpret_cast<const uint4*>(x + sp.head);
+    float edge = -INFINITY, raw_y = 0.0f;
+    Given v{0.0f, 0.0f, 0.0f};
+    MaxSum a{-INFINITY, 0.0f};
+    if (y >= 0) {
+      if (tid < edges) edge = to_f32(x[sp.edge(tid, cols)]);
+      if (tid == 0) {
+        raw_y = to_f32(x[y]);
+        if (GRAD) v = given_of(P, xc.r);
+      }
+      take_run<T, 4, false>(a, body + tid, NT, run_length<NT>(vecs, tid), R.c);
+      if (tid < edges) {
+        const float f[1] = {edge};
+        take<1>(a, f, R.c);
+      }
+      a = lanes_join<32>(a, R.c);
+      if (W > 1) {
+        if ((tid & 31) == 0) sh[tid >> 5] = a;
+        __syncthreads();
+        if (tid < 32) a = lanes_join<W>(sh[tid % W], R.c);
+      }
+    }
+    if (tid == 0) {
+      double lp = 0.0;
+      float inv = 0.0f, off = 0.0f, coef = 0.0f;
+      Token t{0.0f, 0.0f, 0.0f, false};
+      if (y >= 0) {
+        lp = token_logp(raw_y, a, R.mul, W > 1 ? 2 : 1);
+        off = row_off(a.m);
+        inv = 1.0f / a.s;
+        if (GRAD) {
+          t = policy_token(P, v, lp);
+          coef = over(t.coef, inv_denom, gain);
+        }
+      }
+      if (GRAD) row_sh[beside] = slope_of(off, R.c.hi, coef * inv, coef);
+      row_out<GRAD>(O, xc.r, lp, make_float2(off, inv), t);
+    }
+    if (W > 1) __syncthreads(); else __syncwarp();  // row_sh; sh is free again
+    if constexpr (GRAD) {
+      const Slope c = row_sh[beside];
+      GT* g = static_cast<GT*>(G.g) + gc.off;
+      GT* gb = g + sp.head;
+      const bool zero = y < 0 || c.coef == 0.0f;
+      if (zero) {
+        const float f[E] = {};
+        for (int at = tid; at < vecs; at += NT) RowIo<T>::store(gb, at, f);
+      } else {
+        for (int at = tid; at < vecs; at += 4 * NT) {
+          uint4 raw[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (at + u * NT < vecs) raw[u] = __ldg(body + at + u * NT);
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (at + u * NT < vecs) store_slope<T, true>(gb, at + u * NT, raw[u], c);
+        }
+      }
+      if (tid < edges) {
+        const int j = (int)sp.edge(tid, cols);
+        g[j] = from_f32<GT>(zero ? 0.0f : slope_at(edge, c, j == y));
+      }
+      const int yv = y - sp.head;  // the token's element, by the thread that has written its vector
+      if (!zero && yv >= 0 && yv / E < vecs && yv / E % NT == tid) g[y] = from_f32<GT>(slope_at(to_f32(x[y]), c, true));
+      if (W == 1) __syncwarp();  // row_sh is free again
+    }
+  }
+}
+
+// ------------------------------------------------ short rows
+// The policy loss of rows that a warp holds in four vectors a lane: what counts is their fixed
+// work, and here a warp has its next two rows on their way (cp.async by the lane that will use
+// them, so no barrier belongs to the copies) while it does it (bf16 200000 x 1000: 322 us against
+// 364 by the kernel above, int8 100000 x 1000: 192 against 208; of the bandwidth of a copy 0.38
+// and 0.40).
+//
+// Vectors are counted from the 16-byte boundary at or before the row's start: the first and
+// last may hold neighbours' elements, which are read (they share 16 bytes with the row) and
+// left out.
+constexpr int kPieces = 4;  // vectors per lane
+constexpr int kRows = 3;    // rows in the ring
+
+template <typename T>
+__global__ void __launch_bounds__(32, 32)
     held_rows_kernel(const __grid_constant__ Rows R, const __grid_constant__ Policy P, const int* counts, float gain,
                      const __grid_constant__ RowOut O, const __grid_constant__ Grad G) {
   using GT = typename RowIo<T>::G;
-  constexpr int E = RowIo<T>::E, W = NT / 32;
-  extern __shared__ __align__(16) uint4 ring[];  // [kRows][PIECES][NT]
-  __shared__ MaxSum warp_part[2][W];
-  __shared__ Slope row_sh[2];
-  __shared__ int counts_sh[W];
-  const int tid = threadIdx.x, cols = (int)R.cols, rows = (int)R.rows, step = (int)gridDim.x;
-  const double inv_denom = GRAD ? 1.0 / policy_denom(R, P.denom, counts, counts_sh) : 1.0;
-  uint4* const mine = ring + tid;
-  const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
+  constexpr int E = RowIo<T>::E;
+  __shared__ uint4 ring[kRows][kPieces][32];
+  __shared__ Slope row_sh;
+  __shared__ int counts_sh[1];
+  const int lane = threadIdx.x, cols = (int)R.cols, rows = (int)R.rows, step = (int)gridDim.x;
+  const double inv_denom = 1.0 / policy_denom(R, P.denom, counts, counts_sh);
 
   // A row on its way: its token (-1: it does not count) and the element its first vector
   // starts at (0 .. E - 1 before the row).
@@ -454,14 +544,13 @@ __global__ void __launch_bounds__(NT, held_ctas(NT, PIECES))
       const T* x = static_cast<const T*>(R.x) + xc.off;
       w.y = (int)token;
       w.skew = (int)(reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
-      const uint4* src = reinterpret_cast<const uint4*>(x - w.skew) + tid;
-      const int left = (w.skew + cols + E - 1) / E - tid;  // vectors from mine on
-      const uint32_t d = mine_s + slot * (PIECES * NT * 16);
+      const uint4* src = reinterpret_cast<const uint4*>(x - w.skew) + lane;
+      const int left = (w.skew + cols + E - 1) / E - lane;  // vectors from mine on
+      const uint32_t d = (uint32_t)__cvta_generic_to_shared(&ring[slot][0][lane]);
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p)
-        if (p * NT < left)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + p * NT * 16), "l"(src + p * NT)
-                       : "memory");
+      for (int p = 0; p < kPieces; ++p)
+        if (p * 32 < left)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d + p * 512), "l"(src + p * 32) : "memory");
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
     xc.next();
@@ -469,185 +558,115 @@ __global__ void __launch_bounds__(NT, held_ctas(NT, PIECES))
     return w;
   };
   // The row's vectors [first, whole) lie within it.  The elements before and behind them (fewer
-  // than 2 E <= 32) go one to a lane of warp 0, which loads them from the row itself: worked on
-  // in their vectors, they would cost a lane E terms while the others wait.
+  // than 2 E <= 32) go one to a lane, which loads them from the row itself: worked on in their
+  // vectors, they would cost a lane E terms while the others wait.
   auto edge_index = [&](int skew) {
     const int end = skew + cols, head = skew > 0 ? min(E - skew, cols) : 0, tail = skew > 0 && end < E ? 0 : end % E;
-    return tid < head ? tid : tid < head + tail ? cols - tail + tid - head : -1;
-  };
-  auto edge_of = [&](const T* x, Row w) {
-    if (w.y < 0 || (w.skew | cols % E) == 0) return -INFINITY;
-    const int i = edge_index(w.skew);
-    return i >= 0 ? to_f32(x[i]) : -INFINITY;
+    return lane < head ? lane : lane < head + tail ? cols - tail + lane - head : -1;
   };
   auto sum = [&](int slot, Row w, float edge) {
     MaxSum a{-INFINITY, 0.0f};
     if (w.y < 0) return a;
-    const uint4* at = mine + slot * (PIECES * NT);
-    const int first = w.skew > 0, end = w.skew + cols, whole = end / E - tid;
-    const int pieces = (end / E + NT - 1) / NT;
-    auto group = [&](int q, auto n) {
+    const int first = w.skew > 0, end = w.skew + cols, whole = end / E - lane;
+    const int pieces = (end / E + 31) / 32;
+    auto group = [&](auto n) {  // a row of one or two pieces does not work on four
       constexpr int N = decltype(n)::value;
       uint4 raw[N];
       bool in[N];
 #pragma unroll
       for (int p = 0; p < N; ++p) {
-        in[p] = (q + p) * NT < whole && (q + p) * NT + tid >= first;
-        raw[p] = at[(q + p) * NT];
+        in[p] = p * 32 < whole && p * 32 + lane >= first;
+        raw[p] = ring[slot][p][lane];
       }
       take_vectors<T, false, N>(a, raw, in, R.c);
     };
-    constexpr bool kShort = E == 16 || PIECES == 4;
-#pragma unroll
-    for (int q = 0; q < PIECES; q += 4) {
-      // A group of four with one or two vectors in it is worth shortening where it is much of the
-      // row's work: int8, 16 terms a vector (100000 rows of 1000: 141 -> 98 us), and rows of a
-      // single group (bf16 400000 x 300: 296 -> 251); else it cost the full groups 3%.
-      if (kShort && pieces - q == 1)
-        group(q, std::integral_constant<int, 1>());
-      else if (kShort && pieces - q == 2)
-        group(q, std::integral_constant<int, 2>());
-      else if (pieces > q)
-        group(q, std::integral_constant<int, 4>());
-    }
-    if ((w.skew | cols % E) != 0 && tid < 32) {
+    if (pieces == 1) group(std::integral_constant<int, 1>());
+    else if (pieces == 2) group(std::integral_constant<int, 2>());
+    else if (pieces > 2) group(std::integral_constant<int, 4>());
+    if ((w.skew | cols % E) != 0) {
       const float f[1] = {edge};
       take<1>(a, f, R.c);
     }
     return a;
   };
-  // Warps' parts of a row to its scalars (warp 0): the row's results, and for the gradient what
-  // every thread needs.
-  auto finish = [&](int par, int r, int y, float raw_y, const Given& v) {
-    MaxSum a = warp_part[par][tid % W];
-    if (W > 1) a = lanes_join<W>(a, R.c);
-    if (tid == 0) {
-      double lp = 0.0;
-      float inv = 0.0f, off = 0.0f, coef = 0.0f;
-      Token t{0.0f, 0.0f, 0.0f, false};
-      if (y >= 0) {
-        lp = token_logp(raw_y, a, R.mul, W > 1 ? 2 : 1);
-        off = row_off(a.m);
-        inv = 1.0f / a.s;
-        if (GRAD) {
-          t = policy_token(P, v, lp);
-          coef = over(t.coef, inv_denom, gain);
-        }
-      }
-      if (GRAD) row_sh[par] = slope_of(off, R.c.hi, coef * inv, coef);
-      row_out<GRAD>(O, r, lp, make_float2(off, inv), t);
-    }
+  // What a row needs besides its vectors, loaded a row ahead.
+  struct Beside {
+    float raw_y, edge;
+    Given v;
   };
-  auto raw_token = [&](const T* x, int y) { return tid == 0 && y >= 0 ? to_f32(x[y]) : 0.0f; };
-  auto given = [&](int r, int y) {
-    return GRAD && tid == 0 && y >= 0 ? given_of(P, r) : Given{0.0f, 0.0f, 0.0f};
+  Cursor rc(R, blockIdx.x, step, R.s0, R.s1);
+  auto beside = [&](Row w) {
+    Beside b{0.0f, -INFINITY, Given{0.0f, 0.0f, 0.0f}};
+    if (rc.r < rows && w.y >= 0) {
+      const T* x = static_cast<const T*>(R.x) + rc.off;
+      if (lane == 0) {
+        b.raw_y = to_f32(x[w.y]);
+        b.v = given_of(P, rc.r);
+      }
+      const int i = (w.skew | cols % E) != 0 ? edge_index(w.skew) : -1;
+      if (i >= 0) b.edge = to_f32(x[i]);
+    }
+    rc.next();
+    return b;
   };
 
   look(blockIdx.x);
-  Cursor gc(R, blockIdx.x, step, GRAD ? G.s0 : R.s0, GRAD ? G.s1 : R.s1);  // the row in work
-  Cursor rc(R, blockIdx.x, step, R.s0, R.s1);                             // its logits, for the token's own
-  Row w0 = issue(0), w1 = issue(1), w2 = issue(2), w3{-1, 0};
-  float raw0 = raw_token(static_cast<const T*>(R.x) + rc.off, w0.y), raw1 = 0.0f;
-  float edge0 = edge_of(static_cast<const T*>(R.x) + rc.off, w0), edge1 = 0.0f;
-  Given v0 = given(rc.r, w0.y), v1{0.0f, 0.0f, 0.0f};
-  if (gc.r < rows) {
+  Cursor gc(R, blockIdx.x, step, G.s0, G.s1);  // the row in work
+  Row w0 = issue(0), w1 = issue(1), w2 = issue(2);
+  Beside b0 = beside(w0);
+  for (int slot = 0; gc.r < rows; gc.next()) {
+    const Beside b1 = beside(w1);
     asm volatile("cp.async.wait_group %0;" ::"n"(kRows - 1) : "memory");
-    const MaxSum a = lanes_join<32>(sum(0, w0, edge0), R.c);
-    if (!GRAD) w3 = issue(0);
-    if ((tid & 31) == 0) warp_part[0][tid >> 5] = a;
-    if (W > 1) __syncthreads(); else __syncwarp();
-  }
-  int slot = 0;
-  for (int par = 0; gc.r < rows; par ^= 1) {
-    const int slot1 = slot == kRows - 1 ? 0 : slot + 1;
-    if (tid < 32) finish(par, gc.r, w0.y, raw0, v0);
-    rc.next();
-    if (rc.r < rows) {
-      raw1 = raw_token(static_cast<const T*>(R.x) + rc.off, w1.y);
-      edge1 = edge_of(static_cast<const T*>(R.x) + rc.off, w1);
-      v1 = given(rc.r, w1.y);
-      asm volatile("cp.async.wait_group %0;" ::"n"(GRAD ? kRows - 2 : kRows - 1) : "memory");
-      const MaxSum a = lanes_join<32>(sum(slot1, w1, edge1), R.c);
-      if ((tid & 31) == 0) warp_part[par ^ 1][tid >> 5] = a;
+    const MaxSum a = lanes_join<32>(sum(slot, w0, b0.edge), R.c);
+    if (lane == 0) {
+      double lp = 0.0;
+      float inv = 0.0f, off = 0.0f, coef = 0.0f;
+      Token t{0.0f, 0.0f, 0.0f, false};
+      if (w0.y >= 0) {
+        lp = token_logp(b0.raw_y, a, R.mul, 1);
+        off = row_off(a.m);
+        inv = 1.0f / a.s;
+        t = policy_token(P, b0.v, lp);
+        coef = over(t.coef, inv_denom, gain);
+      }
+      row_sh = slope_of(off, R.c.hi, coef * inv, coef);
+      row_out<true>(O, gc.r, lp, make_float2(off, inv), t);
     }
-    if (W > 1) __syncthreads(); else __syncwarp();  // row i's scalars, row i + 1's warps
-    Row w4{-1, 0};
-    if (GRAD) {
-      const Slope c = row_sh[par];
-      GT* g = static_cast<GT*>(G.g) + gc.off;
-      // a row that does not count was not looked at: its gradient starts as its logits do
-      const int skew = (int)((reinterpret_cast<uintptr_t>(g) / sizeof(GT)) & (E - 1));
-      const bool zero = w0.y < 0 || c.coef == 0.0f;
-      const uint4* at = mine + slot * (PIECES * NT);
-      const int first = skew > 0, end = skew + cols, whole = end / E - tid;
-      GT* gv = g - skew + tid * E;
-      if (zero) {
-        const float f[E] = {};
+    __syncwarp();
+    const Slope c = row_sh;
+    GT* g = static_cast<GT*>(G.g) + gc.off;
+    // a row that does not count was not looked at: its gradient starts as its logits do
+    const int skew = (int)((reinterpret_cast<uintptr_t>(g) / sizeof(GT)) & (E - 1));
+    const bool zero = w0.y < 0 || c.coef == 0.0f;
+    const int first = skew > 0, end = skew + cols, whole = end / E - lane;
+    GT* gv = g - skew + lane * E;
+    if (zero) {
+      const float f[E] = {};
 #pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-          if (p * NT < whole && p * NT + tid >= first) RowIo<T>::store(gv, p * NT, f);
-      } else {
-#pragma unroll
-        for (int p = 0; p < PIECES; ++p)
-          if (p * NT < whole && p * NT + tid >= first) store_slope<T, true>(gv, p * NT, at[p * NT], c);
-      }
-      if ((skew | cols % E) != 0) {
-        const int i = edge_index(skew);
-        if (i >= 0) g[i] = from_f32<GT>(zero ? 0.0f : slope_at(edge0, c, i == w0.y));
-      }
-      const int yv = (w0.y + skew) / E;  // the token's element, by the thread that has written its vector
-      if (!zero && yv >= first && yv < end / E && yv % NT == tid) {
-        const float xy = to_f32(reinterpret_cast<const T*>(at + yv / NT * NT)[(w0.y + skew) % E]);
-        g[w0.y] = from_f32<GT>(slope_at(xy, c, true));
-      }
-      w3 = issue(slot);
+      for (int p = 0; p < kPieces; ++p)
+        if (p * 32 < whole && p * 32 + lane >= first) RowIo<T>::store(gv, p * 32, f);
     } else {
-      w4 = issue(slot1);
+#pragma unroll
+      for (int p = 0; p < kPieces; ++p)
+        if (p * 32 < whole && p * 32 + lane >= first) store_slope<T, true>(gv, p * 32, ring[slot][p][lane], c);
     }
-    slot = slot1;
-    gc.next();
-    w0 = w1, w1 = w2, w2 = w3, w3 = w4;
-    raw0 = raw1;
-    edge0 = edge1;
-    v0 = v1;
+    if ((skew | cols % E) != 0) {
+      const int i = edge_index(skew);
+      if (i >= 0) g[i] = from_f32<GT>(zero ? 0.0f : slope_at(b0.edge, c, i == w0.y));
+    }
+    const int yv = (w0.y + skew) / E;  // the token's element, by the lane that has written its vector
+    if (!zero && yv >= first && yv < end / E && yv % 32 == lane) {
+      const float xy = to_f32(reinterpret_cast<const T*>(&ring[slot][yv / 32][lane])[(w0.y + skew) % E]);
+      g[w0.y] = from_f32<GT>(slope_at(xy, c, true));
+    }
+    __syncwarp();  // row_sh is free again
+    w0 = w1, w1 = w2, w2 = issue(slot);
+    b0 = b1;
+    slot = slot == kRows - 1 ? 0 : slot + 1;
   }
 }
 
-// ------------------------------------------------ wider rows
-// The forward alone: one CTA per row.
-constexpr int kWide = 512;
-
-template <typename T>
-__global__ void __launch_bounds__(kWide, 3)
-    wide_logp_kernel(const __grid_constant__ Rows R, const __grid_constant__ RowOut O) {
-  __shared__ MaxSum sh[kWide / 32];
-  const int tid = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < R.rows; r += gridDim.x) {
-    double lp = 0.0;
-    float2 st = make_float2(0.0f, 0.0f);
-    if (R.counts(r)) {
-      const T* x = static_cast<const T*>(R.x) + R.at(r, R.s0, R.s1);
-      const float raw_y = tid == 0 ? to_f32(x[R.tokens[r]]) : 0.0f;
-      const RowSplit sp = RowIo<T>::split(x, R.cols);
-      const float f[1] = {tid < sp.head + sp.tail ? to_f32(x[sp.edge(tid, R.cols)]) : -INFINITY};
-      MaxSum a{-INFINITY, 0.0f};
-      take_run<T, 4, false>(a, reinterpret_cast<const uint4*>(x + sp.head) + tid, kWide,
-                            run_length<kWide>((int)sp.vecs, tid), R.c);
-      if (tid < sp.head + sp.tail) take<1>(a, f, R.c);
-      a = lanes_join<32>(a, R.c);
-      if ((tid & 31) == 0) sh[tid >> 5] = a;
-      __syncthreads();
-      if (tid < 32) a = lanes_join<kWide / 32>(sh[tid % (kWide / 32)], R.c);
-      if (tid == 0) {
-        lp = token_logp(raw_y, a, R.mul, 2);
-        st = make_float2(row_off(a.m), 1.0f / a.s);
-      }
-      __syncthreads();  // sh is free again
-    }
-    if (tid == 0) row_out<false>(O, r, lp, st, Token{});
-  }
-}
-
+// ------------------------------------------------ wide rows
 // The whole policy loss.  The first kPlaces vectors per thread of a row stay in shared memory, the
 // rest is read again for the gradient, from L2: the launch lets no more rows be in work than L2
 // holds the rests of.  As soon as a place has been used for the last time, the next row's vector
@@ -1015,39 +1034,35 @@ int by_type(int type, F f) {
   }
 }
 
-template <typename T, int NT, int PIECES, bool GRAD>
-bool launch_held(const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O, const Grad& G,
-                 cudaStream_t s) {
-  const auto kernel = held_rows_kernel<T, NT, PIECES, GRAD>;
-  constexpr int smem = kRows * PIECES * NT * 16;
-  if (smem > 40 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return false;
-  const int64_t grid = std::min<int64_t>(R.rows, (int64_t)eco_num_sms() * held_ctas(NT, PIECES));
-  kernel<<<(unsigned)grid, NT, smem, s>>>(R, P, counts, gain, O, G);
-  return true;
-}
-
-// Threads per CTA by the vectors of a row (at whatever alignment it starts): as few as hold it,
-// eight vectors each, so that a row's fixed work is shared by as many of its elements as
-// possible.  Rows that a warp holds in four each let twice as many warps be in work, which hides
-// that fixed work better (bf16 200000 x 1000: 355 -> 322 us; int8 100000 x 1000: 224 -> 190);
-// four each with twice the threads for wider rows lost to the barriers among them (bf16 32768 x
-// 8192: 278 -> 298).
+// Vectors of a row, at whatever alignment it starts.
 template <typename T>
 int64_t row_vecs(const Rows& R) {
   constexpr int64_t E = RowIo<T>::E;
   const bool on_16 = eco_aligned16(R.x) && (R.rows == R.n1 || R.s0 % E == 0) && (R.n1 <= 1 || R.s1 % E == 0);
   return (R.cols + (on_16 ? 0 : E - 1) + E - 1) / E;
 }
+
+template <typename T, int NT, bool GRAD>
+void launch_row(const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O, const Grad& G,
+                cudaStream_t s) {
+  const int64_t most = GRAD ? (int64_t)eco_num_sms() * rows_ctas(NT, GRAD) : 1 << 20;
+  const int64_t grid = std::min<int64_t>((R.rows + rows_beside(NT) - 1) / rows_beside(NT), most);
+  row_kernel<T, NT, GRAD><<<(unsigned)grid, NT * rows_beside(NT), 0, s>>>(R, P, counts, gain, O, G);
+}
+// Threads of a row by its vectors: one per sixteen of them (eight of int8 where a gradient of
+// four times their size is written: 32768 x 8192 254 us against 288), one per four where the rows
+// would otherwise leave most of the SMs' threads without work (bf16 1 to 148 rows of 8192: 2.6 to
+// 2.9 us against 3.6 to 3.9; 1500 rows: 7.7 against 7.2).
 template <typename T, bool GRAD>
-bool by_vecs(int64_t vecs, const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O,
+void by_rows(int64_t vecs, const Rows& R, const Policy& P, const int* counts, float gain, const RowOut& O,
              const Grad& G, cudaStream_t s) {
-  if (vecs <= 32 * 4) return launch_held<T, 32, 4, GRAD>(R, P, counts, gain, O, G, s);
-  if (vecs <= 32 * kPieces) return launch_held<T, 32, kPieces, GRAD>(R, P, counts, gain, O, G, s);
-  if (vecs <= 64 * kPieces) return launch_held<T, 64, kPieces, GRAD>(R, P, counts, gain, O, G, s);
-  if (vecs <= 128 * kPieces) return launch_held<T, 128, kPieces, GRAD>(R, P, counts, gain, O, G, s);
-  return launch_held<T, 256, kPieces, GRAD>(R, P, counts, gain, O, G, s);
+  int64_t per = GRAD && sizeof(T) == 1 ? 8 : 16;
+  if (R.rows * (vecs / per) < (int64_t)eco_num_sms() * 512) per = 4;
+  if (vecs <= 32 * per) launch_row<T, 32, GRAD>(R, P, counts, gain, O, G, s);
+  else if (vecs <= 64 * per) launch_row<T, 64, GRAD>(R, P, counts, gain, O, G, s);
+  else if (vecs <= 128 * per) launch_row<T, 128, GRAD>(R, P, counts, gain, O, G, s);
+  else if (vecs <= 256 * per) launch_row<T, 256, GRAD>(R, P, counts, gain, O, G, s);
+  else launch_row<T, 512, GRAD>(R, P, counts, gain, O, G, s);
 }
 
 template <typename T, int NT>
@@ -1060,6 +1075,9 @@ bool launch_wide(const Rows& R, const Policy& P, const int* counts, float gain, 
   kernel<<<(unsigned)grid, NT, smem, s>>>(R, P, counts, gain, O, G);
   return true;
 }
+// Wider rows than this (in vectors) go to the kernel that keeps their first part on the chip: bf16
+// 8192 x 32768, 4096 vectors, 247 us by either; 8192 x 131072 818 us against 960.
+constexpr int64_t kRowVecs = 4096;
 // Whether what the rows in work leave to L2 fits there: half of its 126 MB, since either die
 // keeps its own copy of what its SMs read.
 bool rests_fit(int64_t vecs, int threads) {
@@ -1093,18 +1111,12 @@ extern "C" int eco_token_logp(const eco_logits_t* logits, const int64_t* tokens,
   if (R.rows == 0) return ECO_OK;
   ECO_REQUIRE(logp || logp64, ECO_ERR_ARG, "eco_token_logp: no output");
   float2* st = reinterpret_cast<float2*>(row_stats);
-  bool ok = true;
   by_type(logits->type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    const int64_t vecs = row_vecs<T>(R);
     const RowOut O{logp, logp64, st, coef_zero, Terms{}};
-    if (vecs <= kHeldVecs)
-      ok = by_vecs<T, false>(vecs, R, Policy{}, nullptr, 0.0f, O, Grad{}, eco_stream(stream));
-    else
-      wide_logp_kernel<T><<<(unsigned)std::min<int64_t>(R.rows, 1 << 20), kWide, 0, eco_stream(stream)>>>(R, O);
+    by_rows<T, false>(row_vecs<T>(R), R, Policy{}, nullptr, 0.0f, O, Grad{}, eco_stream(stream));
     return 0;
   });
-  if (!ok) return eco_fail(ECO_ERR_LAUNCH, "eco_token_logp: %s", cudaGetErrorString(cudaGetLastError()));
   return eco_launch_check("eco_token_logp");
 }
 
@@ -1162,8 +1174,11 @@ extern "C" int eco_policy_grad(const eco_logits_t* logits, const int64_t* tokens
     using T = std::remove_pointer_t<decltype(p)>;
     const int64_t vecs = row_vecs<T>(R);
     const RowOut O{logp, nullptr, nullptr, nullptr, t};
-    if (vecs <= kHeldVecs)
-      ok = by_vecs<T, true>(vecs, R, P, counts, (float)gain, O, G, s);
+    if (vecs <= 32 * kPieces)
+      held_rows_kernel<T><<<(unsigned)std::min<int64_t>(R.rows, (int64_t)eco_num_sms() * 32), 32, 0, s>>>(
+          R, P, counts, (float)gain, O, G);
+    else if (vecs <= kRowVecs)
+      by_rows<T, true>(vecs, R, P, counts, (float)gain, O, G, s);
     else
       ok = rests_fit(vecs, 512) ? launch_wide<T, 512>(R, P, counts, (float)gain, O, G, s)
                                 : launch_wide<T, 1024>(R, P, counts, (float)gain, O, G, s);

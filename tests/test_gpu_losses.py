@@ -1,8 +1,10 @@
 """Objectives on token log-probabilities (``ecoint8.losses``) against the oracle in 64 bits.
 
-Tolerances.  With S the spread of a row's logits (over the temperature) and K the additions a
-thread makes in a row (at most cols / 32 up to 1024 columns, / 128 up to 8192, / 512 beyond, plus
-16 joins), the kernel's probabilities are off by the relative error
+Tolerances.  With S the spread of a row's logits (over the temperature) and K a bound of the
+longest chain of additions in a row's sum (a thread's vectors, at most 16 up to 4096 of them and
+one per 512 beyond; half a vector's terms, at most 8; at most 10 joins: below cols / 32 + 24 up to
+1024 columns, cols / 128 + 24 up to 8192, cols / 512 + 24 beyond), the kernel's probabilities are
+off by the relative error
 
     e = 2^-24 (6 S + K + 24):
 
