@@ -1089,7 +1089,9 @@ template <typename T>
 void launch_grad(const Rows& R, const float2* stats, const float* coef, const float* scale, float gain,
                  const Grad& G, cudaStream_t s) {
   const int64_t vecs = R.cols / RowIo<T>::E + 1;
-  if (R.cols <= 1024) {
+  // A warp per row of up to 512 vectors (bf16 65536 x 4096: 171 us, 0.96 of the bandwidth of a
+  // copy; a CTA of 256 threads per row, two vectors each: 213), 128 where there are few rows.
+  if (vecs <= (R.rows >= 8 * (int64_t)eco_num_sms() ? 513 : 129)) {
     const int64_t grid = std::min<int64_t>((R.rows + 7) / 8, 1 << 20);
     token_grad_kernel<T, 32><<<(unsigned)grid, 256, 0, s>>>(R, stats, coef, scale, gain, G, INT64_MAX / 2);
   } else {
