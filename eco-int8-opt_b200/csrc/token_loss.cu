@@ -235,16 +235,18 @@ struct Grad {
 // 0.1e-8; 2^0 is exact).  A thread's own terms come out right on average, but every part of the
 // sum that a join takes to a larger maximum goes through one such factor per join, and a sequence
 // adds up hundreds of rows: the log takes `joins` of them back, from all but the largest term.
-// Mean errors then lie within 1.3e-8 from 200 to 65536 columns (without: 5e-8 to 11e-8).
+// Mean errors then lie within 2e-8 from 200 to 65536 columns (without: 5e-8 to 11e-8).
 constexpr float kEx2Short = 5.0e-8f;
+// Joins over 32 lanes and W warps: of the warps' sums one stays as it is.
+constexpr float joins_of(int warps) { return 2.0f - 1.0f / (float)warps; }
 // The log is that of the mantissa in fp32 (below 0.35 in magnitude, so good to 2^-25) and the
 // exponent's in double: a thread does this once per row in front of a barrier, and the double
 // log's chain of dependent steps took longer than a row of a few thousand columns.
-ECO_DEV double token_logp(float raw_y, MaxSum a, double mul, int joins) {
+ECO_DEV double token_logp(float raw_y, MaxSum a, double mul, float joins) {
   const int bits = __float_as_int(a.s) - 0x3f3504f3;  // mantissa in [sqrt 1/2, sqrt 2)
   const int e = bits >> 23;
   const float f = a.s > 0.0f && a.s < INFINITY ? __int_as_float((bits & 0x007fffff) + 0x3f3504f3) : a.s;
-  const float small = logf(f) + kEx2Short * (float)joins * (1.0f - __fdividef(1.0f, a.s));
+  const float small = logf(f) + kEx2Short * joins * (1.0f - __fdividef(1.0f, a.s));
   const double whole = a.s > 0.0f && a.s < INFINITY ? (double)e * 0.69314718055994530942 : 0.0;
   return ((double)raw_y - (double)a.m) * mul - (whole + (double)small);
 }
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(NT * rows_beside(NT), rows_ctas(NT, GRAD))
       float inv = 0.0f, off = 0.0f, coef = 0.0f;
       Token t{0.0f, 0.0f, 0.0f, false};
       if (y >= 0) {
-        lp = token_logp(raw_y, a, R.mul, W > 1 ? 2 : 1);
+        lp = token_logp(raw_y, a, R.mul, joins_of(W));
         off = row_off(a.m);
         inv = 1.0f / a.s;
         if (GRAD) {
@@ -623,7 +625,7 @@ __global__ void __launch_bounds__(32, 32)
       float inv = 0.0f, off = 0.0f, coef = 0.0f;
       Token t{0.0f, 0.0f, 0.0f, false};
       if (w0.y >= 0) {
-        lp = token_logp(b0.raw_y, a, R.mul, 1);
+        lp = token_logp(b0.raw_y, a, R.mul, joins_of(1));
         off = row_off(a.m);
         inv = 1.0f / a.s;
         t = policy_token(P, b0.v, lp);
@@ -672,9 +674,9 @@ __global__ void __launch_bounds__(32, 32)
 // holds the rests of.  As soon as a place has been used for the last time, the next row's vector
 // is copied there (cp.async by the thread that will use it), so memory is read while the end of a
 // row is summed, joined and written.
-// One read and one write of bf16 8192 x 131072: 850 us, 0.77 of the bandwidth of a copy (fp32 4096
-// rows: 805, 0.81).  DRAM is busy for 0.85 of it (what L2 loses of the rests comes on top) and the
-// issue slots for 0.56 of it; two CTAs per SM take turns at reading and writing.
+// One read and one write of bf16 8192 x 131072: 815 us, 0.80 of the bandwidth of a copy (fp32 4096
+// rows: 810, 0.81).  Reads are 9% above the logits' size (what L2 loses of the rests), the issue
+// slots busy for 0.58 of the time; two CTAs per SM take turns at reading and writing.
 constexpr int kPlaces = 12;
 constexpr int kBatch = 4;  // vectors read again at a time
 
@@ -773,7 +775,7 @@ __global__ void __launch_bounds__(NT, 1024 / NT)
         float inv = 0.0f, off = 0.0f, coef = 0.0f;
         Token t{0.0f, 0.0f, 0.0f, false};
         if (w.y >= 0) {
-          lp = token_logp(raw_y, a, R.mul, 2);
+          lp = token_logp(raw_y, a, R.mul, joins_of(W));
           off = row_off(a.m);
           inv = 1.0f / a.s;
           t = policy_token(P, v, lp);
