@@ -444,12 +444,12 @@ __global__ void __launch_bounds__(NT * rows_beside(NT), rows_ctas(NT, GRAD))
         const float f[1] = {edge};
         take<1>(a, f, R.c);
       }
-      a = lanes_join<32>(a, R.c);
-      if (W > 1) {
-        if ((tid & 31) == 0) sh[tid >> 5] = a;
-        __syncthreads();
-        if (tid < 32) a = lanes_join<W>(sh[tid % W], R.c);
-      }
+    }
+    a = lanes_join<32>(a, R.c);
+    if (W > 1) {
+      if ((tid & 31) == 0) sh[tid >> 5] = a;
+      __syncthreads();  // for rows that do not count too: the last row's slope has been read by all
+      if (tid < 32) a = lanes_join<W>(sh[tid % W], R.c);
     }
     if (tid == 0) {
       double lp = 0.0;
