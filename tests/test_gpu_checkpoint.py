@@ -339,6 +339,28 @@ def test_graph_streams_and_same_bits():
     assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_backward_twice_and_of_two_calls_in_either_order():
+    """Each call keeps its own bytes: a backward may run twice, or after another call's."""
+    from ecoint8.checkpoint import gated_act_i8, rms_norm_i8
+
+    x, gen = _x(40, 516, torch.float32, 8)
+    x2, _ = _x(40, 516, torch.float32, 9)
+    w = torch.rand(516, generator=gen).cuda().requires_grad_()
+    a, b = x.requires_grad_(), x2.requires_grad_()
+    dy = torch.randn(40, 516, generator=gen).cuda()
+    ya, yb = rms_norm_i8(a, w), rms_norm_i8(b, w)
+    gb, ga = torch.autograd.grad(yb, (b, w), dy, retain_graph=True), torch.autograd.grad(ya, (a, w), dy,
+                                                                                        retain_graph=True)
+    again = torch.autograd.grad(ya, (a, w), dy)
+    assert all(torch.equal(u, v) for u, v in zip(ga, again))
+    both = torch.autograd.grad(rms_norm_i8(a, w), (a, w), dy), torch.autograd.grad(rms_norm_i8(b, w), (b, w), dy)
+    assert all(torch.equal(u, v) for u, v in zip(ga + gb, both[0] + both[1]))
+    za, zb = gated_act_i8(a), gated_act_i8(b)
+    (hb,), (ha,) = torch.autograd.grad(zb.sum(), b), torch.autograd.grad(za.sum(), a)
+    assert torch.equal(ha, torch.autograd.grad(gated_act_i8(a).sum(), a)[0])
+    assert torch.equal(hb, torch.autograd.grad(gated_act_i8(b).sum(), b)[0])
+
+
 def test_offsets_beyond_32_bits():
     from ecoint8.checkpoint import checkpoint_i8, gated_act_i8, restore_i8, rms_norm_i8
 

@@ -521,6 +521,36 @@ def test_refusals():
         token_logprobs(x.cpu(), tokens.cpu())
 
 
+def test_byte_masks_and_graphs_side_by_side():
+    """A uint8 mask counts where it is not zero; two captured calls replay on two streams at once."""
+    from ecoint8.losses import policy_loss_grad, preference_loss_grad
+
+    x, tokens, mask, gen = _case(torch.bfloat16, (400,), 9000, 2)
+    raw, x64 = _fp64(x)
+    old, adv, ref = _policy_inputs(x64, tokens, gen)
+    want = policy_loss_grad(x, tokens, old, adv, mask=mask)
+    got = policy_loss_grad(x, tokens, old, adv, mask=mask.to(torch.uint8) * 7)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    cu = torch.tensor([0, 90, 210, 333, 400], dtype=torch.int32).cuda()
+    calls = (lambda: policy_loss_grad(x, tokens, old, adv, mask=mask), lambda: preference_loss_grad(
+        x, tokens, ref, mask=mask, cu_seqlens=cu))
+    wants = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for c, st in zip(calls, streams):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=st):
+            outs.append(c())
+    for _ in range(5):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for w, o in zip(wants, outs):
+        assert all(torch.equal(a, b) for a, b in zip(w, o))
+
+
 def test_factors_that_would_leave_the_range_of_fp32_are_refused():
     from ecoint8.losses import token_logprobs
 
