@@ -46,7 +46,6 @@ template <typename T>
 struct RowIo {  // fp32, bf16, fp16
   static constexpr int E = 16 / (int)sizeof(T);
   using G = T;
-  using Raw = uint4;
   ECO_DEV static RowSplit split(const T* x, int64_t cols) {
     const int skew = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / (int)sizeof(T);
     RowSplit s;
@@ -55,9 +54,8 @@ struct RowIo {  // fp32, bf16, fp16
     s.tail = (int)(cols - s.head - s.vecs * E);
     return s;
   }
-  ECO_DEV static Raw load(const T* p, int64_t v) { return __ldg(reinterpret_cast<const uint4*>(p) + v); }
-  ECO_DEV static Raw load_last(const T* p, int64_t v) { return __ldcs(reinterpret_cast<const uint4*>(p) + v); }
-  ECO_DEV static void unpack(const Raw& r, float (&f)[E]) {
+  ECO_DEV static uint4 load_last(const T* p, int64_t v) { return __ldcs(reinterpret_cast<const uint4*>(p) + v); }
+  ECO_DEV static void unpack(const uint4& r, float (&f)[E]) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -73,7 +71,7 @@ struct RowIo {  // fp32, bf16, fp16
       }
     }
   }
-  ECO_DEV static float max(const Raw& r) {  // of the vector's numbers (NaN only if all are)
+  ECO_DEV static float max(const uint4& r) {  // of the vector's numbers (NaN only if all are)
     if constexpr (sizeof(T) == 4) {
       return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
     } else if constexpr (std::is_same_v<T, __nv_bfloat16>) {
@@ -109,7 +107,6 @@ template <>
 struct RowIo<int8_t> {
   static constexpr int E = 16;
   using G = float;
-  using Raw = uint4;
   ECO_DEV static RowSplit split(const int8_t* x, int64_t cols) {
     const int skew = (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15);
     RowSplit s;
@@ -118,16 +115,15 @@ struct RowIo<int8_t> {
     s.tail = (int)(cols - s.head - s.vecs * E);
     return s;
   }
-  ECO_DEV static Raw load(const int8_t* p, int64_t v) { return __ldg(reinterpret_cast<const uint4*>(p) + v); }
-  ECO_DEV static Raw load_last(const int8_t* p, int64_t v) { return __ldcs(reinterpret_cast<const uint4*>(p) + v); }
-  ECO_DEV static void unpack(const Raw& r, float (&f)[E]) {
+  ECO_DEV static uint4 load_last(const int8_t* p, int64_t v) { return __ldcs(reinterpret_cast<const uint4*>(p) + v); }
+  ECO_DEV static void unpack(const uint4& r, float (&f)[E]) {
     // byte + 128 in the low mantissa bits of 2^23, less 2^23 + 128
     const uint32_t w[4] = {r.x ^ 0x80808080u, r.y ^ 0x80808080u, r.z ^ 0x80808080u, r.w ^ 0x80808080u};
 #pragma unroll
     for (int i = 0; i < E; ++i)
       f[i] = __uint_as_float(__byte_perm(w[i / 4], 0x4B000000u, 0x7440u | (uint32_t)(i & 3))) - 8388736.0f;
   }
-  ECO_DEV static float max(const Raw& r) {
+  ECO_DEV static float max(const uint4& r) {
     const uint32_t m = __vmaxs4(__vmaxs4(r.x, r.y), __vmaxs4(r.z, r.w));
     return (float)::max(::max(sbyte(m, 0), sbyte(m, 1)), ::max(sbyte(m, 2), sbyte(m, 3)));
   }

@@ -13,9 +13,9 @@
 //
 // A row is one online pass (running max m and s = sum 2^((x - m) log2 e), rescaled when m
 // grows) and, for the gradient, one pass that writes -c/s 2^((x - m) log2 e) (+ c at y).
-// Sums are fp32 per thread over its share of the row and joined in a fixed order; the log
-// of the sum and the token's term are taken in double, once per row, because
-// exp(ref - lp) - (ref - lp) - 1 loses what fp32 loses twice over.
+// Sums are fp32 per thread over its share of the row and joined in a fixed order; the log of
+// the sum and the token's term meet in double, once per row, because exp(ref - lp) - (ref - lp)
+// - 1 loses what fp32 loses twice over.
 #include <algorithm>
 #include <cmath>
 
@@ -1102,7 +1102,7 @@ void launch_grad(const Rows& R, const float2* stats, const float* coef, const fl
     const int64_t grid = std::min<int64_t>((R.rows + 7) / 8, 1 << 20);
     token_grad_kernel<T, 32><<<(unsigned)grid, 256, 0, s>>>(R, stats, coef, scale, gain, G, INT64_MAX / 2);
   } else {
-    // segments of 2048 vectors (32 kBatch of logits), eight loads of each thread
+    // segments of 2048 vectors (32 KB of logits), eight loads of each thread
     const int64_t seg = 2048;
     const dim3 grid((unsigned)std::min<int64_t>(R.rows, 1 << 20), (unsigned)((vecs + seg - 1) / seg));
     token_grad_kernel<T, 256><<<grid, 256, 0, s>>>(R, stats, coef, scale, gain, G, seg);

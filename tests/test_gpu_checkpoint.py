@@ -271,7 +271,8 @@ def test_gated_activation(act, name, rows, cols, packed):
     tol = wu.abs() * (_half(dtype) + err(kg)) + low(kg) * d + extra
     assert ((du.double() - wu).abs() <= tol).all()
     # act' sums terms of either sign, each below 1 + |g|
-    tol = wg.abs() * _half(dtype) + d * ku.abs() * ((1 + kg.abs()) * err(kg) + (2.0 ** -22 if act == "gelu" else 0)) + extra
+    slope_err = (1 + kg.abs()) * err(kg) + (2.0 ** -22 if act == "gelu" else 0)
+    tol = wg.abs() * _half(dtype) + d * ku.abs() * slope_err + extra
     assert dg.dtype == dtype and ((dg.double() - wg).abs() <= tol).all()
 
 

@@ -123,7 +123,8 @@ def _logits_spec(**how):
 def test_token_objectives_refuse_bad_arguments():
     nat, lib = _lib()
     bad = [(dict(cols=0), -1, "shape"), (dict(n1=-1), -1, "shape"), (dict(type=9), -1, "type"),
-           (dict(mul=0.0), -1, "factor"), (dict(mul=1e31), -1, "factor"), (dict(mul=math.nan), -1, "factor"), (dict(x=4097), -2, "aligned"),
+           (dict(mul=0.0), -1, "factor"), (dict(mul=1e31), -1, "factor"),
+           (dict(mul=math.nan), -1, "factor"), (dict(x=4097), -2, "aligned"),
            (dict(x=None), -1, "null"), (dict(s1=-64), -1, "strides"), (dict(n0=1 << 20, n1=1 << 12), -1, "2^30 rows"),
            (dict(n1=(1 << 30) + 1), -1, "2^30 rows"),
            (dict(cols=(1 << 28) + 1), -1, "2^28")]
